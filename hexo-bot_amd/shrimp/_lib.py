@@ -136,6 +136,23 @@ class RaytapArgs(ctypes.Structure):
     ]
 
 
+class RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp),
+        ("q_sb", _i64), ("q_sh", _i64), ("q_sn", _i64),
+        ("k_sb", _i64), ("k_sh", _i64), ("k_sn", _i64),
+        ("pos", _vp), ("p_sb", _i64), ("p_sn", _i64), ("p_sa", _i64),
+        ("freqs", _vp), ("q_w", _vp), ("k_w", _vp), ("q_out", _vp), ("k_out", _vp),
+        ("gq", _vp), ("gk", _vp),
+        ("gq_sb", _i64), ("gq_sh", _i64), ("gq_sn", _i64),
+        ("gk_sb", _i64), ("gk_sh", _i64), ("gk_sn", _i64),
+        ("B", _i32), ("S", _i32), ("H", _i32), ("Hk", _i32), ("D", _i32),
+        ("axes", _i32), ("sections", _i32 * 4),
+        ("dt", _i32), ("pos_dt", _i32), ("freq_f64", _i32), ("w_dt", _i32),
+        ("interleaved", _i32), ("inverse", _i32), ("eps", _f32),
+    ]
+
+
 # Exported symbols and their ctypes signatures; tests check every one of them
 # against the header and the built library.
 SIGNATURES: dict = {
@@ -228,6 +245,11 @@ SIGNATURES: dict = {
     "shrimp_fill_tokens_f32": (
         ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, _vp, _i64, ctypes.c_int, _vp]
     ),
+    "shrimp_rope": (ctypes.c_int, [ctypes.POINTER(RopeArgs), _vp]),
+    "shrimp_qk_norm_rope_workspace": (_i64, [ctypes.POINTER(RopeArgs)]),
+    "shrimp_qk_norm_rope_backward": (
+        ctypes.c_int, [ctypes.POINTER(RopeArgs), _vp, _vp, _vp, _i64, _vp]
+    ),
 }
 
 _LIB = None
@@ -300,3 +322,15 @@ def stream_handle(device=None) -> int:
     import torch
 
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(fn, device, what: str, *args) -> None:
+    """fn(*args, current stream of `device`) with that device current, checked."""
+
+    import torch
+
+    if device.index in (None, torch.cuda.current_device()):
+        check(fn(*args, stream_handle(device)), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream_handle(device)), what)

@@ -570,3 +570,12 @@ def attn_pair(
 @attn_pair.register_fake
 def _attn_pair_fake(q, k, v, pair, table2, seq_lens):
     return q.new_empty(q.shape, dtype=torch.bfloat16)
+
+
+# ---- operators in modules of their own, under the same names here ---------------------------
+
+from .rotary import (  # noqa: E402,F401
+    qk_norm_rope,
+    qk_norm_rope_backward,
+    rope_axes,
+)

@@ -763,6 +763,57 @@ int shrimp_prep_csr_feats_f32(const void* node_feats, int nfeat, const int64_t* 
 int shrimp_fill_tokens_f32(const float* tokens, int n_tokens, int C, float* seq, int64_t seq_sb,
                            int B, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Rotary positions on several axes, with an RMS norm of every head before them
+ * when weights are given (shrimp::rope_axes, shrimp::qk_norm_rope; no
+ * counterpart in the reference, whose attention has a bias table instead).
+ *   q (B, H, S, D), k (B, Hk, S, D): element type dt (SHRIMP_DT_BF16 / F16 /
+ *     F32), strides *_sb / *_sh / *_sn in elements, the last one 1; H or Hk may
+ *     be 0. D <= 256.
+ *   pos (B, S, axes) int32, int64 or fp32 (pos_dt), strides p_sb / p_sn / p_sa
+ *     (0 broadcasts); sections[i] pairs turn by axis i, P = their sum, 2 P <= D;
+ *     freqs (P,) fp32, or fp64 with freq_f64: angle = pos * freq, in fp64.
+ *   pair p: dimensions (p, P + p), or (2 p, 2 p + 1) with interleaved; the rest
+ *     of the head passes. inverse turns the other way.
+ *   q_w, k_w (D,) of type w_dt, both or neither: x / sqrt(mean x^2 + eps) * w
+ *     before the rotation, eps > 0.
+ *   q_out, k_out: contiguous (B, H, S, D) and (B, Hk, S, D) of type dt.
+ * The backward entry takes the gradients gq, gk of q_out and k_out (type dt,
+ * their own strides) and the inputs; q_out and k_out receive the gradients of q
+ * and k, dw_q and dw_k (D,) of type w_dt those of the weights, summed in a fixed
+ * order. Its workspace: at least shrimp_qk_norm_rope_workspace(a) bytes (-1 for
+ * arguments it refuses), 4-byte aligned, used only during the call's launches.
+ * ---------------------------------------------------------------------- */
+#define SHRIMP_ROPE_MAX_AXES 4
+
+typedef struct {
+  const void* q;
+  const void* k;
+  int64_t q_sb, q_sh, q_sn;
+  int64_t k_sb, k_sh, k_sn;
+  const void* pos;
+  int64_t p_sb, p_sn, p_sa;
+  const void* freqs;
+  const void* q_w;
+  const void* k_w;
+  void* q_out;
+  void* k_out;
+  const void* gq;
+  const void* gk;
+  int64_t gq_sb, gq_sh, gq_sn;
+  int64_t gk_sb, gk_sh, gk_sn;
+  int32_t B, S, H, Hk, D;
+  int32_t axes, sections[SHRIMP_ROPE_MAX_AXES];
+  int32_t dt, pos_dt, freq_f64, w_dt;
+  int32_t interleaved, inverse;
+  float eps;
+} shrimp_rope_args;
+
+int shrimp_rope(const shrimp_rope_args* a, void* stream);
+int64_t shrimp_qk_norm_rope_workspace(const shrimp_rope_args* a);
+int shrimp_qk_norm_rope_backward(const shrimp_rope_args* a, void* dw_q, void* dw_k,
+                                 void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
