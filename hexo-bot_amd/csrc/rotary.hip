@@ -26,7 +26,10 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int MAX_AXES = SHRIMP_ROPE_MAX_AXES;
 constexpr int MAX_D = 256;
-constexpr int FLIGHT = 4;  // head groups loaded together
+// Elements of an access: 8 bytes of 16-bit elements beat 16, whose units need twice
+// the registers (backward of 512 boards' q and k, 16 heads of 16: 75 against 112 us;
+// 2 x 8190 x 40 heads of 128: 125 against 143).
+constexpr int VEC = 4;
 
 struct RopeTensor {
   const void* x;
@@ -44,18 +47,17 @@ struct RopeParams {
   const void* freqs;
   int64_t p_sb, p_sn, p_sa;
   int pos_dt, freq_f64, w_dt;
-  int cut[MAX_AXES - 1];  // pair at which axis i + 1 begins
-  float eps, sign;
+  int axes, cut[MAX_AXES - 1];  // pair at which axis i + 1 begins
+  float eps, sign, inv_d;
   int tokens, S, D, P;
   int lanes, head_lanes;  // lanes per head, heads across lanes
-  int groups_per_block;
+  int groups_per_block;   // head groups (of q, then of k) per blockIdx.y
+  int q_rows;             // backward: blockIdx.y below takes q alone, the others k alone
   int interleaved;
 };
 
 template <typename T, int V>
-struct alignas(V * sizeof(T)) Vec {
-  T e[V];
-};
+using Vec = T __attribute__((ext_vector_type(V)));
 
 SHRIMP_DEV float load_weight(const void* w, int dt, int i) {
   if (dt == SHRIMP_DT_F32) return static_cast<const float*>(w)[i];
@@ -97,9 +99,11 @@ SHRIMP_DEV float lanes_sum(float v, int lanes) {
   return v;
 }
 
-template <typename T, int V, bool NORM, bool BACK>
+// F: groups of heads loaded together, while the F before them are worked on.
+template <typename T, int V, int F, bool NORM, bool BACK>
 __global__ __launch_bounds__(THREADS) void rope_kernel(const RopeParams p) {
   constexpr int NU = V == 1 ? 2 : 1;  // units per lane: 128 units of one pair at D = 256
+  __shared__ float shared[THREADS * 2 * V];  // angles, then the block's weight gradients
   const int tid = threadIdx.x;
   const int per_token = p.lanes * p.head_lanes;
   const int ul = tid & (p.lanes - 1);
@@ -107,95 +111,157 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(const RopeParams p) {
   const int per_block = THREADS / per_token;
   const int rot_units = p.P / V;
 
-  // the unit's two accesses and what they hold: 2 = both V elements rotate, else
-  // elements that pass (0: none; an odd rest ends in one element, V = 1 only)
-  int off0[NU], off1[NU], n0[NU], n1[NU];
-  bool rot[NU];
+  // the unit's two accesses; they rotate into each other (rot) or pass. An odd
+  // rest ends in one element (V = 1 only), and lanes past the units hold none.
+  int off0[NU], off1[NU];
+  bool n0[NU], n1[NU], rot[NU];
 #pragma unroll
   for (int i = 0; i < NU; ++i) {
     const int u = ul + i * 64;
     rot[i] = u < rot_units;
-    if (rot[i]) {
-      off0[i] = p.interleaved ? 2 * u * V : u * V;
-      off1[i] = p.interleaved ? off0[i] + V : p.P + u * V;
-      n0[i] = n1[i] = 1;
-    } else {
-      off0[i] = 2 * p.P + (u - rot_units) * 2 * V;
-      off1[i] = off0[i] + V;
-      n0[i] = off0[i] + V <= p.D;
-      n1[i] = off1[i] + V <= p.D;
-    }
+    off0[i] = rot[i] ? (p.interleaved ? 2 * u * V : u * V) : 2 * p.P + (u - rot_units) * 2 * V;
+    off1[i] = rot[i] && !p.interleaved ? p.P + u * V : off0[i] + V;
+    n0[i] = off0[i] + V <= p.D;
+    n1[i] = off1[i] + V <= p.D;
   }
-  float wgt[2][NU][2 * V];
-  float dw[2][NU][2 * V];
+
+  const int q_groups = p.t[0].groups;
+  // forward: a block's heads may be of q and of k, and share their angles; backward:
+  // of one tensor, whose weight and its gradient take the registers of one
+  constexpr int NT = BACK ? 1 : 2;
+  const int of_k = BACK && (int)blockIdx.y >= p.q_rows;
+  const int first = of_k ? q_groups + (blockIdx.y - p.q_rows) * p.groups_per_block
+                         : blockIdx.y * p.groups_per_block;
+  const int last = min(first + p.groups_per_block,
+                       BACK && !of_k ? q_groups : q_groups + p.t[1].groups);
+  const int64_t stride = (int64_t)gridDim.x * per_block;
+  struct Place {  // one token: its rows' offsets in q and k, and its position
+    int64_t x[NT], g[NT];
+    int b, s;
+    Vec<double, MAX_AXES> at;  // (an array would be indexed in memory)
+    bool live;
+  };
+  auto locate = [&](int64_t tok) {
+    Place w{};
+    w.live = tok < p.tokens;
+    const int i = w.live ? (int)tok : 0;
+    w.b = i / p.S;
+    w.s = i - w.b * p.S;
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      const RopeTensor& t = p.t[BACK ? of_k : k];
+      w.x[k] = w.b * t.x_sb + w.s * t.x_sn;
+      if constexpr (BACK) w.g[k] = w.b * t.g_sb + w.s * t.g_sn;
+    }
+#pragma unroll
+    for (int a = 0; a < MAX_AXES; ++a)
+      w.at[a] = a < p.axes && p.P > 0
+                    ? load_pos(p.pos, p.pos_dt, w.b * p.p_sb + w.s * p.p_sn + a * p.p_sa) : 0.0;
+    return w;
+  };
+  struct Rows {
+    Vec<T, V> x[F][NU][2], g[BACK ? F : 1][NU][2];
+  };
+  auto load = [&](int64_t xq, int64_t xk, int64_t gx, bool live, int g0, Rows& v) {
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      const bool k = BACK ? of_k : g0 + f >= q_groups;
+      const RopeTensor& t = p.t[k];
+      const int head = (g0 + f - (k ? q_groups : 0)) * p.head_lanes + hl;
+      const bool on = live && g0 + f < last && head < t.heads;
+      const T* x = static_cast<const T*>(t.x) + (k ? xk : xq) + head * t.x_sh;
+      const T* g = static_cast<const T*>(t.g) + gx + head * t.g_sh;
+      const Vec<T, V> zero = (T)0.f;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        v.x[f][i][0] = on && n0[i] ? *reinterpret_cast<const Vec<T, V>*>(x + off0[i]) : zero;
+        v.x[f][i][1] = on && n1[i] ? *reinterpret_cast<const Vec<T, V>*>(x + off1[i]) : zero;
+        if constexpr (BACK) {
+          v.g[f][i][0] = on && n0[i] ? *reinterpret_cast<const Vec<T, V>*>(g + off0[i]) : zero;
+          v.g[f][i][1] = on && n1[i] ? *reinterpret_cast<const Vec<T, V>*>(g + off1[i]) : zero;
+        }
+      }
+    }
+  };
+
+  int64_t base = (int64_t)blockIdx.x * per_block;
+  Place now = locate(base + tid / per_token);
+  Rows rows;
+  load(now.x[0], now.x[NT - 1], now.g[0], now.live, first, rows);
+  float wgt[NT][NU][2 * V], dw[NU][2 * V];
   if constexpr (NORM) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < NT; ++k)
 #pragma unroll
       for (int i = 0; i < NU; ++i)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          wgt[k][i][e] = p.t[k].w && n0[i] ? load_weight(p.t[k].w, p.w_dt, off0[i] + e) : 0.f;
-          wgt[k][i][V + e] = p.t[k].w && n1[i] ? load_weight(p.t[k].w, p.w_dt, off1[i] + e) : 0.f;
-          dw[k][i][e] = dw[k][i][V + e] = 0.f;
+          const void* w = p.t[BACK ? of_k : k].w;
+          wgt[k][i][e] = w && n0[i] ? load_weight(w, p.w_dt, off0[i] + e) : 0.f;
+          wgt[k][i][V + e] = w && n1[i] ? load_weight(w, p.w_dt, off1[i] + e) : 0.f;
+          dw[i][e] = dw[i][V + e] = 0.f;
         }
   }
 
-  const int first = blockIdx.y * p.groups_per_block;
-  const int last = min(first + p.groups_per_block, p.t[0].groups + p.t[1].groups);
-  for (int64_t base = (int64_t)blockIdx.x * per_block; base < p.tokens;
-       base += (int64_t)gridDim.x * per_block) {
-    const int64_t tok = base + tid / per_token;
-    const bool live = tok < p.tokens;
-    const int b = live ? (int)tok / p.S : 0, s = live ? (int)tok - b * p.S : 0;
-    float cs[NU][V], sn[NU][V];
+  for (; base < p.tokens; base += stride) {
+    auto angle = [&](int pair, float& c, float& s) {
+      double at = now.at[0];
 #pragma unroll
-    for (int i = 0; i < NU; ++i)
+      for (int a = 1; a < MAX_AXES; ++a) at = pair >= p.cut[a - 1] ? now.at[a] : at;
+      const double f = p.freq_f64 ? static_cast<const double*>(p.freqs)[pair]
+                                  : (double)static_cast<const float*>(p.freqs)[pair];
+      cos_sin(at * f, c, s);
+      s *= p.sign;
+    };
+    float cs[NU][V], sn[NU][V];
+    if (p.head_lanes == 1) {
+#pragma unroll
+      for (int i = 0; i < NU; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          cs[i][e] = 1.f;
+          sn[i][e] = 0.f;
+          if (rot[i]) angle((ul + i * 64) * V + e, cs[i][e], sn[i][e]);
+        }
+    } else {
+      // the lanes that hold a token's unit for several heads, all of one wave,
+      // share its angles out
+      const int slot = (tid / per_token * p.lanes + ul) * 2 * V;
+      for (int e = hl; e < V; e += p.head_lanes) {
+        float c = 1.f, s = 0.f;
+        if (rot[0]) angle(ul * V + e, c, s);
+        shared[slot + e] = c;
+        shared[slot + V + e] = s;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        cs[i][e] = 1.f;
-        sn[i][e] = 0.f;
-        if (rot[i]) {
-          const int pair = (ul + i * 64) * V + e;
-          int axis = 0;
-#pragma unroll
-          for (int a = 0; a < MAX_AXES - 1; ++a) axis += pair >= p.cut[a];
-          const double f = p.freq_f64 ? static_cast<const double*>(p.freqs)[pair]
-                                      : (double)static_cast<const float*>(p.freqs)[pair];
-          const double at = load_pos(p.pos, p.pos_dt, b * p.p_sb + s * p.p_sn + axis * p.p_sa);
-          cos_sin(at * f, cs[i][e], sn[i][e]);
-          sn[i][e] *= p.sign;
+        cs[0][e] = shared[slot + e];
+        sn[0][e] = shared[slot + V + e];
+        if constexpr (NU == 2) {  // more than one head: at most 32 units
+          cs[1][e] = 1.f;
+          sn[1][e] = 0.f;
         }
       }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    const Place next = locate(base + stride + tid / per_token);
 
-    for (int g0 = first; g0 < last; g0 += FLIGHT) {
-      Vec<T, V> xv[FLIGHT][NU][2];
-      Vec<T, V> gv[BACK ? FLIGHT : 1][NU][2];
+    for (int g0 = first; g0 < last; g0 += F) {
+      const Rows cur = rows;
+      const bool end = g0 + F >= last;
+      load(end ? next.x[0] : now.x[0], end ? next.x[NT - 1] : now.x[NT - 1],
+           end ? next.g[0] : now.g[0], end ? next.live : now.live, end ? first : g0 + F, rows);
 #pragma unroll
-      for (int f = 0; f < FLIGHT; ++f) {
-        const int g = g0 + f, k = g >= p.t[0].groups;
+      for (int f = 0; f < F; ++f) {
+        if (g0 + f >= last) break;
+        const bool k = BACK ? of_k : g0 + f >= q_groups;
         const RopeTensor& t = p.t[k];
-        const int head = (g - (k ? p.t[0].groups : 0)) * p.head_lanes + hl;
-        const bool on = live && g < last && head < t.heads;
-        const T* x = static_cast<const T*>(t.x) + b * t.x_sb + head * t.x_sh + s * t.x_sn;
-        const T* gr = BACK ? static_cast<const T*>(t.g) + b * t.g_sb + head * t.g_sh + s * t.g_sn : nullptr;
-#pragma unroll
-        for (int i = 0; i < NU; ++i) {
-          xv[f][i][0] = on && n0[i] ? *reinterpret_cast<const Vec<T, V>*>(x + off0[i]) : Vec<T, V>{};
-          xv[f][i][1] = on && n1[i] ? *reinterpret_cast<const Vec<T, V>*>(x + off1[i]) : Vec<T, V>{};
-          if constexpr (BACK) {
-            gv[f][i][0] = on && n0[i] ? *reinterpret_cast<const Vec<T, V>*>(gr + off0[i]) : Vec<T, V>{};
-            gv[f][i][1] = on && n1[i] ? *reinterpret_cast<const Vec<T, V>*>(gr + off1[i]) : Vec<T, V>{};
-          }
-        }
-      }
-#pragma unroll
-      for (int f = 0; f < FLIGHT; ++f) {
-        const int g = g0 + f, k = g >= p.t[0].groups;
-        if (g >= last) break;
-        const RopeTensor& t = p.t[k];
-        const int head = (g - (k ? p.t[0].groups : 0)) * p.head_lanes + hl;
-        const bool on = live && head < t.heads;
+        const int head = (g0 + f - (k ? q_groups : 0)) * p.head_lanes + hl;
         float y[NU][2 * V];  // what is rotated: x, x r w, or the gradient
         float r = 1.f;
         if constexpr (NORM) {
@@ -204,66 +270,65 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(const RopeParams p) {
           for (int i = 0; i < NU; ++i)
 #pragma unroll
             for (int e = 0; e < 2 * V; ++e) {
-              const float v = (float)xv[f][i][e / V].e[e % V];
+              const float v = (float)cur.x[f][i][e / V][e % V];
               ss = fmaf(v, v, ss);
             }
-          r = rsqrtf(lanes_sum(ss, p.lanes) / (float)p.D + p.eps);
+          r = rsqrtf(fmaf(lanes_sum(ss, p.lanes), p.inv_d, p.eps));
         }
 #pragma unroll
         for (int i = 0; i < NU; ++i)
 #pragma unroll
           for (int e = 0; e < 2 * V; ++e) {
-            const float v = BACK ? (float)gv[f][i][e / V].e[e % V] : (float)xv[f][i][e / V].e[e % V];
-            y[i][e] = NORM && !BACK ? v * r * (k ? wgt[1][i][e] : wgt[0][i][e]) : v;
+            if constexpr (BACK)
+              y[i][e] = (float)cur.g[f][i][e / V][e % V];
+            else
+              y[i][e] = (float)cur.x[f][i][e / V][e % V];
+            if constexpr (NORM && !BACK) y[i][e] *= r * (k ? wgt[NT - 1][i][e] : wgt[0][i][e]);
           }
-        // rotation; the gradient's is the inverse, the sign of the sines says which
+        // the gradient's rotation is the inverse; the sign of the sines says which
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
           if (!rot[i]) continue;
+          auto turn = [&](float& a, float& c, int e) {
+            const float a0 = a, c0 = c;
+            a = a0 * cs[i][e] - c0 * sn[i][e];
+            c = c0 * cs[i][e] + a0 * sn[i][e];
+          };
+          if (p.interleaved) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            if (p.interleaved) {
-              const float a = y[i][2 * e], c = y[i][2 * e + 1];
-              y[i][2 * e] = a * cs[i][e] - c * sn[i][e];
-              y[i][2 * e + 1] = c * cs[i][e] + a * sn[i][e];
-            } else {
-              const float a = y[i][e], c = y[i][V + e];
-              y[i][e] = a * cs[i][e] - c * sn[i][e];
-              y[i][V + e] = c * cs[i][e] + a * sn[i][e];
-            }
+            for (int e = 0; e < V; ++e) turn(y[i][2 * e], y[i][2 * e + 1], e);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) turn(y[i][e], y[i][V + e], e);
           }
         }
-        if constexpr (NORM && BACK) {
+        if constexpr (BACK) {
           float dot = 0.f;
 #pragma unroll
           for (int i = 0; i < NU; ++i)
 #pragma unroll
             for (int e = 0; e < 2 * V; ++e) {
-              const float v = (float)xv[f][i][e / V].e[e % V];
-              const float d = y[i][e] * v * r;
-              if (k)
-                dw[1][i][e] += d;
-              else
-                dw[0][i][e] += d;
-              y[i][e] *= k ? wgt[1][i][e] : wgt[0][i][e];
+              const float v = (float)cur.x[f][i][e / V][e % V];
+              dw[i][e] = fmaf(y[i][e], v * r, dw[i][e]);
+              y[i][e] *= wgt[0][i][e];
               dot = fmaf(y[i][e], v, dot);
             }
-          const float q = lanes_sum(dot, p.lanes) / (float)p.D * r * r;
+          const float q = lanes_sum(dot, p.lanes) * p.inv_d * r * r;
 #pragma unroll
           for (int i = 0; i < NU; ++i)
 #pragma unroll
             for (int e = 0; e < 2 * V; ++e)
-              y[i][e] = r * (y[i][e] - (float)xv[f][i][e / V].e[e % V] * q);
+              y[i][e] = r * (y[i][e] - (float)cur.x[f][i][e / V][e % V] * q);
         }
-        if (on) {
-          T* o = static_cast<T*>(t.out) + (((int64_t)b * t.heads + head) * p.S + s) * p.D;
+        if (now.live && head < t.heads) {
+          T* o = static_cast<T*>(t.out) + (((int64_t)now.b * t.heads + head) * p.S + now.s) * p.D;
 #pragma unroll
           for (int i = 0; i < NU; ++i) {
             Vec<T, V> o0, o1;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-              o0.e[e] = (T)y[i][e];
-              o1.e[e] = (T)y[i][V + e];
+              o0[e] = (T)y[i][e];
+              o1[e] = (T)y[i][V + e];
             }
             if (n0[i]) *reinterpret_cast<Vec<T, V>*>(o + off0[i]) = o0;
             if (n1[i]) *reinterpret_cast<Vec<T, V>*>(o + off1[i]) = o1;
@@ -271,32 +336,27 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(const RopeParams p) {
         }
       }
     }
+    now = next;
   }
 
-  if constexpr (NORM && BACK) {
+  if constexpr (BACK) {
     // the block's weight gradients: threads of one unit added in thread order
-    __shared__ float acc[THREADS * 2 * V];
-    const int block = blockIdx.y * gridDim.x + blockIdx.x;
+    const int block = (blockIdx.y - (of_k ? p.q_rows : 0)) * gridDim.x + blockIdx.x;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (p.t[k].part == nullptr) continue;
+    for (int i = 0; i < NU; ++i) {
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NU; ++i) {
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 2 * V; ++e) acc[e * THREADS + tid] = dw[k][i][e];
-        __syncthreads();
-        for (int j = tid; j < p.lanes * 2 * V; j += THREADS) {
-          const int e = j / p.lanes, l = j % p.lanes, u = l + i * 64;
-          const int o0 = u < rot_units ? (p.interleaved ? 2 * u * V : u * V)
-                                       : 2 * p.P + (u - rot_units) * 2 * V;
-          const int o1 = u < rot_units && !p.interleaved ? p.P + u * V : o0 + V;
-          const int d = e < V ? o0 + e : o1 + e - V;
-          if (d >= p.D) continue;
-          float sum = 0.f;
-          for (int t = l; t < THREADS; t += p.lanes) sum += acc[e * THREADS + t];
-          p.t[k].part[(int64_t)block * p.D + d] = sum;
-        }
+      for (int e = 0; e < 2 * V; ++e) shared[e * THREADS + tid] = dw[i][e];
+      __syncthreads();
+      for (int j = tid; j < p.lanes * 2 * V; j += THREADS) {
+        const int e = j / p.lanes, l = j % p.lanes, u = l + i * 64;
+        const bool r = u < rot_units;
+        const int o0 = r ? (p.interleaved ? 2 * u * V : u * V) : 2 * p.P + (u - rot_units) * 2 * V;
+        const int d = e < V ? o0 + e : (r && !p.interleaved ? p.P + u * V : o0 + V) + e - V;
+        if (d >= p.D) continue;
+        float sum = 0.f;
+        for (int t = l; t < THREADS; t += p.lanes) sum += shared[e * THREADS + t];
+        p.t[of_k].part[(int64_t)block * p.D + d] = sum;
       }
     }
   }
@@ -305,10 +365,11 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(const RopeParams p) {
 // Weight gradients from the blocks' partial sums, in float64 and in block order:
 // workgroup (column block, tensor), 16 columns x 16 interleaved runs of blocks.
 __global__ __launch_bounds__(THREADS) void rope_dw_kernel(const float* part_q, const float* part_k,
-                                                          int blocks, int D, void* dw_q, void* dw_k,
-                                                          int dt) {
+                                                          int blocks_q, int blocks_k, int D,
+                                                          void* dw_q, void* dw_k, int dt) {
   __shared__ double acc[16][17];
   const float* part = blockIdx.y ? part_k : part_q;
+  const int blocks = blockIdx.y ? blocks_k : blocks_q;
   void* dw = blockIdx.y ? dw_k : dw_q;
   const int c = threadIdx.x & 15, run = threadIdx.x >> 4, d = blockIdx.x * 16 + c;
   double sum = 0.0;
@@ -339,15 +400,13 @@ int pow2_ceil(int n) {
 
 struct RopePlan {
   RopeParams p;
-  int vec, grid_x, grid_y;
+  int vec, flight, grid_x, grid_y;
 };
 
-// Blocks of a backward launch: enough for four workgroups on every compute unit, few
-// enough that their partial weight gradients (4 D bytes each) stay a small read.
-constexpr int BACK_BLOCKS = 1024;
-// Forward blocks below which a token's heads are spread over more blocks: eight
-// workgroups per compute unit.
-constexpr int FULL_BLOCKS = 2048;
+// Blocks of a launch per tensor: enough to fill the compute units, each with several
+// tokens whose reads are in flight under the token before (and, backward, few enough
+// that their partial weight gradients, 4 D bytes each, stay a small read).
+constexpr int FULL_BLOCKS = 1024;
 
 int plan_rope(const shrimp_rope_args* a, bool back, RopePlan* out, const char* what) {
   SHRIMP_REQUIRE(a != nullptr, "%s: null arguments", what);
@@ -385,7 +444,7 @@ int plan_rope(const shrimp_rope_args* a, bool back, RopePlan* out, const char* w
   }
 
   const int es = element_size(a->dt);
-  // widest access that divides the sections, the rest and every address
+  // wide accesses divide the sections, the rest and every address
   const int rest = a->D - 2 * (int)pairs;
   auto fits = [&](int v) {
     if (pairs % v || rest % (2 * v)) return false;
@@ -398,7 +457,7 @@ int plan_rope(const shrimp_rope_args* a, bool back, RopePlan* out, const char* w
            (!back || (ok(a->gq, a->gq_sb, a->gq_sh, a->gq_sn) &&
                       ok(a->gk, a->gk_sb, a->gk_sh, a->gk_sn)));
   };
-  out->vec = es == 2 && fits(8) ? 8 : fits(4) ? 4 : 1;
+  out->vec = fits(VEC) ? VEC : 1;
 
   RopeParams& p = out->p;
   p = RopeParams{};
@@ -414,6 +473,7 @@ int plan_rope(const shrimp_rope_args* a, bool back, RopePlan* out, const char* w
   p.pos_dt = a->pos_dt;
   p.freq_f64 = a->freq_f64;
   p.w_dt = a->w_dt;
+  p.axes = a->axes;
   int cut = 0;
   for (int i = 0; i < MAX_AXES - 1; ++i) {
     cut += i < a->axes ? a->sections[i] : 0;
@@ -424,6 +484,7 @@ int plan_rope(const shrimp_rope_args* a, bool back, RopePlan* out, const char* w
   p.tokens = a->B * a->S;
   p.S = a->S;
   p.D = a->D;
+  p.inv_d = 1.f / (float)a->D;
   p.P = (int)pairs;
   p.interleaved = a->interleaved != 0;
   const int units = (int)pairs / out->vec + (rest + 2 * out->vec - 1) / (2 * out->vec);
@@ -435,42 +496,42 @@ int plan_rope(const shrimp_rope_args* a, bool back, RopePlan* out, const char* w
   if (sh < sn)
     while (p.head_lanes * a->D * es < 256 && p.head_lanes < heads && p.head_lanes * p.lanes < 64)
       p.head_lanes *= 2;
+  const int per_block = THREADS / (p.lanes * p.head_lanes);
+  const int64_t blocks = ((int64_t)p.tokens + per_block - 1) / per_block;
+  const int64_t full = FULL_BLOCKS;
+  out->grid_x = (int)(blocks > full ? full : blocks);
   p.t[0].groups = (a->H + p.head_lanes - 1) / p.head_lanes;
   p.t[1].groups = (a->Hk + p.head_lanes - 1) / p.head_lanes;
   const int groups = p.t[0].groups + p.t[1].groups;
-  const int per_block = THREADS / (p.lanes * p.head_lanes);
-  const int64_t blocks = ((int64_t)p.tokens + per_block - 1) / per_block;
-  const int full = back ? BACK_BLOCKS : FULL_BLOCKS;
-  int gy = 1;
-  if (blocks > 0 && groups > 0) {
-    gy = (int)((full + blocks - 1) / blocks);
-    if (gy > groups) gy = groups;
-  }
-  p.groups_per_block = groups > 0 ? (groups + gy - 1) / gy : 0;
-  out->grid_y = groups > 0 ? (groups + p.groups_per_block - 1) / p.groups_per_block : 0;
-  out->grid_x = (int)(back && blocks > BACK_BLOCKS ? BACK_BLOCKS : blocks);
+  int split = 1;
+  if (blocks > 0 && blocks < full) split = (int)((full + blocks - 1) / blocks);
+  if (split > groups) split = groups;
+  p.groups_per_block = groups > 0 ? (groups + split - 1) / split : 0;
+  auto rows = [&](int n) { return n > 0 ? (n + p.groups_per_block - 1) / p.groups_per_block : 0; };
+  p.q_rows = rows(p.t[0].groups);
+  out->grid_y = back ? p.q_rows + rows(p.t[1].groups) : rows(groups);
+  out->flight = p.groups_per_block > 1 && !back ? 2 : 1;
   return SHRIMP_OK;
 }
 
 template <typename T, int V, bool NORM, bool BACK>
 void launch(const RopePlan& pl, hipStream_t st) {
-  hipLaunchKernelGGL((rope_kernel<T, V, NORM, BACK>), dim3(pl.grid_x, pl.grid_y), dim3(THREADS), 0,
-                     st, pl.p);
+  const dim3 grid(pl.grid_x, pl.grid_y), block(THREADS);
+  if (pl.flight == 1)
+    hipLaunchKernelGGL((rope_kernel<T, V, 1, NORM, BACK>), grid, block, 0, st, pl.p);
+  else
+    hipLaunchKernelGGL((rope_kernel<T, V, BACK ? 1 : 2, NORM, BACK>), grid, block, 0, st, pl.p);
 }
 
 template <bool NORM, bool BACK>
 void launch_any(const RopePlan& pl, int dt, hipStream_t st) {
-  if (dt == SHRIMP_DT_F32) {
-    pl.vec == 4 ? launch<float, 4, NORM, BACK>(pl, st) : launch<float, 1, NORM, BACK>(pl, st);
-  } else if (dt == SHRIMP_DT_F16) {
-    pl.vec == 8   ? launch<_Float16, 8, NORM, BACK>(pl, st)
-    : pl.vec == 4 ? launch<_Float16, 4, NORM, BACK>(pl, st)
-                  : launch<_Float16, 1, NORM, BACK>(pl, st);
-  } else {
-    pl.vec == 8   ? launch<__bf16, 8, NORM, BACK>(pl, st)
-    : pl.vec == 4 ? launch<__bf16, 4, NORM, BACK>(pl, st)
-                  : launch<__bf16, 1, NORM, BACK>(pl, st);
-  }
+  const bool wide = pl.vec == VEC;
+  if (dt == SHRIMP_DT_F32)
+    wide ? launch<float, VEC, NORM, BACK>(pl, st) : launch<float, 1, NORM, BACK>(pl, st);
+  else if (dt == SHRIMP_DT_F16)
+    wide ? launch<_Float16, VEC, NORM, BACK>(pl, st) : launch<_Float16, 1, NORM, BACK>(pl, st);
+  else
+    wide ? launch<__bf16, VEC, NORM, BACK>(pl, st) : launch<__bf16, 1, NORM, BACK>(pl, st);
 }
 
 }  // namespace
@@ -493,7 +554,7 @@ extern "C" int64_t shrimp_qk_norm_rope_workspace(const shrimp_rope_args* a) {
   using namespace shrimp;
   RopePlan pl;
   if (plan_rope(a, true, &pl, "qk_norm_rope_workspace") != SHRIMP_OK) return -1;
-  return (int64_t)2 * pl.grid_x * pl.grid_y * a->D * 4;
+  return (int64_t)pl.grid_x * pl.grid_y * a->D * 4;
 }
 
 extern "C" int shrimp_qk_norm_rope_backward(const shrimp_rope_args* a, void* dw_q, void* dw_k,
@@ -503,19 +564,19 @@ extern "C" int shrimp_qk_norm_rope_backward(const shrimp_rope_args* a, void* dw_
   const int rc = plan_rope(a, true, &pl, "qk_norm_rope_backward");
   if (rc != SHRIMP_OK) return rc;
   SHRIMP_REQUIRE(dw_q && dw_k, "qk_norm_rope_backward: null weight gradient");
-  const int blocks = pl.grid_x * pl.grid_y;
-  const int64_t part = (int64_t)blocks * a->D;
-  SHRIMP_REQUIRE(blocks == 0 || (workspace && workspace_bytes >= 2 * part * 4),
+  const int blocks[2] = {pl.grid_x * pl.p.q_rows, pl.grid_x * (pl.grid_y - pl.p.q_rows)};
+  const int64_t need = (int64_t)(blocks[0] + blocks[1]) * a->D * 4;
+  SHRIMP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                  "qk_norm_rope_backward: workspace of %lld bytes, %lld needed",
-                 (long long)workspace_bytes, (long long)(2 * part * 4));
+                 (long long)workspace_bytes, (long long)need);
   pl.p.t[0].part = static_cast<float*>(workspace);
-  pl.p.t[1].part = blocks ? static_cast<float*>(workspace) + part : nullptr;
-  if (blocks > 0) {
+  pl.p.t[1].part = need ? static_cast<float*>(workspace) + (int64_t)blocks[0] * a->D : nullptr;
+  if (need > 0) {
     launch_any<true, true>(pl, a->dt, as_stream(stream));
     const int e = check_launch("qk_norm_rope_backward");
     if (e != SHRIMP_OK) return e;
   }
   hipLaunchKernelGGL(rope_dw_kernel, dim3((a->D + 15) / 16, 2), dim3(THREADS), 0, as_stream(stream),
-                     pl.p.t[0].part, pl.p.t[1].part, blocks, a->D, dw_q, dw_k, a->w_dt);
+                     pl.p.t[0].part, pl.p.t[1].part, blocks[0], blocks[1], a->D, dw_q, dw_k, a->w_dt);
   return check_launch("qk_norm_rope_backward");
 }

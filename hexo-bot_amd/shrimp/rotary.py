@@ -21,6 +21,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
+from ._oplib import below, define
 
 MAX_AXES = 4
 MAX_HEAD_DIM = 256
@@ -127,15 +128,36 @@ def _args(what, q, k, pos, freqs, sections, interleaved, inverse, eps=0.0, q_w=N
 # ---- rope_axes -----------------------------------------------------------------------------
 
 
-@torch.library.custom_op("shrimp::rope_axes", mutates_args=())
-def rope_axes(
-    x: torch.Tensor,
-    pos: torch.Tensor,
-    freqs: torch.Tensor,
-    sections: Sequence[int],
-    interleaved: bool = False,
-    inverse: bool = False,
-) -> torch.Tensor:
+def _rope_kernel(x, pos, freqs, sections, interleaved=False, inverse=False):
+    a, out, _, keep = _args("shrimp::rope_axes", x, None, pos, freqs, sections, interleaved, inverse)
+    _lib.launch(_lib.load().shrimp_rope, x.device, "shrimp::rope_axes", ctypes.byref(a))
+    del keep
+    return out
+
+
+def _rope_fake(x, pos, freqs, sections, interleaved=False, inverse=False):
+    return x.new_empty(x.shape)
+
+
+class _RopeAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, pos, freqs, sections, interleaved, inverse):
+        ctx.save_for_backward(pos, freqs)
+        ctx.turn = (sections, interleaved, not inverse)
+        return below(_rope_axes, x, pos, freqs, sections, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, g):
+        return _rope_axes(g, *ctx.saved_tensors, *ctx.turn), None, None, None, None, None
+
+
+_rope_axes = define(
+    "rope_axes(Tensor x, Tensor pos, Tensor freqs, int[] sections, bool interleaved, bool inverse)"
+    " -> Tensor", _rope_kernel, _rope_fake, _RopeAxes)
+
+
+def rope_axes(x: torch.Tensor, pos: torch.Tensor, freqs: torch.Tensor, sections: Sequence[int],
+              interleaved: bool = False, inverse: bool = False) -> torch.Tensor:
     """x (B, H, S, D) with the first 2 P dimensions of every head turned in P = sum(sections)
     pairs: pair p by pos[b, s, axis] * freqs[p], the first sections[0] pairs by axis 0, and
     so on. A pair is dimensions (p, P + p), or (2 p, 2 p + 1) with ``interleaved``; further
@@ -143,50 +165,13 @@ def rope_axes(
     float32; freqs (P,) float32 or float64. Angles are formed in float64. ``inverse`` turns
     back."""
 
-    a, out, _, keep = _args("shrimp::rope_axes", x, None, pos, freqs, sections, interleaved, inverse)
-    _lib.launch(_lib.load().shrimp_rope, x.device, "shrimp::rope_axes", ctypes.byref(a))
-    del keep
-    return out
-
-
-@rope_axes.register_fake
-def _rope_axes_fake(x, pos, freqs, sections, interleaved=False, inverse=False):
-    return x.new_empty(x.shape)
-
-
-def _rope_setup(ctx, inputs, output):
-    _, pos, freqs, ctx.sections, ctx.interleaved, ctx.inverse = inputs
-    ctx.save_for_backward(pos, freqs)
-
-
-def _rope_backward(ctx, g):
-    pos, freqs = ctx.saved_tensors
-    gx = rope_axes(g, pos, freqs, ctx.sections, ctx.interleaved, not ctx.inverse)
-    return gx, None, None, None, None, None
-
-
-rope_axes.register_autograd(_rope_backward, setup_context=_rope_setup)
+    return _rope_axes(x, pos, freqs, sections, interleaved, inverse)
 
 
 # ---- qk_norm_rope --------------------------------------------------------------------------
 
 
-@torch.library.custom_op("shrimp::qk_norm_rope", mutates_args=())
-def qk_norm_rope(
-    q: torch.Tensor,
-    k: torch.Tensor,
-    q_weight: torch.Tensor,
-    k_weight: torch.Tensor,
-    pos: torch.Tensor,
-    freqs: torch.Tensor,
-    sections: Sequence[int],
-    eps: float = 1e-6,
-    interleaved: bool = False,
-) -> Tuple[torch.Tensor, torch.Tensor]:
-    """x / sqrt(mean(x^2) + eps) * weight over the dimensions of every head of q (B, H, S, D)
-    and k (B, Hk, S, D), then rope_axes, in one launch with fp32 statistics. Weights (D,) of
-    one type (bfloat16, float16 or float32)."""
-
+def _norm_kernel(q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved):
     what = "shrimp::qk_norm_rope"
     a, q_out, k_out, keep = _args(what, q, k, pos, freqs, sections, interleaved, False, eps,
                                   q_weight, k_weight)
@@ -195,28 +180,41 @@ def qk_norm_rope(
     return q_out, k_out
 
 
-@qk_norm_rope.register_fake
-def _qk_norm_rope_fake(q, k, q_weight, k_weight, pos, freqs, sections, eps=1e-6, interleaved=False):
+def _norm_fake(q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved):
     return q.new_empty(q.shape), k.new_empty(k.shape)
 
 
-@torch.library.custom_op("shrimp::qk_norm_rope_backward", mutates_args=())
-def qk_norm_rope_backward(
-    gq: torch.Tensor,
-    gk: torch.Tensor,
-    q: torch.Tensor,
-    k: torch.Tensor,
-    q_weight: torch.Tensor,
-    k_weight: torch.Tensor,
-    pos: torch.Tensor,
-    freqs: torch.Tensor,
-    sections: Sequence[int],
-    eps: float = 1e-6,
-    interleaved: bool = False,
-) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Gradients of q, k, q_weight and k_weight from those of qk_norm_rope's results. The
-    weights' sums have a fixed order, so the same call gives the same bits."""
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved):
+        ctx.save_for_backward(q, k, q_weight, k_weight, pos, freqs)
+        ctx.rest = (sections, eps, interleaved)
+        return below(_qk_norm_rope, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved)
 
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        grads = _qk_norm_rope_backward(gq, gk, *ctx.saved_tensors, *ctx.rest)
+        return (*grads, None, None, None, None, None)
+
+
+_qk_norm_rope = define(
+    "qk_norm_rope(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor pos, Tensor freqs,"
+    " int[] sections, float eps, bool interleaved) -> (Tensor, Tensor)",
+    _norm_kernel, _norm_fake, _QkNormRope)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                 pos: torch.Tensor, freqs: torch.Tensor, sections: Sequence[int], eps: float = 1e-6,
+                 interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x / sqrt(mean(x^2) + eps) * weight over the dimensions of every head of q (B, H, S, D)
+    and k (B, Hk, S, D), then rope_axes, in one launch with fp32 statistics. Weights (D,) of
+    one type (bfloat16, float16 or float32)."""
+
+    return _qk_norm_rope(q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved)
+
+
+def _norm_back_kernel(gq, gk, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved):
     what = "shrimp::qk_norm_rope_backward"
     a, dq, dk, keep = _args(what, q, k, pos, freqs, sections, interleaved, False, eps, q_weight,
                             k_weight, gq, gk)
@@ -230,22 +228,24 @@ def qk_norm_rope_backward(
     return dq, dk, dqw, dkw
 
 
-@qk_norm_rope_backward.register_fake
-def _qk_norm_rope_backward_fake(gq, gk, q, k, q_weight, k_weight, pos, freqs, sections, eps=1e-6,
-                                interleaved=False):
+def _norm_back_fake(gq, gk, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved):
     return (q.new_empty(q.shape), k.new_empty(k.shape), q_weight.new_empty(q_weight.shape),
             k_weight.new_empty(k_weight.shape))
 
 
-def _norm_setup(ctx, inputs, output):
-    ctx.save_for_backward(*inputs[:6])
-    ctx.sections, ctx.eps, ctx.interleaved = inputs[6:]
+_qk_norm_rope_backward = define(
+    "qk_norm_rope_backward(Tensor gq, Tensor gk, Tensor q, Tensor k, Tensor q_weight,"
+    " Tensor k_weight, Tensor pos, Tensor freqs, int[] sections, float eps, bool interleaved)"
+    " -> (Tensor, Tensor, Tensor, Tensor)", _norm_back_kernel, _norm_back_fake)
 
 
-def _norm_backward(ctx, gq, gk):
-    q, k, qw, kw, pos, freqs = ctx.saved_tensors
-    return (*qk_norm_rope_backward(gq, gk, q, k, qw, kw, pos, freqs, ctx.sections, ctx.eps,
-                                   ctx.interleaved), None, None, None, None, None)
+def qk_norm_rope_backward(
+    gq: torch.Tensor, gk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
+    k_weight: torch.Tensor, pos: torch.Tensor, freqs: torch.Tensor, sections: Sequence[int],
+    eps: float = 1e-6, interleaved: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of q, k, q_weight and k_weight from those of qk_norm_rope's results. The
+    weights' sums have a fixed order, so the same call gives the same bits."""
 
-
-qk_norm_rope.register_autograd(_norm_backward, setup_context=_norm_setup)
+    return _qk_norm_rope_backward(gq, gk, q, k, q_weight, k_weight, pos, freqs, sections, eps,
+                                  interleaved)

@@ -318,3 +318,16 @@ def test_refused_on_the_device():
             ops.qk_norm_rope(**{**ok, **bad})
     with pytest.raises(ValueError):
         ops.qk_norm_rope_backward(x, x[:, :1], **ok)
+
+
+def test_no_second_derivative_and_no_grad():
+    x = torch.randn(1, 2, 3, 16, device=DEV, requires_grad=True)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    pos, freqs = torch.ones(3, 1, dtype=torch.int32, device=DEV), _freqs([8])
+    with torch.no_grad():
+        q, k = ops.qk_norm_rope(x, x, w, w, pos, freqs, [8])
+    assert not q.requires_grad and not k.requires_grad
+    q, k = ops.qk_norm_rope(x, x, w, w, pos, freqs, [8])
+    (gx,) = torch.autograd.grad(q.square().sum() + k.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):  # refused, not silently zero
+        torch.autograd.grad(gx.sum(), x)
