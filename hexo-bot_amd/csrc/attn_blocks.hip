@@ -1,0 +1,547 @@
+// Attention of every query over its own blocks of keys.
+//
+//   out[b, h, i] = sum_j p_j v_j,  p = softmax_j(q . k_j / sqrt(d)),  j over the keys
+//   below k_lens[b] of the blocks that sel[b, h / G, i] names (each once);
+//   lse[b, h, i] = log sum_j exp(q . k_j / sqrt(d)). A row without a key: 0 and -inf.
+//
+// Neighbouring queries choose different blocks, so no tile of queries shares its
+// keys. The chunk kernel turns the choice round: a wave owns R rows (queries x the
+// G heads of a key head) and their output accumulators, in LDS, goes through the
+// blocks, and for each gathers the rows that chose it, 16 to a matrix product.
+// Every (row, block) pair is computed once on full tiles but for the last of a block,
+// nothing leaves the chip in between, and a row meets its blocks in ascending order
+// alone, so its bits depend on its own inputs only. Products stay transposed
+// (S^T = K Q^T, O^T = V^T P^T): a lane's scores are already its part of the next
+// product's operand. K rows are MFMA operands as they lie in memory; V^T's are put
+// together from 4 keys x EPL dimensions per lane with byte permutes, so nothing is
+// staged in LDS and waves never wait for each other.
+//
+// Softmax in base 2 around the running maximum, statistics and accumulators in fp32;
+// the weights are rounded once to the type of V (half a step relative to each
+// weight, as large as the rounding of the result).
+#include "capi.hpp"
+#include "common.hpp"
+
+namespace shrimp {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int R = 64;       // rows of a chunk: one bit each in a 64-bit mask
+constexpr int WINDOW = 512; // blocks whose masks are in LDS at a time
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<__bf16> {
+  static SHRIMP_DEV f32x4 k32(u32x4 a, u32x4 b, f32x4 c) { return mfma16x16x32(a, b, c); }
+  static SHRIMP_DEV f32x4 k16(u32x2 a, u32x2 b, f32x4 c) { return mfma16x16x16(a, b, c); }
+  static SHRIMP_DEV unsigned pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+template <>
+struct Mma<_Float16> {
+  static SHRIMP_DEV f32x4 k32(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static SHRIMP_DEV f32x4 k16(u32x2 a, u32x2 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a),
+                                                 __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+  }
+  static SHRIMP_DEV unsigned pack(float lo, float hi) {
+    const f16x2 v = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(unsigned, v);
+  }
+};
+
+struct BlocksParams {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn;
+  const int32_t* sel;
+  const int32_t* q_lens;
+  const int32_t* k_lens;
+  uint16_t* out;
+  float* lse;
+  int B, H, Hk, Sq, Sk, d, block, topk;
+  int group;    // query heads per key head
+  int queries;  // queries per chunk
+  int chunks;   // chunks per (sequence, key head)
+  int by_xcd;   // a key head's chunks stay on one XCD
+  float scale2; // log2(e) / sqrt(d)
+};
+
+// The waves of one (sequence, key head) read the same keys: with by_xcd the blocks that
+// one XCD receives (every eighth) take whole key heads, so these stay in its L2.
+SHRIMP_DEV bool place_chunk(const BlocksParams& p, int64_t& bh, int& chunk) {
+  const int64_t id = blockIdx.x, pairs = (int64_t)p.B * p.Hk;
+  if (p.by_xcd) {
+    const int64_t slot = id >> 3;
+    bh = slot / p.chunks * 8 + (id & 7);
+    chunk = (int)(slot % p.chunks);
+  } else {
+    bh = id / p.chunks;
+    chunk = (int)(id % p.chunks);
+  }
+  return bh < pairs;
+}
+
+SHRIMP_DEV unsigned perm(unsigned hi, unsigned lo, unsigned sel) {
+  return __builtin_amdgcn_perm(hi, lo, sel);
+}
+constexpr unsigned SEL_LO = 0x05040100u, SEL_HI = 0x07060302u;
+
+// Rows of 16-bit elements read in 32-bit words.
+template <int W>
+using Words = unsigned __attribute__((ext_vector_type(W)));
+
+// KT tiles of 16 keys from key0 as the A operand of S^T = K Q^T: lane (lr, lg) has
+// dimensions 32 ks + 8 lg .. + 7 of key 16 kt + lr; zero past the keys and past d.
+template <int D, int KT>
+SHRIMP_DEV void load_rows(const uint16_t* base, int64_t sn, int key0, int len, int d, int lr, int lg,
+                          u32x4 (&f)[KT][D / 32]) {
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    const int key = key0 + kt * 16 + lr;
+    const uint16_t* row = base + (int64_t)key * sn + lg * 8;
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks)
+      f[kt][ks] = key < len && ks * 32 + lg * 8 < d ? *reinterpret_cast<const u32x4*>(row + ks * 32)
+                                                    : u32x4{0, 0, 0, 0};
+  }
+}
+
+// The same keys' rows for a transposed operand: lane (lr, lg) reads, of keys
+// 16 kt + 4 lg + j (j < 4), the EPL = D / 16 dimensions EPL lr .. of each.
+template <int D, int KT>
+struct Turned {
+  static constexpr int EPL = D / 16, W = EPL / 2;
+  Words<W> raw[KT][4];
+
+  SHRIMP_DEV void load(const uint16_t* base, int64_t sn, int key0, int len, int d, int lr, int lg) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = key0 + kt * 16 + lg * 4 + j;
+        const bool ok = key < len && lr * EPL < d;
+        raw[kt][j] = ok ? *reinterpret_cast<const Words<W>*>(base + (int64_t)key * sn + lr * EPL)
+                        : (Words<W>)0u;
+      }
+  }
+  // Element e of the lane's dimensions, keys 4 lg .. + 3 of tile kt, as two words.
+  SHRIMP_DEV u32x2 four(int kt, int e) const {
+    const unsigned s = e & 1 ? SEL_HI : SEL_LO;
+    const int w = e >> 1;
+    return u32x2{perm(raw[kt][1][w], raw[kt][0][w], s), perm(raw[kt][3][w], raw[kt][2][w], s)};
+  }
+};
+
+// acc[e] += (dimension-major A of these keys) x (their weights pk of 16 rows); the order of
+// the keys inside a product is that of the lanes' weights, the same on both sides.
+template <typename T, int D, int KT>
+SHRIMP_DEV void weigh(const Turned<D, KT>& v, const u32x2 (&pk)[KT], f32x4 (&acc)[D / 16]) {
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e) {
+    if constexpr (KT == 1) {
+      acc[e] = Mma<T>::k16(v.four(0, e), pk[0], acc[e]);
+    } else {
+#pragma unroll
+      for (int kt = 0; kt < KT; kt += 2) {
+        const u32x2 a = v.four(kt, e), b = v.four(kt + 1, e);
+        acc[e] = Mma<T>::k32(u32x4{a[0], a[1], b[0], b[1]},
+                             u32x4{pk[kt][0], pk[kt][1], pk[kt + 1][0], pk[kt + 1][1]}, acc[e]);
+      }
+    }
+  }
+}
+
+// What the scores of KT tiles start from: -inf for the keys past the sequence (their
+// rows were read as zeros), so that no select stands between a product and its readers.
+// (A branch there is more than slow: hipcc 7.2 left out the wait states that a VALU read
+// of a product's result needs where a branch jumps to the read, and maxima came out wrong.)
+template <int KT>
+SHRIMP_DEV void score_start(int key0, int len, int lg, f32x4 (&c)[KT]) {
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[kt][i] = key0 + kt * 16 + lg * 4 + i < len ? 0.f : -INFINITY;
+}
+
+// One step of the softmax of 16 rows (row lr, keys 16 kt + 4 lg + i at the lane): from
+// scores s and the row's (m, l) the weights pk in T, the factor for what came before,
+// and the new (m, l).
+template <typename T, int KT>
+SHRIMP_DEV float soft_step(const f32x4 (&s)[KT], float scale2, float& m, float& l, u32x2 (&pk)[KT]) {
+  float mx = s[0][0];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kt][i]);
+  const float top = fmaxf(m, max_groups_swap(mx) * scale2);
+  const float off = top == -INFINITY ? 0.f : top;  // no key yet: weights 0, not exp(nan)
+  float sum = 0.f;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], scale2, -off));
+      sum += w[i];
+    }
+    pk[kt] = u32x2{Mma<T>::pack(w[0], w[1]), Mma<T>::pack(w[2], w[3])};
+  }
+  const float alpha = __builtin_amdgcn_exp2f(m - off);
+  l = fmaf(l, alpha, sum_groups_swap(sum));
+  m = top;
+  return alpha;
+}
+
+// ---- chunk kernel: R rows per wave ----------------------------------------------------
+
+// Fills the masks of blocks [w0, w0 + n): bit r of mask[block] = row r chose it.
+SHRIMP_DEV void fill_masks(const BlocksParams& p, const int32_t* sel, int rows_q, int w0, int n,
+                           unsigned* mask, int lane) {
+  for (int i = lane; i < 2 * n; i += 64) mask[i] = 0;
+  __syncthreads();
+  const uint64_t ones = p.group >= 64 ? ~0ull : (1ull << p.group) - 1;
+  for (int j = lane; j < rows_q * p.topk; j += 64) {
+    const unsigned blk = (unsigned)(sel[j] - w0);
+    if (sel[j] >= 0 && blk < (unsigned)n) {
+      const uint64_t bits = ones << (j / p.topk * p.group);
+      if ((unsigned)bits) atomicOr(&mask[2 * blk], (unsigned)bits);
+      if ((unsigned)(bits >> 32)) atomicOr(&mask[2 * blk + 1], (unsigned)(bits >> 32));
+    }
+  }
+  __syncthreads();
+}
+
+template <int D>
+constexpr int row_floats() {
+  return D + 4;  // rows 16 bytes apart in the banks
+}
+
+template <typename T, int D, int KT>
+__global__ __launch_bounds__(64) void attn_blocks_kernel(const BlocksParams p) {
+  extern __shared__ char lds[];
+  constexpr int RF = row_floats<D>(), EPL = D / 16, KS = D / 32;
+  float* acc_lds = reinterpret_cast<float*>(lds);  // [R][RF], per row: lane group, e, i
+  float* m_lds = acc_lds + R * RF;
+  float* l_lds = m_lds + R;
+  unsigned* mask_lds = reinterpret_cast<unsigned*>(l_lds + R);  // [WINDOW][2]
+  const int lane = threadIdx.x, lr = lane & 15, lg = lane >> 4;
+  int64_t bh;
+  int chunk;
+  if (!place_chunk(p, bh, chunk)) return;
+  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
+  const int q0 = chunk * p.queries;
+  const int queries = min(p.queries, p.Sq - q0);          // written
+  const int asking = min(queries, max(q_len - q0, 0));    // with a choice
+  const int live = (k_len + p.block - 1) / p.block;
+
+  for (int i = lane; i < R * RF; i += 64) acc_lds[i] = 0.f;
+  m_lds[lane] = -INFINITY;
+  l_lds[lane] = 0.f;
+
+  // row `lane` of the chunk: query lane / G, head lane % G
+  const int my_query = lane / p.group, my_head = hk * p.group + lane - my_query * p.group;
+  const int64_t my_row = my_head * p.q_sh + (int64_t)(q0 + my_query) * p.q_sn;
+  const uint16_t* q = p.q + b * p.q_sb;
+  const uint16_t* k = p.k + b * p.k_sb + hk * p.k_sh;
+  const uint16_t* v = p.v + b * p.v_sb + hk * p.v_sh;
+  const int32_t* sel = p.sel + (bh * p.Sq + q0) * p.topk;
+
+  for (int w0 = 0; w0 < live; w0 += WINDOW) {
+    const int wn = min(WINDOW, live - w0);
+    fill_masks(p, sel, asking, w0, wn, mask_lds, lane);
+    for (int g0 = 0; g0 < wn; g0 += 64) {
+      unsigned mlo = 0, mhi = 0;
+      if (g0 + lane < wn) {
+        mlo = mask_lds[2 * (g0 + lane)];
+        mhi = mask_lds[2 * (g0 + lane) + 1];
+      }
+      uint64_t todo = __ballot((mlo | mhi) != 0);
+      while (todo) {
+        const int at = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const uint64_t mask = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)mhi, at) << 32 |
+                              (unsigned)__builtin_amdgcn_readlane((int)mlo, at);
+        const int count = __popcll(mask);
+        // lane j: the j-th row of the mask (the others behind them)
+        const bool in = mask >> lane & 1;
+        const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+        const int row_at = __builtin_amdgcn_ds_permute((in ? before : count + lane - before) << 2, lane);
+        const int start = (w0 + g0 + at) * p.block;
+        for (int key0 = start; key0 < min(start + p.block, k_len); key0 += KT * 16) {
+          u32x4 kf[KT][KS];
+          load_rows<D, KT>(k, p.k_sn, key0, k_len, p.d, lr, lg, kf);
+          Turned<D, KT> vf;
+          vf.load(v, p.v_sn, key0, k_len, p.d, lr, lg);
+          f32x4 start_at[KT];
+          score_start<KT>(key0, k_len, lg, start_at);
+          for (int t = 0; t < count; t += 16) {
+            const int row = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at);
+            const int64_t off = (int64_t)(unsigned)__builtin_amdgcn_ds_bpermute(row << 2, (int)my_row) |
+                                (int64_t)__builtin_amdgcn_ds_bpermute(row << 2, (int)(my_row >> 32)) << 32;
+            const bool on = t + lr < count;
+            u32x4 qf[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+              qf[ks] = on && ks * 32 + lg * 8 < p.d
+                           ? *reinterpret_cast<const u32x4*>(q + off + ks * 32 + lg * 8)
+                           : u32x4{0, 0, 0, 0};
+            float m = on ? m_lds[row] : -INFINITY, l = on ? l_lds[row] : 0.f;
+            f32x4 s[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+              s[kt] = start_at[kt];
+#pragma unroll
+              for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], qf[ks], s[kt]);
+            }
+            u32x2 pk[KT];
+            const float alpha = soft_step<T, KT>(s, p.scale2, m, l, pk);
+            float* mine = acc_lds + row * RF + lg * EPL * 4;
+            f32x4 acc[EPL];
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4) * alpha;
+            weigh<T, D, KT>(vf, pk, acc);
+            if (on) {
+#pragma unroll
+              for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
+              if (lg == 0) {
+                m_lds[row] = m;
+                l_lds[row] = l;
+              }
+            }
+            __syncthreads();  // (one wave: the rows' state is read again by other lanes)
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  // 16 lanes per row (D >= 64; four dimensions each), the rows' result and lse
+  constexpr int LPR = D / 4;  // lanes per row
+  __syncthreads();
+  for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
+    const int r = r0 + lane / LPR, c = lane % LPR;
+    if (r >= queries * p.group) continue;
+    const int query = r / p.group, head = hk * p.group + r - query * p.group;
+    const int64_t o = ((int64_t)b * p.H + head) * p.Sq + q0 + query;
+    const float l = l_lds[r], m = m_lds[r];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (c * 4 < p.d) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // dimension c 4 + e is element x % EPL of MFMA row x / EPL = 4 lg + i
+        const int dim = c * 4 + e, rr = dim / EPL, ee = dim % EPL;
+        x[e] = acc_lds[r * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3)] * inv;
+      }
+      *reinterpret_cast<u32x2*>(p.out + o * p.d + c * 4) =
+          u32x2{Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3])};
+    }
+    if (c == 0) p.lse[o] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+  }
+}
+
+// ---- few queries: a workgroup per query, its blocks dealt to the waves ----------------------
+
+constexpr int QW = 8;  // waves
+
+template <typename T, int D, int KT>
+__global__ __launch_bounds__(QW * 64) void attn_blocks_query_kernel(const BlocksParams p) {
+  constexpr int EPL = D / 16, KS = D / 32, RF = row_floats<D>();
+  __shared__ float o_lds[QW][16 * RF];
+  __shared__ float m_lds[QW][16], l_lds[QW][16];
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4, wave = wave_id();
+  const int64_t bh = blockIdx.x / p.Sq;
+  const int i = (int)(blockIdx.x - bh * p.Sq);
+  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
+  const int live = i < q_len ? (k_len + p.block - 1) / p.block : 0;
+  // lane t: entry t of the choice (topk <= 64), -1 where nothing is to be read
+  int mine = lane < p.topk ? p.sel[(bh * p.Sq + i) * p.topk + lane] : -1;
+  if (mine >= live) mine = -1;
+  const uint16_t* k = p.k + b * p.k_sb + hk * p.k_sh;
+  const uint16_t* v = p.v + b * p.v_sb + hk * p.v_sh;
+
+  for (int g0 = 0; g0 < p.group; g0 += 16) {  // heads of the key head, 16 rows
+    const int head = hk * p.group + g0 + lr;
+    const bool on = g0 + lr < p.group;
+    const uint16_t* q = p.q + b * p.q_sb + head * p.q_sh + (int64_t)i * p.q_sn;
+    u32x4 qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qf[ks] = on && ks * 32 + lg * 8 < p.d ? *reinterpret_cast<const u32x4*>(q + ks * 32 + lg * 8)
+                                            : u32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = wave; t < p.topk; t += QW) {
+      const int blk = __builtin_amdgcn_readlane(mine, t);
+      if (blk < 0 || __builtin_ctzll(__ballot(mine == blk)) != t) continue;  // absent, or named before
+      const int start = blk * p.block;
+      for (int key0 = start; key0 < min(start + p.block, k_len); key0 += KT * 16) {
+        u32x4 kf[KT][KS];
+        load_rows<D, KT>(k, p.k_sn, key0, k_len, p.d, lr, lg, kf);
+        Turned<D, KT> vf;
+        vf.load(v, p.v_sn, key0, k_len, p.d, lr, lg);
+        f32x4 s[KT];
+        score_start<KT>(key0, k_len, lg, s);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], qf[ks], s[kt]);
+        u32x2 pk[KT];
+        const float alpha = soft_step<T, KT>(s, p.scale2, m, l, pk);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) acc[e] *= alpha;
+        weigh<T, D, KT>(vf, pk, acc);
+      }
+    }
+    // join: every wave's rows around its own maximum, added in wave order
+#pragma unroll
+    for (int e = 0; e < EPL; ++e)
+      *reinterpret_cast<f32x4*>(&o_lds[wave][lr * RF + (lg * EPL + e) * 4]) = acc[e];
+    if (lg == 0) {
+      m_lds[wave][lr] = m;
+      l_lds[wave][lr] = l;
+    }
+    __syncthreads();
+    const int rows = min(16, p.group - g0);
+    for (int x = threadIdx.x; x < rows * (D / 4); x += QW * 64) {
+      const int r = x / (D / 4), c = x % (D / 4);
+      float top = -INFINITY;
+      for (int w = 0; w < QW; ++w) top = fmaxf(top, m_lds[w][r]);
+      const float off = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < QW; ++w) {
+        const float f = __builtin_amdgcn_exp2f(m_lds[w][r] - off);
+        sum = fmaf(l_lds[w][r], f, sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int dim = c * 4 + e, rr = dim / EPL, ee = dim % EPL;
+          y[e] = fmaf(o_lds[w][r * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3)], f, y[e]);
+        }
+      }
+      const int64_t o = ((int64_t)b * p.H + hk * p.group + g0 + r) * p.Sq + i;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      if (c * 4 < p.d)
+        *reinterpret_cast<u32x2*>(p.out + o * p.d + c * 4) =
+            u32x2{Mma<T>::pack(y[0] * inv, y[1] * inv), Mma<T>::pack(y[2] * inv, y[3] * inv)};
+      if (c == 0) p.lse[o] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------
+
+// Few enough queries that a workgroup for each (its tile holding the G heads alone)
+// beats waves that go through every block for 64 rows.
+constexpr int FEW_QUERIES = 8;
+
+int check_blocks(const shrimp_attn_blocks_args* a, const char* what) {
+  SHRIMP_REQUIRE(a != nullptr, "%s: null arguments", what);
+  SHRIMP_REQUIRE(a->dt == SHRIMP_DT_BF16 || a->dt == SHRIMP_DT_F16, "%s: element type %d", what, a->dt);
+  SHRIMP_REQUIRE(a->B >= 0 && a->H >= 0 && a->Sq >= 0 && a->Sk >= 0, "%s: negative size", what);
+  SHRIMP_REQUIRE(a->Hk >= 1 && a->H % a->Hk == 0 && a->H / a->Hk <= R,
+                 "%s: %d query heads for %d key heads (at most %d each)", what, a->H, a->Hk, R);
+  SHRIMP_REQUIRE(a->d >= 8 && a->d <= SHRIMP_BLOCK_MAX_D && a->d % 8 == 0,
+                 "%s: head dim %d is not a multiple of 8 in [8, %d]", what, a->d, SHRIMP_BLOCK_MAX_D);
+  SHRIMP_REQUIRE(a->block >= 16 && a->block % 16 == 0 && a->block <= (1 << 20),
+                 "%s: blocks of %d keys, a multiple of 16 expected", what, a->block);
+  SHRIMP_REQUIRE(a->topk >= 1 && a->topk <= SHRIMP_BLOCK_MAX_TOPK, "%s: topk %d outside [1, %d]", what,
+                 a->topk, SHRIMP_BLOCK_MAX_TOPK);
+  SHRIMP_REQUIRE(a->Sq <= (1 << 30) && a->Sk <= (1 << 30), "%s: Sq=%d, Sk=%d", what, a->Sq, a->Sk);
+  SHRIMP_REQUIRE(a->scale > 0.f, "%s: scale must be positive", what);
+  if (a->B == 0 || a->H == 0 || a->Sq == 0) return SHRIMP_OK;
+  auto aligned = [](const void* base, int64_t sb, int64_t sh, int64_t sn) {
+    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && sb % 8 == 0 && sh % 8 == 0 && sn % 8 == 0;
+  };
+  SHRIMP_REQUIRE(a->q && a->sel && a->q_lens && a->k_lens && a->out && a->lse, "%s: null pointer", what);
+  SHRIMP_REQUIRE(a->Sk == 0 || (a->k && a->v), "%s: null k or v", what);
+  SHRIMP_REQUIRE(aligned(a->q, a->q_sb, a->q_sh, a->q_sn) && aligned(a->k, a->k_sb, a->k_sh, a->k_sn) &&
+                     aligned(a->v, a->v_sb, a->v_sh, a->v_sn) && aligned(a->out, 0, 0, 0),
+                 "%s: rows must start on 16-byte boundaries", what);
+  return SHRIMP_OK;
+}
+
+BlocksParams blocks_params(const shrimp_attn_blocks_args* a) {
+  BlocksParams p{};
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.k = static_cast<const uint16_t*>(a->k);
+  p.v = static_cast<const uint16_t*>(a->v);
+  p.q_sb = a->q_sb, p.q_sh = a->q_sh, p.q_sn = a->q_sn;
+  p.k_sb = a->k_sb, p.k_sh = a->k_sh, p.k_sn = a->k_sn;
+  p.v_sb = a->v_sb, p.v_sh = a->v_sh, p.v_sn = a->v_sn;
+  p.sel = a->sel;
+  p.q_lens = a->q_lens;
+  p.k_lens = a->k_lens;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.lse = a->lse;
+  p.B = a->B, p.H = a->H, p.Hk = a->Hk, p.Sq = a->Sq, p.Sk = a->Sk;
+  p.d = a->d, p.block = a->block, p.topk = a->topk;
+  p.group = a->H / a->Hk;
+  p.queries = R / p.group;
+  p.chunks = (a->Sq + p.queries - 1) / p.queries;
+  const int64_t pairs = (int64_t)a->B * a->Hk;
+  p.by_xcd = pairs % 8 == 0 || pairs >= 64;
+  p.scale2 = a->scale * LOG2E;
+  return p;
+}
+
+template <typename T, int D, int KT>
+int launch_forward(const BlocksParams& p, hipStream_t st) {
+  if (p.Sq <= FEW_QUERIES) {
+    const int64_t n = (int64_t)p.B * p.Hk * p.Sq;
+    SHRIMP_REQUIRE(n <= INT32_MAX, "attn_blocks: %lld queries", (long long)n);
+    hipLaunchKernelGGL((attn_blocks_query_kernel<T, D, KT>), dim3((unsigned)n), dim3(QW * 64), 0, st, p);
+    return SHRIMP_OK;
+  }
+  const int64_t pairs = (int64_t)p.B * p.Hk;
+  const int64_t n = (p.by_xcd ? (pairs + 7) / 8 * 8 : pairs) * p.chunks;
+  SHRIMP_REQUIRE(n <= INT32_MAX, "attn_blocks: %lld chunks of queries", (long long)n);
+  const size_t lds = (size_t)R * (row_floats<D>() + 2) * 4 + (size_t)WINDOW * 8;
+  hipLaunchKernelGGL((attn_blocks_kernel<T, D, KT>), dim3((unsigned)n), dim3(64), lds, st, p);
+  return SHRIMP_OK;
+}
+
+template <typename T, int D>
+int launch_forward_kt(const BlocksParams& p, hipStream_t st) {
+  if (p.block % 64 == 0) return launch_forward<T, D, 4>(p, st);
+  if (p.block % 32 == 0) return launch_forward<T, D, 2>(p, st);
+  return launch_forward<T, D, 1>(p, st);
+}
+
+template <typename T>
+int launch_forward_d(const BlocksParams& p, hipStream_t st) {
+  if (p.d <= 32) return launch_forward_kt<T, 32>(p, st);
+  if (p.d <= 64) return launch_forward_kt<T, 64>(p, st);
+  return launch_forward_kt<T, 128>(p, st);
+}
+
+}  // namespace
+}  // namespace shrimp
+
+extern "C" int shrimp_attn_blocks(const shrimp_attn_blocks_args* a, void* stream) {
+  using namespace shrimp;
+  const int rc = check_blocks(a, "attn_blocks");
+  if (rc != SHRIMP_OK) return rc;
+  if (a->B == 0 || a->H == 0 || a->Sq == 0) return SHRIMP_OK;
+  const BlocksParams p = blocks_params(a);
+  const int e = a->dt == SHRIMP_DT_F16 ? launch_forward_d<_Float16>(p, as_stream(stream))
+                                       : launch_forward_d<__bf16>(p, as_stream(stream));
+  if (e != SHRIMP_OK) return e;
+  return check_launch("attn_blocks");
+}

@@ -1,0 +1,429 @@
+// Mean key of every block of keys, and for every query the blocks whose mean has
+// the largest product with it.
+//
+//   mean[b, h, n] = sum of block n's live keys / their number      (fp32, zero without one)
+//   score[b, h, i, n] = (sum of the queries i of the heads that share key head h) . mean
+//   sel[b, h, i] = the topk live blocks of largest score, ascending, then -1
+//
+// A choice hangs on which of two scores is larger, so means and scores are summed in
+// float64: a program that computes them in another order (or another batch) chooses
+// the same blocks, up to scores that agree in some 50 bits. Equal scores go to the lower
+// block; a NaN counts as the lowest. Scores run on the fp64 matrix product,
+// 16 queries x 16 blocks x 4 dimensions, at 1/16 of the bf16 one's rate; with D
+// dimensions and NB blocks it is 2 D NB operations a query beside the 2 D bytes that
+// the query costs to read, so long sequences are bound by it (64000 query groups,
+// 125 blocks, D = 128: 28 us at the rate of a large fp64 product).
+#include "capi.hpp"
+#include "common.hpp"
+
+namespace shrimp {
+namespace {
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+constexpr int MAX_TOPK = SHRIMP_BLOCK_MAX_TOPK;
+constexpr int MAX_D = SHRIMP_BLOCK_MAX_D;
+constexpr int MAX_BLOCKS = SHRIMP_BLOCK_MAX_BLOCKS;
+
+template <typename T, int V>
+using Vec = T __attribute__((ext_vector_type(V)));
+
+struct MeanParams {
+  const void* k;
+  const int32_t* lens;
+  float* means;
+  int64_t sb, sh, sn;
+  int B, Hk, Sk, D, NB, block;
+  int lanes;  // lanes per row
+  int last_only;
+};
+
+// One wave per block of keys: lanes take a row's dimensions, groups of lanes rows.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void block_means_kernel(const MeanParams p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + wave_id();
+  const int per = p.last_only ? 1 : p.NB;
+  const int64_t bh = item / per;
+  if (bh >= (int64_t)p.B * p.Hk) return;
+  const int b = (int)(bh / p.Hk), h = (int)(bh - (int64_t)b * p.Hk);
+  const int len = min(max(p.lens[b], 0), p.Sk);
+  const int n = p.last_only ? max(len - 1, 0) / p.block : (int)(item - bh * per);
+  const int64_t start = (int64_t)n * p.block;
+  const int rows = (int)min((int64_t)p.block, len - start);  // live keys, none if <= 0
+  const int ul = lane & (p.lanes - 1), group = lane / p.lanes, groups = 64 / p.lanes;
+  float* out = p.means + (bh * p.NB + n) * p.D;
+  const T* k = static_cast<const T*>(p.k) + b * p.sb + h * p.sh + start * p.sn;
+  for (int d = ul * V; d < p.D; d += p.lanes * V) {
+    double sum[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[e] = 0.0;
+#pragma unroll 8
+    for (int r = group; r < rows; r += groups) {
+      const Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(k + r * p.sn + d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[e] += (double)(float)x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      for (int m = p.lanes; m < 64; m <<= 1) sum[e] += __shfl_xor(sum[e], m, 64);
+      if (group == 0) out[d + e] = rows > 0 ? (float)(sum[e] / (double)rows) : 0.f;
+    }
+  }
+}
+
+struct SelectParams {
+  const void* q;
+  const float* means;
+  const int32_t* q_lens;
+  const int32_t* k_lens;
+  int32_t* sel;
+  int64_t sb, sh, sn;
+  int B, H, Hk, Sq, Sk, D, NB, block, topk;
+  int group;   // query heads per key head
+  int tiles;   // tiles of 16 queries per (sequence, key head)
+  int chunk;   // blocks scored before a choice among them and the carried ones
+  int vec;     // rows of q readable four elements at a time
+};
+
+// Order of doubles as order of unsigned integers; 0 is left for "none".
+SHRIMP_DEV uint64_t order_key(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);  // -0 as 0
+  if (x != x) return 1;
+  return u >> 63 ? ~u : u | (1ull << 63);
+}
+
+template <typename T>
+SHRIMP_DEV double load_f64(const T* p) {
+  return (double)(float)*p;
+}
+
+// One wave: 16 queries of a (sequence, key head). LDS: per query row the carried keys
+// and a chunk's keys, the carried indices, and the chosen of this chunk.
+template <typename T, int DP>
+__global__ __launch_bounds__(64) void block_select_kernel(const SelectParams p) {
+  extern __shared__ uint64_t lds[];
+  constexpr int DK = DP / 4;  // dimensions of a lane: of the four that a product takes
+                              // at a time, lane group g supplies dimensions g DK + step
+  const int lane = threadIdx.x, lr = lane & 15, lg = lane >> 4;
+  const int64_t bh = blockIdx.x / p.tiles;
+  const int tile = (int)(blockIdx.x - bh * p.tiles);
+  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
+  const int live = (k_len + p.block - 1) / p.block;
+  const int i0 = tile * 16;
+  const int entries = p.topk + p.chunk;
+  uint64_t* keys = lds;                               // [16][entries]
+  uint64_t* best_key = keys + 16 * entries;           // [16][topk]
+  int* best_id = reinterpret_cast<int*>(best_key + 16 * p.topk);  // [16][topk]
+  int* carry_id = best_id + 16 * p.topk;              // [16][topk]
+  int32_t* sel = p.sel + (bh * p.Sq + i0) * p.topk;
+  const int rows = min(16, p.Sq - i0);
+
+  if (i0 >= q_len || live <= p.topk) {  // none, or every live block
+    for (int j = lane; j < rows * p.topk; j += 64) {
+      const int r = j / p.topk, t = j - r * p.topk;
+      sel[j] = i0 + r < q_len && t < live ? t : -1;
+    }
+    return;
+  }
+
+  double a[DK];
+#pragma unroll
+  for (int s = 0; s < DK; ++s) a[s] = 0.0;
+  if (i0 + lr < q_len) {
+    for (int h = 0; h < p.group; ++h) {
+      const T* q = static_cast<const T*>(p.q) + b * p.sb + (int64_t)(hk * p.group + h) * p.sh +
+                   (int64_t)(i0 + lr) * p.sn;
+      if (p.vec) {
+#pragma unroll
+        for (int s = 0; s < DK; s += 4) {
+          const int d = lg * DK + s;
+          if (d < p.D) {
+            const Vec<T, 4> x = *reinterpret_cast<const Vec<T, 4>*>(q + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[s + e] += (double)(float)x[e];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < DK; ++s)
+          if (lg * DK + s < p.D) a[s] += load_f64(q + lg * DK + s);
+      }
+    }
+  }
+
+  const float* means = p.means + bh * p.NB * p.D;
+  const bool mvec = p.D % 4 == 0;
+  const int row = lane >> 2, sub = lane & 3;  // the choice: four lanes per query
+  int carried = 0;
+  for (int c0 = 0; c0 < live; c0 += p.chunk) {
+    const int here = min(p.chunk, live - c0);
+    for (int t = 0; t < here; t += 16) {
+      const int n = c0 + t + lr;
+      float m[DK];
+#pragma unroll
+      for (int s = 0; s < DK; ++s) m[s] = 0.f;
+      if (n < live) {
+        const float* row_n = means + (int64_t)n * p.D;
+        if (mvec) {
+#pragma unroll
+          for (int s = 0; s < DK; s += 4) {
+            const int d = lg * DK + s;
+            if (d < p.D) {
+              const f32x4 x = *reinterpret_cast<const f32x4*>(row_n + d);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) m[s + e] = x[e];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < DK; ++s)
+            if (lg * DK + s < p.D) m[s] = row_n[lg * DK + s];
+        }
+      }
+      f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+      for (int s = 0; s < DK; ++s)
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s], (double)m[s], acc, 0, 0, 0);
+      // lane (lr, lg) holds block column lr of queries 4 i + lg
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        keys[(4 * i + lg) * entries + p.topk + t + lr] = n < live ? order_key(acc[i]) : 0;
+    }
+    __syncthreads();
+    // the topk largest of the carried and the new, largest first
+    const int first = carried ? 0 : p.topk, last = p.topk + ((here + 15) & ~15);
+    uint64_t* mine = keys + row * entries;
+    for (int it = 0; it < p.topk; ++it) {
+      uint64_t key = 0;
+      int at = -1;
+      for (int j = first + sub; j < last; j += 4) {
+        const uint64_t k = mine[j];
+        if (k > key) {
+          key = k;
+          at = j;
+        }
+      }
+#pragma unroll
+      for (int m = 1; m <= 2; m <<= 1) {
+        const uint64_t k = __shfl_xor(key, m, 64);
+        const int j = __shfl_xor(at, m, 64);
+        if (k > key || (k == key && k != 0 && j < at)) {
+          key = k;
+          at = j;
+        }
+      }
+      if (sub == 0) {
+        best_key[row * p.topk + it] = key;
+        best_id[row * p.topk + it] =
+            key == 0 ? -1 : at < p.topk ? carry_id[row * p.topk + at] : c0 + at - p.topk;
+        if (key != 0) mine[at] = 0;
+      }
+      __syncthreads();
+    }
+    carried = 1;
+    for (int j = lane; j < 16 * p.topk; j += 64) {
+      const int r = j / p.topk, t = j - r * p.topk;
+      keys[r * entries + t] = best_key[j];
+      carry_id[j] = best_id[j];
+    }
+    __syncthreads();
+  }
+  // ascending: a chosen block's place is the number of chosen ones below it
+  for (int j = lane; j < rows * p.topk; j += 64) {
+    const int r = j / p.topk;
+    const int id = best_id[j];
+    int at = 0;
+    for (int t = 0; t < p.topk; ++t) at += best_id[r * p.topk + t] < id;
+    sel[r * p.topk + at] = i0 + r < q_len ? id : -1;
+  }
+}
+
+// Few queries (serving): a workgroup per query, 16 lanes per block's product.
+constexpr int ROW_THREADS = 256;
+
+template <typename T>
+__global__ __launch_bounds__(ROW_THREADS) void block_select_row_kernel(const SelectParams p) {
+  extern __shared__ uint64_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t bh = blockIdx.x / p.Sq;
+  const int i = (int)(blockIdx.x - bh * p.Sq);
+  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
+  const int live = (k_len + p.block - 1) / p.block;
+  int32_t* sel = p.sel + (bh * p.Sq + i) * p.topk;
+  if (i >= q_len || live <= p.topk) {
+    for (int t = tid; t < p.topk; t += ROW_THREADS) sel[t] = i < q_len && t < live ? t : -1;
+    return;
+  }
+  double* q = reinterpret_cast<double*>(lds);  // [MAX_D]
+  uint64_t* keys = lds + MAX_D;                // [live]
+  if (tid < p.D) {
+    double s = 0.0;
+    for (int h = 0; h < p.group; ++h)
+      s += load_f64(static_cast<const T*>(p.q) + b * p.sb + (int64_t)(hk * p.group + h) * p.sh +
+                    (int64_t)i * p.sn + tid);
+    q[tid] = s;
+  }
+  __syncthreads();
+  const float* means = p.means + bh * p.NB * p.D;
+  const int part = tid & 15;
+#pragma unroll 4
+  for (int n = tid >> 4; n < live; n += ROW_THREADS / 16) {
+    const float* m = means + (int64_t)n * p.D;
+    double s = 0.0;
+    for (int d = part; d < p.D; d += 16) s = __builtin_fma(q[d], (double)m[d], s);
+    for (int x = 1; x < 16; x <<= 1) s += __shfl_xor(s, x, 64);
+    if (part == 0) keys[n] = order_key(s);
+  }
+  __syncthreads();
+  if (tid >= 64) return;
+  uint64_t key = 0;
+  int at = -1;
+  auto scan = [&]() {  // the largest of this lane's keys, the lowest index of equals
+    key = 0;
+    at = -1;
+    for (int n = lane; n < live; n += 64)
+      if (keys[n] > key) {
+        key = keys[n];
+        at = n;
+      }
+  };
+  scan();
+  int mine = 0x7fffffff;  // lane t: the t-th largest's index
+  for (int t = 0; t < p.topk; ++t) {
+    uint64_t k = key;
+    int j = at;
+    for (int m = 1; m < 64; m <<= 1) {
+      const uint64_t ko = __shfl_xor(k, m, 64);
+      const int jo = __shfl_xor(j, m, 64);
+      if (ko > k || (ko == k && ko != 0 && jo < j)) {
+        k = ko;
+        j = jo;
+      }
+    }
+    if (lane == t) mine = j;
+    if (at == j) {  // (live > topk: there is one)
+      keys[j] = 0;
+      scan();
+    }
+  }
+  int place = 0;
+  for (int t = 0; t < p.topk; ++t) place += __shfl(mine, t, 64) < mine;
+  if (lane < p.topk) sel[place] = mine;
+}
+
+int pow2_ceil(int n) {
+  int v = 1;
+  while (v < n) v <<= 1;
+  return v;
+}
+
+int dt_size(int dt) { return dt == SHRIMP_DT_F32 ? 4 : 2; }
+
+bool row_vec4(const void* base, int64_t sb, int64_t sh, int64_t sn, int D, int es) {
+  return D % 4 == 0 && sb % 4 == 0 && sh % 4 == 0 && sn % 4 == 0 &&
+         reinterpret_cast<uintptr_t>(base) % (uintptr_t)(4 * es) == 0;
+}
+
+template <typename T>
+void means_grid(const MeanParams& p, bool vec, dim3 grid, hipStream_t st) {
+  if (vec)
+    hipLaunchKernelGGL((block_means_kernel<T, 4>), grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((block_means_kernel<T, 1>), grid, dim3(256), 0, st, p);
+}
+
+int means_launch(const void* k, int64_t sb, int64_t sh, int64_t sn, int dt, const int32_t* lens,
+                 float* means, int B, int Hk, int Sk, int D, int block, bool last_only,
+                 void* stream, const char* what) {
+  SHRIMP_REQUIRE(dt == SHRIMP_DT_BF16 || dt == SHRIMP_DT_F16 || dt == SHRIMP_DT_F32,
+                 "%s: element type %d", what, dt);
+  SHRIMP_REQUIRE(B >= 0 && Hk >= 0 && Sk >= 0, "%s: negative size", what);
+  SHRIMP_REQUIRE(D >= 1 && D <= MAX_D, "%s: head dim %d outside [1, %d]", what, D, MAX_D);
+  SHRIMP_REQUIRE(block >= 1, "%s: block of %d keys", what, block);
+  const int64_t nb = ((int64_t)Sk + block - 1) / block;
+  SHRIMP_REQUIRE(nb <= MAX_BLOCKS, "%s: %lld blocks, at most %d", what, (long long)nb, MAX_BLOCKS);
+  if (B == 0 || Hk == 0 || nb == 0) return SHRIMP_OK;
+  SHRIMP_REQUIRE(k && lens && means, "%s: null pointer", what);
+  const int64_t items = (int64_t)B * Hk * (last_only ? 1 : nb);
+  SHRIMP_REQUIRE(items <= INT32_MAX, "%s: %lld blocks of keys", what, (long long)items);
+  const bool vec = row_vec4(k, sb, sh, sn, D, dt_size(dt));
+  const int units = vec ? D / 4 : D;
+  const MeanParams p{k, lens, means, sb, sh, sn, B, Hk, Sk, D, (int)nb, block,
+                     pow2_ceil(units < 64 ? units : 64), last_only};
+  const dim3 grid((unsigned)((items + 3) / 4));
+  hipStream_t st = as_stream(stream);
+  if (dt == SHRIMP_DT_F32)
+    means_grid<float>(p, vec, grid, st);
+  else if (dt == SHRIMP_DT_F16)
+    means_grid<_Float16>(p, vec, grid, st);
+  else
+    means_grid<__bf16>(p, vec, grid, st);
+  return check_launch(what);
+}
+
+template <typename T>
+void select_launch(const SelectParams& p, int64_t rows, size_t row_lds, size_t tile_lds, bool by_row,
+                   hipStream_t st) {
+  if (by_row) {
+    hipLaunchKernelGGL((block_select_row_kernel<T>), dim3((unsigned)rows), dim3(ROW_THREADS), row_lds,
+                       st, p);
+    return;
+  }
+  const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.tiles));
+  if (p.D <= 32)
+    hipLaunchKernelGGL((block_select_kernel<T, 32>), grid, dim3(64), tile_lds, st, p);
+  else if (p.D <= 64)
+    hipLaunchKernelGGL((block_select_kernel<T, 64>), grid, dim3(64), tile_lds, st, p);
+  else
+    hipLaunchKernelGGL((block_select_kernel<T, 128>), grid, dim3(64), tile_lds, st, p);
+}
+
+}  // namespace
+}  // namespace shrimp
+
+extern "C" int shrimp_block_means(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, int dt,
+                                  const int32_t* k_lens, float* means, int B, int Hk, int Sk, int D,
+                                  int block, int last_only, void* stream) {
+  return shrimp::means_launch(k, k_sb, k_sh, k_sn, dt, k_lens, means, B, Hk, Sk, D, block,
+                              last_only != 0, stream, "block_means");
+}
+
+extern "C" int shrimp_block_select(const shrimp_block_select_args* a, void* stream) {
+  using namespace shrimp;
+  SHRIMP_REQUIRE(a != nullptr, "block_select: null arguments");
+  SHRIMP_REQUIRE(a->dt == SHRIMP_DT_BF16 || a->dt == SHRIMP_DT_F16 || a->dt == SHRIMP_DT_F32,
+                 "block_select: element type %d", a->dt);
+  SHRIMP_REQUIRE(a->B >= 0 && a->H >= 0 && a->Sq >= 0 && a->Sk >= 0, "block_select: negative size");
+  SHRIMP_REQUIRE(a->Hk >= 1 && a->H % a->Hk == 0, "block_select: %d query heads for %d key heads",
+                 a->H, a->Hk);
+  SHRIMP_REQUIRE(a->D >= 1 && a->D <= MAX_D, "block_select: head dim %d outside [1, %d]", a->D, MAX_D);
+  SHRIMP_REQUIRE(a->block >= 1, "block_select: block of %d keys", a->block);
+  SHRIMP_REQUIRE(a->topk >= 1 && a->topk <= MAX_TOPK, "block_select: topk %d outside [1, %d]", a->topk,
+                 MAX_TOPK);
+  const int64_t nb = ((int64_t)a->Sk + a->block - 1) / a->block;
+  SHRIMP_REQUIRE(nb <= MAX_BLOCKS, "block_select: %lld blocks, at most %d", (long long)nb, MAX_BLOCKS);
+  if (a->B == 0 || a->H == 0 || a->Sq == 0) return SHRIMP_OK;
+  SHRIMP_REQUIRE(a->q && a->q_lens && a->k_lens && a->sel && (a->means || nb == 0),
+                 "block_select: null pointer");
+  SelectParams p{a->q, a->means, a->q_lens, a->k_lens, a->sel, a->q_sb, a->q_sh, a->q_sn,
+                 a->B, a->H, a->Hk, a->Sq, a->Sk, a->D, (int)nb, a->block, a->topk, a->H / a->Hk,
+                 (a->Sq + 15) / 16, 0, row_vec4(a->q, a->q_sb, a->q_sh, a->q_sn, a->D, dt_size(a->dt))};
+  p.chunk = nb < 128 ? (int)(nb + 15) / 16 * 16 : 128;
+  const int64_t rows = (int64_t)a->B * a->Hk * a->Sq;
+  SHRIMP_REQUIRE(rows <= INT32_MAX, "block_select: %lld queries", (long long)rows);
+  // A tile of 16 queries takes a product's time however few of them there are.
+  const bool by_row = a->Sq <= 2;
+  const size_t row_lds = (MAX_D + nb) * 8;
+  const size_t tile_lds = (size_t)16 * (a->topk + p.chunk) * 8 + (size_t)16 * a->topk * 16;
+  hipStream_t st = as_stream(stream);
+  if (a->dt == SHRIMP_DT_F32)
+    select_launch<float>(p, rows, row_lds, tile_lds, by_row, st);
+  else if (a->dt == SHRIMP_DT_F16)
+    select_launch<_Float16>(p, rows, row_lds, tile_lds, by_row, st);
+  else
+    select_launch<__bf16>(p, rows, row_lds, tile_lds, by_row, st);
+  return check_launch("block_select");
+}

@@ -153,6 +153,27 @@ class RopeArgs(ctypes.Structure):
     ]
 
 
+class BlockSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("q_sb", _i64), ("q_sh", _i64), ("q_sn", _i64),
+        ("means", _vp), ("q_lens", _vp), ("k_lens", _vp), ("sel", _vp),
+        ("B", _i32), ("H", _i32), ("Hk", _i32), ("Sq", _i32), ("Sk", _i32), ("D", _i32),
+        ("block", _i32), ("topk", _i32), ("dt", _i32),
+    ]
+
+
+class AttnBlocksArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp),
+        ("q_sb", _i64), ("q_sh", _i64), ("q_sn", _i64),
+        ("k_sb", _i64), ("k_sh", _i64), ("k_sn", _i64),
+        ("v_sb", _i64), ("v_sh", _i64), ("v_sn", _i64),
+        ("sel", _vp), ("q_lens", _vp), ("k_lens", _vp), ("out", _vp), ("lse", _vp),
+        ("B", _i32), ("H", _i32), ("Hk", _i32), ("Sq", _i32), ("Sk", _i32), ("d", _i32),
+        ("block", _i32), ("topk", _i32), ("dt", _i32), ("scale", _f32),
+    ]
+
+
 # Exported symbols and their ctypes signatures; tests check every one of them
 # against the header and the built library.
 SIGNATURES: dict = {
@@ -250,6 +271,11 @@ SIGNATURES: dict = {
     "shrimp_qk_norm_rope_backward": (
         ctypes.c_int, [ctypes.POINTER(RopeArgs), _vp, _vp, _vp, _i64, _vp]
     ),
+    "shrimp_block_means": (
+        ctypes.c_int, [_vp] + [_i64] * 3 + [ctypes.c_int, _vp, _vp] + [ctypes.c_int] * 6 + [_vp]
+    ),
+    "shrimp_block_select": (ctypes.c_int, [ctypes.POINTER(BlockSelectArgs), _vp]),
+    "shrimp_attn_blocks": (ctypes.c_int, [ctypes.POINTER(AttnBlocksArgs), _vp]),
 }
 
 _LIB = None

@@ -574,6 +574,12 @@ def _attn_pair_fake(q, k, v, pair, table2, seq_lens):
 
 # ---- operators in modules of their own, under the same names here ---------------------------
 
+from .block_attn import (  # noqa: E402,F401
+    attn_blocks,
+    block_means,
+    block_means_update,
+    block_select,
+)
 from .rotary import (  # noqa: E402,F401
     qk_norm_rope,
     qk_norm_rope_backward,

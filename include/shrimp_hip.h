@@ -814,6 +814,75 @@ int64_t shrimp_qk_norm_rope_workspace(const shrimp_rope_args* a);
 int shrimp_qk_norm_rope_backward(const shrimp_rope_args* a, void* dw_q, void* dw_k,
                                  void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Blocks of keys chosen by a score (shrimp::block_means, shrimp::block_select;
+ * no counterpart in the reference). NB = ceil(Sk / block) blocks per sequence.
+ *   means (B, Hk, NB, D) fp32 contiguous: mean of block n's keys below k_lens[b]
+ *     (clamped to [0, Sk]), summed in fp64; zero for a block without one. k (B,
+ *     Hk, Sk, D) of type dt (SHRIMP_DT_BF16 / F16 / F32), strides in elements, the
+ *     last one 1. last_only writes only the block of each sequence's last key
+ *     (block 0 for an empty sequence) and leaves the others as they are.
+ *   sel (B, Hk, Sq, topk) int32 contiguous: for every query row i < q_lens[b] the
+ *     topk blocks below ceil(k_lens[b] / block) of largest score, ascending, then
+ *     -1; rows from q_lens[b] on are -1. Score: mean . (sum of the rows i of the
+ *     H / Hk query heads that share the key head), in fp64; equal scores go to
+ *     the lower block, NaN ranks lowest. q (B, H, Sq, D) of type dt.
+ * D <= SHRIMP_BLOCK_MAX_D, topk <= SHRIMP_BLOCK_MAX_TOPK, NB <=
+ * SHRIMP_BLOCK_MAX_BLOCKS.
+ * ---------------------------------------------------------------------- */
+#define SHRIMP_BLOCK_MAX_D 128
+#define SHRIMP_BLOCK_MAX_TOPK 64
+#define SHRIMP_BLOCK_MAX_BLOCKS 4096
+
+typedef struct {
+  const void* q;
+  int64_t q_sb, q_sh, q_sn;
+  const float* means;
+  const int32_t* q_lens;
+  const int32_t* k_lens;
+  int32_t* sel;
+  int32_t B, H, Hk, Sq, Sk, D;
+  int32_t block, topk, dt;
+} shrimp_block_select_args;
+
+int shrimp_block_means(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, int dt,
+                       const int32_t* k_lens, float* means, int B, int Hk, int Sk, int D, int block,
+                       int last_only, void* stream);
+int shrimp_block_select(const shrimp_block_select_args* a, void* stream);
+
+/* ------------------------------------------------------------------------
+ * shrimp::attn_blocks: softmax attention of every query over its own blocks of keys
+ * (no counterpart in the reference; shrimp_attn reads all of them).
+ *   q (B, H, Sq, d), k, v (B, Hk, Sk, d) of type dt (SHRIMP_DT_BF16 / F16), Hk
+ *     divides H, at most 64 query heads per key head; strides in elements,
+ *     multiples of 8, the last one 1, rows on 16-byte boundaries; d a multiple of
+ *     8 up to SHRIMP_BLOCK_MAX_D. block a multiple of 16.
+ *   sel (B, Hk, Sq, topk) int32 contiguous: a row's blocks in any order; entries
+ *     outside [0, ceil(k_lens[b] / block)) name none, repeated ones count once.
+ *   out (B, H, Sq, d) of type dt and lse (B, H, Sq) fp32, contiguous: rows from
+ *     q_lens[b] on, and rows that no key below k_lens[b] reaches, are 0 and -inf.
+ *     Lengths are clamped to [0, Sq] and [0, Sk]; keys past them are not read.
+ *   scale multiplies the scores (> 0).
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_sb, q_sh, q_sn;
+  int64_t k_sb, k_sh, k_sn;
+  int64_t v_sb, v_sh, v_sn;
+  const int32_t* sel;
+  const int32_t* q_lens;
+  const int32_t* k_lens;
+  void* out;
+  float* lse;
+  int32_t B, H, Hk, Sq, Sk, d;
+  int32_t block, topk, dt;
+  float scale;
+} shrimp_attn_blocks_args;
+
+int shrimp_attn_blocks(const shrimp_attn_blocks_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
