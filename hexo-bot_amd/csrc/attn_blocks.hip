@@ -78,15 +78,15 @@ struct BlocksParams {
 
 // The waves of one (sequence, key head) read the same keys: with by_xcd the blocks that
 // one XCD receives (every eighth) take whole key heads, so these stay in its L2.
-SHRIMP_DEV bool place_chunk(const BlocksParams& p, int64_t& bh, int& chunk) {
+SHRIMP_DEV bool place_chunk(const BlocksParams& p, int chunks, int64_t& bh, int& chunk) {
   const int64_t id = blockIdx.x, pairs = (int64_t)p.B * p.Hk;
   if (p.by_xcd) {
     const int64_t slot = id >> 3;
-    bh = slot / p.chunks * 8 + (id & 7);
-    chunk = (int)(slot % p.chunks);
+    bh = slot / chunks * 8 + (id & 7);
+    chunk = (int)(slot % chunks);
   } else {
-    bh = id / p.chunks;
-    chunk = (int)(id % p.chunks);
+    bh = id / chunks;
+    chunk = (int)(id % chunks);
   }
   return bh < pairs;
 }
@@ -221,6 +221,56 @@ SHRIMP_DEV void fill_masks(const BlocksParams& p, const int32_t* sel, int rows_q
   __syncthreads();
 }
 
+// f(mask, row_at, block) for every block that a row of the chunk chose, ascending: bit r
+// of the mask is row r, and lane j holds in row_at the j-th row of the mask (lanes from
+// its count on hold the others). `keep`, when given, receives every live block's mask,
+// `keep_stride` apart.
+template <typename F>
+SHRIMP_DEV void each_block(const BlocksParams& p, const int32_t* sel, int asking, int live,
+                           unsigned* mask_lds, int lane, uint64_t* keep, int64_t keep_stride, F f) {
+  for (int w0 = 0; w0 < live; w0 += WINDOW) {
+    const int wn = min(WINDOW, live - w0);
+    fill_masks(p, sel, asking, w0, wn, mask_lds, lane);
+    for (int g0 = 0; g0 < wn; g0 += 64) {
+      unsigned mlo = 0, mhi = 0;
+      if (g0 + lane < wn) {
+        mlo = mask_lds[2 * (g0 + lane)];
+        mhi = mask_lds[2 * (g0 + lane) + 1];
+        if (keep) keep[(w0 + g0 + lane) * keep_stride] = (uint64_t)mhi << 32 | mlo;
+      }
+      uint64_t todo = __ballot((mlo | mhi) != 0);
+      while (todo) {
+        const int at = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const uint64_t mask = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)mhi, at) << 32 |
+                              (unsigned)__builtin_amdgcn_readlane((int)mlo, at);
+        const bool in = mask >> lane & 1;
+        const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+        const int to = in ? before : __popcll(mask) + lane - before;
+        f(mask, __builtin_amdgcn_ds_permute(to << 2, lane), w0 + g0 + at);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// 64-bit value of lane `src` (byte address 4 src) for every lane.
+SHRIMP_DEV int64_t lane_i64(int64_t v, int src) {
+  return (int64_t)(unsigned)__builtin_amdgcn_ds_bpermute(src << 2, (int)v) |
+         (int64_t)__builtin_amdgcn_ds_bpermute(src << 2, (int)(v >> 32)) << 32;
+}
+
+// 16-byte pieces of a row of d elements as a product's operand (lane group lg), zeros
+// where `on` is false and past d.
+template <int D>
+SHRIMP_DEV void load_row(const uint16_t* row, bool on, int d, int lg, u32x4 (&f)[D / 32]) {
+#pragma unroll
+  for (int ks = 0; ks < D / 32; ++ks)
+    f[ks] = on && ks * 32 + lg * 8 < d ? *reinterpret_cast<const u32x4*>(row + ks * 32 + lg * 8)
+                                       : u32x4{0, 0, 0, 0};
+}
+
 template <int D>
 constexpr int row_floats() {
   return D + 4;  // rows 16 bytes apart in the banks
@@ -237,7 +287,7 @@ __global__ __launch_bounds__(64) void attn_blocks_kernel(const BlocksParams p) {
   const int lane = threadIdx.x, lr = lane & 15, lg = lane >> 4;
   int64_t bh;
   int chunk;
-  if (!place_chunk(p, bh, chunk)) return;
+  if (!place_chunk(p, p.chunks, bh, chunk)) return;
   const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
   const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
   const int q0 = chunk * p.queries;
@@ -257,76 +307,47 @@ __global__ __launch_bounds__(64) void attn_blocks_kernel(const BlocksParams p) {
   const uint16_t* v = p.v + b * p.v_sb + hk * p.v_sh;
   const int32_t* sel = p.sel + (bh * p.Sq + q0) * p.topk;
 
-  for (int w0 = 0; w0 < live; w0 += WINDOW) {
-    const int wn = min(WINDOW, live - w0);
-    fill_masks(p, sel, asking, w0, wn, mask_lds, lane);
-    for (int g0 = 0; g0 < wn; g0 += 64) {
-      unsigned mlo = 0, mhi = 0;
-      if (g0 + lane < wn) {
-        mlo = mask_lds[2 * (g0 + lane)];
-        mhi = mask_lds[2 * (g0 + lane) + 1];
-      }
-      uint64_t todo = __ballot((mlo | mhi) != 0);
-      while (todo) {
-        const int at = __builtin_ctzll(todo);
-        todo &= todo - 1;
-        const uint64_t mask = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)mhi, at) << 32 |
-                              (unsigned)__builtin_amdgcn_readlane((int)mlo, at);
-        const int count = __popcll(mask);
-        // lane j: the j-th row of the mask (the others behind them)
-        const bool in = mask >> lane & 1;
-        const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
-                                                     __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
-        const int row_at = __builtin_amdgcn_ds_permute((in ? before : count + lane - before) << 2, lane);
-        const int start = (w0 + g0 + at) * p.block;
-        for (int key0 = start; key0 < min(start + p.block, k_len); key0 += KT * 16) {
-          u32x4 kf[KT][KS];
-          load_rows<D, KT>(k, p.k_sn, key0, k_len, p.d, lr, lg, kf);
-          Turned<D, KT> vf;
-          vf.load(v, p.v_sn, key0, k_len, p.d, lr, lg);
-          f32x4 start_at[KT];
-          score_start<KT>(key0, k_len, lg, start_at);
-          for (int t = 0; t < count; t += 16) {
-            const int row = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at);
-            const int64_t off = (int64_t)(unsigned)__builtin_amdgcn_ds_bpermute(row << 2, (int)my_row) |
-                                (int64_t)__builtin_amdgcn_ds_bpermute(row << 2, (int)(my_row >> 32)) << 32;
-            const bool on = t + lr < count;
-            u32x4 qf[KS];
+  each_block(p, sel, asking, live, mask_lds, lane, nullptr, 0, [&](uint64_t mask, int row_at, int blk) {
+    const int count = __popcll(mask), start = blk * p.block;
+    for (int key0 = start; key0 < min(start + p.block, k_len); key0 += KT * 16) {
+      u32x4 kf[KT][KS];
+      load_rows<D, KT>(k, p.k_sn, key0, k_len, p.d, lr, lg, kf);
+      Turned<D, KT> vf;
+      vf.load(v, p.v_sn, key0, k_len, p.d, lr, lg);
+      f32x4 start_at[KT];
+      score_start<KT>(key0, k_len, lg, start_at);
+      for (int t = 0; t < count; t += 16) {
+        const int row = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at);
+        const bool on = t + lr < count;
+        u32x4 qf[KS];
+        load_row<D>(q + lane_i64(my_row, row), on, p.d, lg, qf);
+        float m = on ? m_lds[row] : -INFINITY, l = on ? l_lds[row] : 0.f;
+        f32x4 s[KT];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-              qf[ks] = on && ks * 32 + lg * 8 < p.d
-                           ? *reinterpret_cast<const u32x4*>(q + off + ks * 32 + lg * 8)
-                           : u32x4{0, 0, 0, 0};
-            float m = on ? m_lds[row] : -INFINITY, l = on ? l_lds[row] : 0.f;
-            f32x4 s[KT];
+        for (int kt = 0; kt < KT; ++kt) {
+          s[kt] = start_at[kt];
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-              s[kt] = start_at[kt];
+          for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], qf[ks], s[kt]);
+        }
+        u32x2 pk[KT];
+        const float alpha = soft_step<T, KT>(s, p.scale2, m, l, pk);
+        float* mine = acc_lds + row * RF + lg * EPL * 4;
+        f32x4 acc[EPL];
 #pragma unroll
-              for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], qf[ks], s[kt]);
-            }
-            u32x2 pk[KT];
-            const float alpha = soft_step<T, KT>(s, p.scale2, m, l, pk);
-            float* mine = acc_lds + row * RF + lg * EPL * 4;
-            f32x4 acc[EPL];
+        for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4) * alpha;
+        weigh<T, D, KT>(vf, pk, acc);
+        if (on) {
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4) * alpha;
-            weigh<T, D, KT>(vf, pk, acc);
-            if (on) {
-#pragma unroll
-              for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
-              if (lg == 0) {
-                m_lds[row] = m;
-                l_lds[row] = l;
-              }
-            }
-            __syncthreads();  // (one wave: the rows' state is read again by other lanes)
+          for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
+          if (lg == 0) {
+            m_lds[row] = m;
+            l_lds[row] = l;
           }
         }
+        __syncthreads();  // (one wave: the rows' state is read again by other lanes)
       }
     }
-    __syncthreads();
-  }
+  });
 
   // 16 lanes per row (D >= 64; four dimensions each), the rows' result and lse
   constexpr int LPR = D / 4;  // lanes per row
@@ -379,10 +400,7 @@ __global__ __launch_bounds__(QW * 64) void attn_blocks_query_kernel(const Blocks
     const bool on = g0 + lr < p.group;
     const uint16_t* q = p.q + b * p.q_sb + head * p.q_sh + (int64_t)i * p.q_sn;
     u32x4 qf[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      qf[ks] = on && ks * 32 + lg * 8 < p.d ? *reinterpret_cast<const u32x4*>(q + ks * 32 + lg * 8)
-                                            : u32x4{0, 0, 0, 0};
+    load_row<D>(q, on, p.d, lg, qf);
     float m = -INFINITY, l = 0.f;
     f32x4 acc[EPL];
 #pragma unroll
@@ -445,13 +463,325 @@ __global__ __launch_bounds__(QW * 64) void attn_blocks_query_kernel(const Blocks
   }
 }
 
+// ---- gradients ----------------------------------------------------------------------------------
+//
+// With p = exp(s - lse), delta_i = sum_d g_id out_id - g_lse_i and
+// ds_ij = p_ij (sum_d g_id v_jd - delta_i) / sqrt(d):
+//   dq_i = sum_j ds_ij k_j,   dk_j = sum_i ds_ij q_i,   dv_j = sum_i p_ij g_i,
+// the sums over a shared key head's queries of all its heads. Two kernels, each
+// computing the scores again: dq in the forward's chunks (accumulators in LDS), which
+// also leaves every block's row masks and every row's (lse, delta) behind; dk and dv
+// with a workgroup per run of keys, which gathers the rows of those masks, 32 to
+// a product, and keeps both accumulators in registers. Every sum has one order, so
+// gradients repeat bit for bit. p and ds are rounded once to the operands' type.
+
+struct GradParams {
+  const uint16_t* g;
+  const float* g_lse;  // or null
+  int64_t g_sb, g_sh, g_sn;
+  uint16_t* dq;
+  uint16_t* dk;
+  uint16_t* dv;
+  float2* stat;     // (B, H, Sq): lse log2(e) (+inf: no key), delta
+  uint64_t* masks;  // (B, Hk, NB, chunks)
+  float scale;
+  int nb, segments; // blocks; runs of keys per (sequence, key head)
+};
+
+template <typename T>
+SHRIMP_DEV float elem(unsigned word, int hi);
+template <>
+SHRIMP_DEV float elem<__bf16>(unsigned word, int hi) {
+  return hi ? bf16_hi(word) : bf16_lo(word);
+}
+template <>
+SHRIMP_DEV float elem<_Float16>(unsigned word, int hi) {
+  return (float)__builtin_bit_cast(f16x2, word)[hi];
+}
+
+template <typename T, int D, int KT>
+__global__ __launch_bounds__(64) void attn_blocks_dq_kernel(const BlocksParams p, const GradParams gp) {
+  extern __shared__ char lds[];
+  constexpr int RF = row_floats<D>(), EPL = D / 16, KS = D / 32;
+  float* acc_lds = reinterpret_cast<float*>(lds);
+  float2* stat_lds = reinterpret_cast<float2*>(acc_lds + R * RF);
+  unsigned* mask_lds = reinterpret_cast<unsigned*>(stat_lds + R);
+  const int lane = threadIdx.x, lr = lane & 15, lg = lane >> 4;
+  int64_t bh;
+  int chunk;
+  if (!place_chunk(p, p.chunks, bh, chunk)) return;
+  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
+  const int q0 = chunk * p.queries;
+  const int queries = min(p.queries, p.Sq - q0);
+  const int asking = min(queries, max(q_len - q0, 0));
+  const int live = (k_len + p.block - 1) / p.block;
+  const uint16_t* g = gp.g + b * gp.g_sb;
+
+  for (int i = lane; i < R * RF; i += 64) acc_lds[i] = 0.f;
+  constexpr int LPR = D / 4;  // lanes per row, four dimensions each
+  for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
+    const int r = r0 + lane / LPR, c = lane % LPR;
+    const bool on = r < queries * p.group;
+    const int query = on ? r / p.group : 0, head = hk * p.group + (on ? r - query * p.group : 0);
+    const int64_t o = ((int64_t)b * p.H + head) * p.Sq + q0 + query;
+    float delta = 0.f;
+    if (on && c * 4 < p.d) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p.out + o * p.d + c * 4);
+      const u32x2 y = *reinterpret_cast<const u32x2*>(g + head * gp.g_sh + (int64_t)(q0 + query) * gp.g_sn + c * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) delta = fmaf(elem<T>(x[e >> 1], e & 1), elem<T>(y[e >> 1], e & 1), delta);
+    }
+    for (int m = 1; m < LPR; m <<= 1) delta += xor_shfl(delta, m);
+    if (on && c == 0) {
+      if (gp.g_lse) delta -= gp.g_lse[o];
+      const float lse = p.lse[o];
+      const float2 st = {lse == -INFINITY ? INFINITY : lse * LOG2E, delta};
+      stat_lds[r] = st;
+      gp.stat[o] = st;
+    }
+  }
+  __syncthreads();
+
+  const int my_query = lane / p.group, my_head = hk * p.group + lane - my_query * p.group;
+  const int64_t my_row = my_head * p.q_sh + (int64_t)(q0 + my_query) * p.q_sn;
+  const int64_t my_grad = my_head * gp.g_sh + (int64_t)(q0 + my_query) * gp.g_sn;
+  const uint16_t* q = p.q + b * p.q_sb;
+  const uint16_t* k = p.k + b * p.k_sb + hk * p.k_sh;
+  const uint16_t* v = p.v + b * p.v_sb + hk * p.v_sh;
+  const int32_t* sel = p.sel + (bh * p.Sq + q0) * p.topk;
+  uint64_t* keep = gp.masks + bh * gp.nb * p.chunks + chunk;
+
+  each_block(p, sel, asking, live, mask_lds, lane, keep, p.chunks, [&](uint64_t mask, int row_at, int blk) {
+    const int count = __popcll(mask), start = blk * p.block;
+    for (int key0 = start; key0 < min(start + p.block, k_len); key0 += KT * 16) {
+      u32x4 kf[KT][KS], vf[KT][KS];
+      load_rows<D, KT>(k, p.k_sn, key0, k_len, p.d, lr, lg, kf);
+      load_rows<D, KT>(v, p.v_sn, key0, k_len, p.d, lr, lg, vf);
+      Turned<D, KT> kt_;
+      kt_.load(k, p.k_sn, key0, k_len, p.d, lr, lg);
+      f32x4 start_at[KT];
+      score_start<KT>(key0, k_len, lg, start_at);
+      for (int t = 0; t < count; t += 16) {
+        const int row = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at);
+        const bool on = t + lr < count;
+        u32x4 qf[KS], gf[KS];
+        load_row<D>(q + lane_i64(my_row, row), on, p.d, lg, qf);
+        load_row<D>(g + lane_i64(my_grad, row), on, p.d, lg, gf);
+        const float2 st = stat_lds[row];
+        u32x2 pk[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          f32x4 s = start_at[kt], dp = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) s = Mma<T>::k32(kf[kt][ks], qf[ks], s);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) dp = Mma<T>::k32(vf[kt][ks], gf[ks], dp);
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -st.x)) * gp.scale * (dp[i] - st.y);
+          pk[kt] = u32x2{Mma<T>::pack(w[0], w[1]), Mma<T>::pack(w[2], w[3])};
+        }
+        float* mine = acc_lds + row * RF + lg * EPL * 4;
+        f32x4 acc[EPL];
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4);
+        weigh<T, D, KT>(kt_, pk, acc);
+        if (on) {
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
+        }
+        __syncthreads();
+      }
+    }
+  });
+
+  __syncthreads();
+  for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
+    const int r = r0 + lane / LPR, c = lane % LPR;
+    if (r >= queries * p.group || c * 4 >= p.d) continue;
+    const int query = r / p.group, head = hk * p.group + r - query * p.group;
+    const int64_t o = ((int64_t)b * p.H + head) * p.Sq + q0 + query;
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int dim = c * 4 + e, rr = dim / EPL, ee = dim % EPL;
+      x[e] = acc_lds[r * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3)];
+    }
+    *reinterpret_cast<u32x2*>(gp.dq + o * p.d + c * 4) =
+        u32x2{Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3])};
+  }
+}
+
+constexpr int GW = 4;  // waves of a workgroup at most
+
+// One workgroup: KT tiles of 16 keys of one block. Its waves take every GW-th word of the
+// block's row masks (a word: the 64 rows of a chunk), 64 words at a time, list their
+// rows in LDS and go through them 32 at a time; at the end the waves' sums are added in
+// wave order.
+template <typename T, int D, int KT>
+__global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksParams p, const GradParams gp) {
+  constexpr int EPL = D / 16, KS = D / 32, W = EPL / 2;
+  // the lists, and at the end the sums: KT 16 keys x D dimensions x 2
+  extern __shared__ char lds[];
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4, wave = wave_id();
+  const int waves = blockDim.x >> 6;
+  uint16_t* list = reinterpret_cast<uint16_t*>(lds) + wave * (64 * 64);
+  int64_t bh;
+  int seg;
+  if (!place_chunk(p, gp.segments, bh, seg)) return;
+  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  const int k_len = min(max(p.k_lens[b], 0), p.Sk);
+  const int key0 = seg * KT * 16, blk = key0 / p.block;
+  const uint16_t* q = p.q + b * p.q_sb + hk * p.group * p.q_sh;
+  const uint16_t* g = gp.g + b * gp.g_sb + hk * p.group * gp.g_sh;
+  const float2* stat = gp.stat + ((int64_t)b * p.H + hk * p.group) * p.Sq;
+
+  f32x4 dk[KT][EPL], dv[KT][EPL];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) dk[kt][e] = dv[kt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (key0 < k_len) {
+    u32x4 kf[KT][KS], vf[KT][KS];
+    load_rows<D, KT>(p.k + b * p.k_sb + hk * p.k_sh, p.k_sn, key0, k_len, p.d, lr, lg, kf);
+    load_rows<D, KT>(p.v + b * p.v_sb + hk * p.v_sh, p.v_sn, key0, k_len, p.d, lr, lg, vf);
+    f32x4 start_at[KT];  // the lane's key (column lr of each tile)
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const float c = key0 + kt * 16 + lr < k_len ? 0.f : -INFINITY;
+      start_at[kt] = f32x4{c, c, c, c};
+    }
+    const uint64_t* masks = gp.masks + (bh * gp.nb + blk) * p.chunks;
+    for (int c0 = 0; c0 < p.chunks; c0 += 64 * waves) {
+      // list entries: lane of the word, row of its chunk
+      const int word = c0 + lane * waves + wave;
+      uint64_t m = word < p.chunks ? masks[word] : 0;
+      int at = __popcll(m);
+      const int mine = at;
+#pragma unroll
+      for (int s = 1; s < 64; s <<= 1) {
+        const int o = __shfl_up(at, s, 64);
+        if (lane >= s) at += o;
+      }
+      const int count = __shfl(at, 63, 64);
+      at -= mine;
+      while (m) {
+        list[at++] = (uint16_t)(lane << 6 | __builtin_ctzll(m));
+        m &= m - 1;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      for (int t = 0; t < count; t += 32) {
+        // (query, head) of entry i, -1 past the list
+        auto locate = [&](int i, int& query, int& head) {
+          const bool on = i < count;
+          const int e = on ? list[i] : 0;
+          const int r = e & 63, qi = r / p.group;
+          query = on ? (c0 + (e >> 6) * waves + wave) * p.queries + qi : -1;
+          head = r - qi * p.group;
+        };
+        u32x4 qf[2][KS], gf[2][KS];
+        Words<W> qt[2][4], gt[2][4];
+        float2 st[2][4];
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+          int query, head;
+          locate(t + rt * 16 + lr, query, head);
+          load_row<D>(q + head * p.q_sh + (int64_t)query * p.q_sn, query >= 0, p.d, lg, qf[rt]);
+          load_row<D>(g + head * gp.g_sh + (int64_t)query * gp.g_sn, query >= 0, p.d, lg, gf[rt]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            locate(t + rt * 16 + lg * 4 + j, query, head);
+            const bool on = query >= 0, wide = on && lr * EPL < p.d;
+            qt[rt][j] = wide ? *reinterpret_cast<const Words<W>*>(q + head * p.q_sh + (int64_t)query * p.q_sn + lr * EPL)
+                             : (Words<W>)0u;
+            gt[rt][j] = wide ? *reinterpret_cast<const Words<W>*>(g + head * gp.g_sh + (int64_t)query * gp.g_sn + lr * EPL)
+                             : (Words<W>)0u;
+            st[rt][j] = on ? stat[(int64_t)head * p.Sq + query] : float2{INFINITY, 0.f};
+          }
+        }
+        auto turn = [&](const Words<W> (&x)[2][4], int e) {
+          const unsigned s = e & 1 ? SEL_HI : SEL_LO;
+          const int w = e >> 1;
+          return u32x4{perm(x[0][1][w], x[0][0][w], s), perm(x[0][3][w], x[0][2][w], s),
+                       perm(x[1][1][w], x[1][0][w], s), perm(x[1][3][w], x[1][2][w], s)};
+        };
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          u32x4 pp, ds;
+#pragma unroll
+          for (int rt = 0; rt < 2; ++rt) {
+            f32x4 s = start_at[kt], dp = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s = Mma<T>::k32(qf[rt][ks], kf[kt][ks], s);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) dp = Mma<T>::k32(gf[rt][ks], vf[kt][ks], dp);
+            float w[4], x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -st[rt][i].x));
+              x[i] = w[i] * gp.scale * (dp[i] - st[rt][i].y);
+            }
+            pp[2 * rt] = Mma<T>::pack(w[0], w[1]);
+            pp[2 * rt + 1] = Mma<T>::pack(w[2], w[3]);
+            ds[2 * rt] = Mma<T>::pack(x[0], x[1]);
+            ds[2 * rt + 1] = Mma<T>::pack(x[2], x[3]);
+          }
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) {
+            dv[kt][e] = Mma<T>::k32(turn(gt, e), pp, dv[kt][e]);
+            dk[kt][e] = Mma<T>::k32(turn(qt, e), ds, dk[kt][e]);
+          }
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+  }
+
+  // sums of the waves, in their order: [tensor][key][RF], per key lane group, e, i
+  constexpr int RF = row_floats<D>();
+  float* sum = reinterpret_cast<float*>(lds);
+  for (int w = 0; w < waves; ++w) {
+    __syncthreads();
+    if (wave != w) continue;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        f32x4* a = reinterpret_cast<f32x4*>(sum + (kt * 16 + lr) * RF + (lg * EPL + e) * 4);
+        f32x4* c = reinterpret_cast<f32x4*>(sum + (KT * 16 + kt * 16 + lr) * RF + (lg * EPL + e) * 4);
+        *a = w ? *a + dk[kt][e] : dk[kt][e];
+        *c = w ? *c + dv[kt][e] : dv[kt][e];
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * KT * 16 * (D / 4); i += blockDim.x) {
+    const int c = i % (D / 4), row = i / (D / 4), key = key0 + row % (KT * 16);
+    if (c * 4 >= p.d || key >= p.Sk) continue;
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int dim = c * 4 + e, rr = dim / EPL, ee = dim % EPL;
+      x[e] = sum[row * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3)];
+    }
+    uint16_t* out = (row < KT * 16 ? gp.dk : gp.dv) + (bh * p.Sk + key) * p.d + c * 4;
+    *reinterpret_cast<u32x2*>(out) = u32x2{Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3])};
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------
 
 // Few enough queries that a workgroup for each (its tile holding the G heads alone)
 // beats waves that go through every block for 64 rows.
 constexpr int FEW_QUERIES = 8;
 
-int check_blocks(const shrimp_attn_blocks_args* a, const char* what) {
+int check_blocks(const shrimp_attn_blocks_args* a, bool back, const char* what) {
   SHRIMP_REQUIRE(a != nullptr, "%s: null arguments", what);
   SHRIMP_REQUIRE(a->dt == SHRIMP_DT_BF16 || a->dt == SHRIMP_DT_F16, "%s: element type %d", what, a->dt);
   SHRIMP_REQUIRE(a->B >= 0 && a->H >= 0 && a->Sq >= 0 && a->Sk >= 0, "%s: negative size", what);
@@ -465,14 +795,16 @@ int check_blocks(const shrimp_attn_blocks_args* a, const char* what) {
                  a->topk, SHRIMP_BLOCK_MAX_TOPK);
   SHRIMP_REQUIRE(a->Sq <= (1 << 30) && a->Sk <= (1 << 30), "%s: Sq=%d, Sk=%d", what, a->Sq, a->Sk);
   SHRIMP_REQUIRE(a->scale > 0.f, "%s: scale must be positive", what);
-  if (a->B == 0 || a->H == 0 || a->Sq == 0) return SHRIMP_OK;
   auto aligned = [](const void* base, int64_t sb, int64_t sh, int64_t sn) {
     return reinterpret_cast<uintptr_t>(base) % 16 == 0 && sb % 8 == 0 && sh % 8 == 0 && sn % 8 == 0;
   };
-  SHRIMP_REQUIRE(a->q && a->sel && a->q_lens && a->k_lens && a->out && a->lse, "%s: null pointer", what);
-  SHRIMP_REQUIRE(a->Sk == 0 || (a->k && a->v), "%s: null k or v", what);
-  SHRIMP_REQUIRE(aligned(a->q, a->q_sb, a->q_sh, a->q_sn) && aligned(a->k, a->k_sb, a->k_sh, a->k_sn) &&
-                     aligned(a->v, a->v_sb, a->v_sh, a->v_sn) && aligned(a->out, 0, 0, 0),
+  const bool rows = a->B > 0 && a->H > 0 && a->Sq > 0, keys = a->B > 0 && a->Sk > 0 && (rows || back);
+  SHRIMP_REQUIRE(!rows || (a->q && a->sel && a->q_lens && a->k_lens && a->out && a->lse),
+                 "%s: null pointer", what);
+  SHRIMP_REQUIRE(!keys || (a->k && a->v && a->k_lens), "%s: null k, v or k_lens", what);
+  SHRIMP_REQUIRE(!rows || (aligned(a->q, a->q_sb, a->q_sh, a->q_sn) && aligned(a->out, 0, 0, 0)),
+                 "%s: rows must start on 16-byte boundaries", what);
+  SHRIMP_REQUIRE(!keys || (aligned(a->k, a->k_sb, a->k_sh, a->k_sn) && aligned(a->v, a->v_sb, a->v_sh, a->v_sn)),
                  "%s: rows must start on 16-byte boundaries", what);
   return SHRIMP_OK;
 }
@@ -493,7 +825,7 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a) {
   p.B = a->B, p.H = a->H, p.Hk = a->Hk, p.Sq = a->Sq, p.Sk = a->Sk;
   p.d = a->d, p.block = a->block, p.topk = a->topk;
   p.group = a->H / a->Hk;
-  p.queries = R / p.group;
+  p.queries = p.group > 0 ? R / p.group : R;
   p.chunks = (a->Sq + p.queries - 1) / p.queries;
   const int64_t pairs = (int64_t)a->B * a->Hk;
   p.by_xcd = pairs % 8 == 0 || pairs >= 64;
@@ -531,12 +863,63 @@ int launch_forward_d(const BlocksParams& p, hipStream_t st) {
   return launch_forward_kt<T, 128>(p, st);
 }
 
+int64_t grad_stat_bytes(const shrimp_attn_blocks_args* a) {
+  return mul_sat({a->B, a->H, a->Sq, 8});
+}
+int64_t grad_mask_bytes(const shrimp_attn_blocks_args* a) {
+  const BlocksParams p = blocks_params(a);
+  return mul_sat({a->B, a->Hk, ((int64_t)a->Sk + a->block - 1) / a->block, p.chunks, 8});
+}
+
+// Keys a workgroup of the dk / dv kernel takes: their two accumulators fill 128 registers.
+template <int D, int KT>
+constexpr int key_tiles() {
+  return D == 128 && KT == 4 ? 2 : KT;
+}
+
+template <typename T, int D, int KT>
+int launch_backward(const BlocksParams& p, GradParams gp, hipStream_t st) {
+  constexpr int KG = key_tiles<D, KT>();
+  const int64_t pairs = (int64_t)p.B * p.Hk, sets = p.by_xcd ? (pairs + 7) / 8 * 8 : pairs;
+  const int64_t n = sets * p.chunks;
+  gp.segments = (p.Sk + KG * 16 - 1) / (KG * 16);
+  const int64_t m = sets * gp.segments;
+  SHRIMP_REQUIRE(n <= INT32_MAX && m <= INT32_MAX, "attn_blocks_backward: %lld chunks of queries, %lld of keys",
+                 (long long)n, (long long)m);
+  const size_t lds = (size_t)R * (row_floats<D>() + 2) * 4 + (size_t)WINDOW * 8;
+  if (n > 0)
+    hipLaunchKernelGGL((attn_blocks_dq_kernel<T, D, KT>), dim3((unsigned)n), dim3(64), lds, st, p, gp);
+  if (m > 0) {
+    // waves by the rows that a block has on average: tiles of 32 that stay full
+    const int64_t rows = (int64_t)p.Sq * p.group * p.topk / (gp.nb > 0 ? gp.nb : 1);
+    const int waves = rows >= 256 ? GW : rows >= 128 ? 2 : 1;
+    const size_t list = (size_t)waves * 64 * 64 * 2, sum = (size_t)2 * KG * 16 * row_floats<D>() * 4;
+    hipLaunchKernelGGL((attn_blocks_dkv_kernel<T, D, KG>), dim3((unsigned)m), dim3(waves * 64),
+                       list > sum ? list : sum, st, p, gp);
+  }
+  return SHRIMP_OK;
+}
+
+template <typename T, int D>
+int launch_backward_kt(const BlocksParams& p, const GradParams& gp, hipStream_t st) {
+  if (p.block % 64 == 0) return launch_backward<T, D, 4>(p, gp, st);
+  if (p.block % 32 == 0) return launch_backward<T, D, 2>(p, gp, st);
+  return launch_backward<T, D, 1>(p, gp, st);
+}
+
+template <typename T>
+int launch_backward_d(const BlocksParams& p, const GradParams& gp, hipStream_t st) {
+  if (p.d <= 32) return launch_backward_kt<T, 32>(p, gp, st);
+  if (p.d <= 64) return launch_backward_kt<T, 64>(p, gp, st);
+  return launch_backward_kt<T, 128>(p, gp, st);
+}
+
 }  // namespace
 }  // namespace shrimp
 
 extern "C" int shrimp_attn_blocks(const shrimp_attn_blocks_args* a, void* stream) {
   using namespace shrimp;
-  const int rc = check_blocks(a, "attn_blocks");
+  const int rc = check_blocks(a, false, "attn_blocks");
   if (rc != SHRIMP_OK) return rc;
   if (a->B == 0 || a->H == 0 || a->Sq == 0) return SHRIMP_OK;
   const BlocksParams p = blocks_params(a);
@@ -544,4 +927,48 @@ extern "C" int shrimp_attn_blocks(const shrimp_attn_blocks_args* a, void* stream
                                        : launch_forward_d<__bf16>(p, as_stream(stream));
   if (e != SHRIMP_OK) return e;
   return check_launch("attn_blocks");
+}
+
+extern "C" int64_t shrimp_attn_blocks_workspace(const shrimp_attn_blocks_args* a) {
+  using namespace shrimp;
+  if (check_blocks(a, true, "attn_blocks_workspace") != SHRIMP_OK) return -1;
+  const int64_t stat = grad_stat_bytes(a), mask = grad_mask_bytes(a);
+  return stat > INT64_MAX - mask ? INT64_MAX : stat + mask;
+}
+
+extern "C" int shrimp_attn_blocks_backward(const shrimp_attn_blocks_args* a,
+                                           const shrimp_attn_blocks_grads* g, void* stream) {
+  using namespace shrimp;
+  const int rc = check_blocks(a, true, "attn_blocks_backward");
+  if (rc != SHRIMP_OK) return rc;
+  SHRIMP_REQUIRE(g != nullptr, "attn_blocks_backward: null gradients");
+  if (a->B == 0) return SHRIMP_OK;
+  const bool rows = a->H > 0 && a->Sq > 0;
+  SHRIMP_REQUIRE(!rows || (g->g && g->dq), "attn_blocks_backward: null gradient of out or q");
+  SHRIMP_REQUIRE(a->Sk == 0 || (g->dk && g->dv), "attn_blocks_backward: null gradient of k or v");
+  SHRIMP_REQUIRE(reinterpret_cast<uintptr_t>(g->g) % 16 == 0 && g->g_sb % 8 == 0 && g->g_sh % 8 == 0 &&
+                     g->g_sn % 8 == 0 && reinterpret_cast<uintptr_t>(g->dq) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(g->dk) % 16 == 0 && reinterpret_cast<uintptr_t>(g->dv) % 16 == 0,
+                 "attn_blocks_backward: gradients must start on 16-byte boundaries");
+  const int64_t stat = grad_stat_bytes(a), mask = grad_mask_bytes(a);
+  SHRIMP_REQUIRE(g->workspace_bytes >= stat && g->workspace_bytes - stat >= mask &&
+                     (g->workspace || stat + mask == 0) && reinterpret_cast<uintptr_t>(g->workspace) % 8 == 0,
+                 "attn_blocks_backward: workspace of %lld bytes, %lld + %lld needed",
+                 (long long)g->workspace_bytes, (long long)stat, (long long)mask);
+  const BlocksParams p = blocks_params(a);
+  GradParams gp{};
+  gp.g = static_cast<const uint16_t*>(g->g);
+  gp.g_lse = g->g_lse;
+  gp.g_sb = g->g_sb, gp.g_sh = g->g_sh, gp.g_sn = g->g_sn;
+  gp.dq = static_cast<uint16_t*>(g->dq);
+  gp.dk = static_cast<uint16_t*>(g->dk);
+  gp.dv = static_cast<uint16_t*>(g->dv);
+  gp.stat = static_cast<float2*>(g->workspace);
+  gp.masks = reinterpret_cast<uint64_t*>(static_cast<char*>(g->workspace) + stat);
+  gp.scale = a->scale;
+  gp.nb = (a->Sk + a->block - 1) / a->block;
+  const int e = a->dt == SHRIMP_DT_F16 ? launch_backward_d<_Float16>(p, gp, as_stream(stream))
+                                       : launch_backward_d<__bf16>(p, gp, as_stream(stream));
+  if (e != SHRIMP_OK) return e;
+  return check_launch("attn_blocks_backward");
 }

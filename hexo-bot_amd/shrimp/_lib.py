@@ -174,6 +174,13 @@ class AttnBlocksArgs(ctypes.Structure):
     ]
 
 
+class AttnBlocksGrads(ctypes.Structure):
+    _fields_ = [
+        ("g", _vp), ("g_sb", _i64), ("g_sh", _i64), ("g_sn", _i64), ("g_lse", _vp),
+        ("dq", _vp), ("dk", _vp), ("dv", _vp), ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
 # Exported symbols and their ctypes signatures; tests check every one of them
 # against the header and the built library.
 SIGNATURES: dict = {
@@ -276,6 +283,10 @@ SIGNATURES: dict = {
     ),
     "shrimp_block_select": (ctypes.c_int, [ctypes.POINTER(BlockSelectArgs), _vp]),
     "shrimp_attn_blocks": (ctypes.c_int, [ctypes.POINTER(AttnBlocksArgs), _vp]),
+    "shrimp_attn_blocks_workspace": (_i64, [ctypes.POINTER(AttnBlocksArgs)]),
+    "shrimp_attn_blocks_backward": (
+        ctypes.c_int, [ctypes.POINTER(AttnBlocksArgs), ctypes.POINTER(AttnBlocksGrads), _vp]
+    ),
 }
 
 _LIB = None

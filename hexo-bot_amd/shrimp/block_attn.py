@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -254,9 +254,30 @@ def _attn_fake(q, k, v, sel, q_lens, k_lens, block):
     return q.new_empty(q.shape), q.new_empty(q.shape[:3], dtype=torch.float32)
 
 
+class _AttnBlocks(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, sel, q_lens, k_lens, block):
+        out, lse = below(_attn_blocks, q, k, v, sel, q_lens, k_lens, block)
+        ctx.save_for_backward(q, k, v, sel, q_lens, k_lens, out, lse)
+        ctx.block = block
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, g_lse):
+        if g is None and g_lse is None:
+            return (None,) * 7
+        out = ctx.saved_tensors[6]
+        if g is None:
+            g = torch.zeros_like(out)
+        grads = _attn_blocks_backward(g, g_lse, *ctx.saved_tensors, ctx.block)
+        return (*grads, None, None, None, None)
+
+
 _attn_blocks = define(
     "attn_blocks(Tensor q, Tensor k, Tensor v, Tensor sel, Tensor q_lens, Tensor k_lens, int block)"
-    " -> (Tensor, Tensor)", _attn_kernel, _attn_fake)
+    " -> (Tensor, Tensor)", _attn_kernel, _attn_fake, _AttnBlocks)
 
 
 def attn_blocks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sel: torch.Tensor,
@@ -269,3 +290,51 @@ def attn_blocks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sel: torch.Te
     and v bfloat16 or float16, H a multiple of Hk; block a multiple of 16."""
 
     return _attn_blocks(q, k, v, sel, q_lens, k_lens, block)
+
+
+def _attn_back_kernel(g, g_lse, q, k, v, sel, q_lens, k_lens, out, lse, block):
+    what = "shrimp::attn_blocks_backward"
+    d = q.shape[-1]
+    for name, t, like in (("g", g, q), ("out", out, q)):
+        if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+            raise ValueError(f"{what}: {name} {t.dtype} {tuple(t.shape)} on {t.device} for q "
+                             f"{like.dtype} {tuple(like.shape)} on {like.device}")
+    for name, t in (("lse", lse), ("g_lse", g_lse)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != q.shape[:3] or t.device != q.device):
+            raise ValueError(f"{what}: {name} {t.dtype} {tuple(t.shape)} on {t.device}")
+    q, k, v, sel, ql, kl = _attn_args(what, q, k, v, sel, q_lens, k_lens, block)
+    d8 = q.shape[3]
+    g, out = _aligned(g, d8), _aligned(out, d8).contiguous()
+    lse = lse.contiguous()
+    g_lse = None if g_lse is None else g_lse.contiguous()
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
+    a = _attn_struct(q, k, v, sel, ql, kl, out, lse, block, d)
+    lib = _lib.load()
+    n = lib.shrimp_attn_blocks_workspace(ctypes.byref(a))
+    ws = torch.empty(max(n, 0), dtype=torch.uint8, device=q.device)
+    gr = _lib.AttnBlocksGrads(g.data_ptr(), *g.stride()[:3], _lib.ptr(g_lse), dq.data_ptr(),
+                              dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n)
+    _lib.launch(lib.shrimp_attn_blocks_backward, q.device, what, ctypes.byref(a), ctypes.byref(gr))
+    return tuple(t if d8 == d else t[..., :d].contiguous() for t in (dq, dk, dv))
+
+
+def _attn_back_fake(g, g_lse, q, k, v, sel, q_lens, k_lens, out, lse, block):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+
+_attn_blocks_backward = define(
+    "attn_blocks_backward(Tensor g, Tensor? g_lse, Tensor q, Tensor k, Tensor v, Tensor sel,"
+    " Tensor q_lens, Tensor k_lens, Tensor out, Tensor lse, int block) -> (Tensor, Tensor, Tensor)",
+    _attn_back_kernel, _attn_back_fake)
+
+
+def attn_blocks_backward(g: torch.Tensor, g_lse: Optional[torch.Tensor], q: torch.Tensor,
+                         k: torch.Tensor, v: torch.Tensor, sel: torch.Tensor, q_lens: torch.Tensor,
+                         k_lens: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, block: int
+                         ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of q, k and v from those of attn_blocks' results (that of lse may be None),
+    its arguments and its results. Every sum has a fixed order: the same call gives the same
+    bits."""
+
+    return _attn_blocks_backward(g, g_lse, q, k, v, sel, q_lens, k_lens, out, lse, block)

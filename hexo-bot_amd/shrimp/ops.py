@@ -576,6 +576,7 @@ def _attn_pair_fake(q, k, v, pair, table2, seq_lens):
 
 from .block_attn import (  # noqa: E402,F401
     attn_blocks,
+    attn_blocks_backward,
     block_means,
     block_means_update,
     block_select,

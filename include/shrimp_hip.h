@@ -883,6 +883,28 @@ typedef struct {
 
 int shrimp_attn_blocks(const shrimp_attn_blocks_args* a, void* stream);
 
+/* Its gradients: the arguments of the forward call with the out and lse it wrote,
+ * g (B, H, Sq, d) of type dt, the gradient of out (strides multiples of 8, 16-byte
+ * aligned), and g_lse (B, H, Sq) fp32 contiguous, that of lse, or NULL. dq (B, H,
+ * Sq, d), dk and dv (B, Hk, Sk, d) of type dt, contiguous, written whole (zeros
+ * where nothing flows); every sum in a fixed order. workspace: at least
+ * shrimp_attn_blocks_workspace(a) bytes (-1 for arguments it refuses), 8-byte
+ * aligned, used only during the call's launches. */
+typedef struct {
+  const void* g;
+  int64_t g_sb, g_sh, g_sn;
+  const float* g_lse;
+  void* dq;
+  void* dk;
+  void* dv;
+  void* workspace;
+  int64_t workspace_bytes;
+} shrimp_attn_blocks_grads;
+
+int64_t shrimp_attn_blocks_workspace(const shrimp_attn_blocks_args* a);
+int shrimp_attn_blocks_backward(const shrimp_attn_blocks_args* a, const shrimp_attn_blocks_grads* g,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

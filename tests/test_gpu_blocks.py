@@ -288,3 +288,288 @@ def test_rows_do_not_depend_on_the_batch():
     for i in (0, 4, 8):
         one = run(slice(i, i + 1))
         assert all(torch.equal(a[i : i + 1], c) for a, c in zip(full, one))
+
+
+# ---- gradients -----------------------------------------------------------------------------
+
+
+def _grad_want(q, k, v, sel, ql, kl, block, g, g_lse, dt):
+    """Float64 gradients and their bounds: p is off by rp relative (E for the score and for
+    lse, see above) and by H where it is an operand; dp by (d + 2) U of its magnitudes;
+    delta by g times the bound and the rounding of out; ds by these and H; sums by a step
+    of U per term."""
+    b, h, nq, d = q.shape
+    hk, n = k.shape[1:3]
+    half, scale = torch.finfo(dt).eps / 2, 1 / math.sqrt(d)
+    out, ob, lse, _ = _attend_want(q, k, v, sel, ql, kl, block, dt)
+    dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    eq, ek, ev = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    for i in range(b):
+        m = min(max(kl[i], 0), n)
+        for j in range(h):
+            c = j // (h // hk)
+            seen = torch.zeros(nq, m, dtype=torch.bool)
+            for row in range(min(max(ql[i], 0), nq)):
+                for blk in sel[i, c, row].tolist():
+                    if 0 <= blk < -(-m // block):
+                        seen[row, blk * block : (blk + 1) * block] = True
+            if not seen.any():
+                continue
+            qq, kk, vv, gg = q[i, j], k[i, c, :m], v[i, c, :m], g[i, j]
+            s = (qq @ kk.T * scale).masked_fill(~seen, 0)
+            p = torch.where(seen, torch.exp(s - lse[i, j][:, None]), 0.0)
+            e = (qq.abs() @ kk.T.abs() * scale * (d + 2) * U).masked_fill(~seen, 0).amax(-1, keepdim=True)
+            rp = 2 * e + (seen.sum(1, keepdim=True) + 90 + 8 * s.abs().amax(-1, keepdim=True)) * U
+            tiny = 2.0**-25 if dt == torch.float16 else 0.0
+            dp, edp = gg @ vv.T, (d + 2) * U * (gg.abs() @ vv.abs().T)
+            delta = (gg * out[i, j]).sum(-1, keepdim=True) - g_lse[i, j][:, None]
+            edelta = (gg.abs() * (ob[i, j] + half * out[i, j].abs())).sum(-1, keepdim=True) + (d + 4) * U * (
+                (gg * out[i, j]).abs().sum(-1, keepdim=True) + g_lse[i, j].abs()[:, None])
+            ds = p * scale * (dp - delta)
+            eds = p * scale * ((dp.abs() + delta.abs()) * (rp + 6 * U) + edp + edelta) + half * ds.abs() + tiny * seen
+            rows = seen.any(1, keepdim=True)
+            dq[i, j] = torch.where(rows, ds @ kk, 0.0)
+            eq[i, j] = torch.where(rows, eds @ kk.abs() + (m + 8) * U * (ds.abs() @ kk.abs()), 0.0)
+            dk[i, c, :m] += ds.T @ qq
+            ek[i, c, :m] += eds.T @ qq.abs() + (nq * (h // hk) + 8) * U * (ds.abs().T @ qq.abs())
+            dv[i, c, :m] += p.T @ gg
+            ev[i, c, :m] += (p * (rp + half) + tiny * seen).T @ gg.abs() + (nq * (h // hk) + 8) * U * (p.T @ gg.abs())
+    return (dq, eq), (dk, ek), (dv, ev)
+
+
+def _check_grads(q, k, v, sel, ql, kl, block, g, g_lse):
+    dt = q.dtype
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    out, lse = ops.attn_blocks(q, k, v, sel, _lens(*ql), _lens(*kl), block)
+    if g_lse is None:
+        grads = torch.autograd.grad(out, [q, k, v], g)
+    else:
+        grads = torch.autograd.grad([out, lse], [q, k, v], [g, g_lse])
+    gl = torch.zeros(q.shape[:3], dtype=torch.float64) if g_lse is None else g_lse.cpu().double()
+    clean = lambda t, lens: torch.stack([torch.where(torch.arange(t.shape[2])[:, None] < lens[i], t[i], 0.0)
+                                         for i in range(t.shape[0])])
+    want = _grad_want(q.detach().cpu().double(), clean(k.detach().cpu().double(), kl),
+                      clean(v.detach().cpu().double(), kl), sel.cpu(), ql, kl, block, g.cpu().double(), gl, dt)
+    for name, got, (x, err) in zip("qkv", grads, want):
+        assert got.dtype == dt and got.shape == x.shape
+        y = got.cpu().double()
+        tol = err + (x.abs() + err) * torch.finfo(dt).eps / 2 + torch.finfo(dt).smallest_normal
+        bad = ~((y - x).abs() <= tol)
+        assert not bad.any(), (name, int(bad.sum()), ((y - x).abs() / tol).max().item())
+    return grads
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", ATTN, ids=str)
+def test_gradients(shape, dt):
+    b, h, hk, sq, sk, d, block, topk, layout = shape
+    gen = _gen(8)
+    q, k, v = (_heads(gen, b, n, s, d, dt, layout) for n, s in ((h, sq), (hk, sk), (hk, sk)))
+    kl = [sk, max(sk - block - 3, 1), 1][:b]
+    ql = [sq, max(sq - 2, 1), sq][:b]
+    for i, x in enumerate(kl):
+        k[i, :, x:], v[i, :, x:] = float("nan"), float("inf")
+    g = _heads(gen, b, h, sq, d, dt, layout)
+    means = ops.block_means(k, _lens(*kl), block)
+    sel = ops.block_select(q, means, _lens(*ql), _lens(*kl), block, topk)
+    first = _check_grads(q, k, v, sel, ql, kl, block, g, None)
+    again = _check_grads(q, k, v, sel, ql, kl, block, g, None)
+    assert all(torch.equal(a, c) for a, c in zip(first, again))
+    nb = -(-sk // block)
+    sel = torch.randint(-2, nb + 2, (b, hk, sq, topk), generator=gen, dtype=torch.int32)
+    sel[:, :, ::5] = -1
+    sel[..., topk // 2] = sel[..., 0]
+    _check_grads(q, k, v, sel.to(DEV), ql, kl, block, g, torch.randn(b, h, sq, generator=gen).to(DEV))
+
+
+def test_gradients_of_empty_rows():
+    """Nothing flows from rows without a key or past q_lens, whatever their gradient."""
+    gen = _gen(9)
+    b, h, hk, sq, sk, d, block = 3, 2, 1, 40, 50, 64, 16
+    q, k, v = (_heads(gen, b, n, s, d, torch.bfloat16) for n, s in ((h, sq), (hk, sk), (hk, sk)))
+    sel = torch.zeros(b, hk, sq, 2, dtype=torch.int32, device=DEV)
+    sel[:, :, ::2] = -1
+    g = _heads(gen, b, h, sq, d, torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    lens = (_lens(sq, 10, 0), _lens(0, 20, sk))
+    out, lse = ops.attn_blocks(*leaves, sel, *lens, block)
+    clean = torch.autograd.grad(out, leaves, g, retain_graph=True)
+    g[:, :, ::2], g[0], g[1, :, 10:], g[2] = (float("nan"),) * 4
+    grads = torch.autograd.grad(out, leaves, g)
+    assert all(torch.equal(a, c) for a, c in zip(clean, grads))
+    assert all((t[0] == 0).all() and (t[2] == 0).all() for t in grads)
+    assert (grads[0][1, :, 1:10:2] != 0).any() and (grads[1][1, :, 16:] == 0).all()
+    # no queries: the keys' gradients are zeros; no keys: the queries'
+    e = ops.attn_blocks_backward(g[:, :, :0], None, q[:, :, :0], k, v, sel[:, :, :0], *lens,
+                                 out[:, :, :0], lse[:, :, :0], block)
+    assert (e[1] == 0).all() and (e[2] == 0).all()
+    e = ops.attn_blocks_backward(g, None, q, k[:, :, :0], v[:, :, :0], sel, *lens, out, lse, block)
+    assert (e[0] == 0).all() and e[1].shape == (b, hk, 0, d)
+
+
+def test_gradient_against_differences():
+    """Directional derivatives of a weighted sum of out and lse against central differences
+    of the float64 restatement at a fixed choice (fp16 operands: each gradient's own bounds,
+    H and some roundings, stay below 1e-2 of the sum of magnitudes)."""
+    gen = _gen(10)
+    b, h, hk, s, d, block = 1, 4, 2, 60, 32, 16
+    q, k, v = (_heads(gen, b, n, s, d, torch.float16).requires_grad_() for n in (h, hk, hk))
+    sel = torch.randint(0, 4, (b, hk, s, 2), generator=gen, dtype=torch.int32)
+    out, lse = ops.attn_blocks(q, k, v, sel.to(DEV), _lens(s), _lens(s), block)
+    g = torch.randn(out.shape, generator=gen).half()
+    gl = torch.randn(lse.shape, generator=gen)
+    grads = torch.autograd.grad([out, lse], [q, k, v], [g.to(DEV), gl.to(DEV)])
+    base = [t.detach().cpu().double() for t in (q, k, v)]
+    for i in range(3):
+        d_i = torch.randn(base[i].shape, generator=gen).double()
+
+        def f(t):
+            x = [c + t * d_i if j == i else c for j, c in enumerate(base)]
+            o, _, ls, _ = _attend_want(*x, sel, [s], [s], block, torch.float16)
+            return (o * g.double()).sum() + (ls * gl.double()).sum()
+
+        want = ((f(1e-5) - f(-1e-5)) / 2e-5).item()
+        part = grads[i].cpu().double() * d_i
+        assert abs(part.sum().item() - want) <= 1e-2 * part.abs().sum().item()
+
+
+# ---- together, captured, on other streams ----------------------------------------------------
+
+
+def test_norm_choice_attention_together():
+    """The four operators in a row, as an attention block uses them, forward and backward,
+    against the same row in float64 from the kernels' own choice: gradients within 5 % of
+    their norms (each stage rounds to bf16: some 2^-8 each, amplified by the norm)."""
+    gen = _gen(11)
+    b, h, hk, s, d, block, topk = 2, 4, 2, 150, 64, 16, 4
+    x = torch.randn(b, s, h + 2 * hk, d, generator=gen).to(torch.bfloat16).to(DEV).requires_grad_()
+    w = (1 + 0.2 * torch.randn(2, d, generator=gen)).to(DEV).requires_grad_()
+    pos = torch.randint(-20, 20, (b, s, 2), generator=gen, dtype=torch.int32).to(DEV)
+    freqs = 100.0 ** (-torch.arange(16, dtype=torch.float32, device=DEV) / 16)
+    lens = _lens(s, s - 30)
+
+    def block_of(x, w):
+        q, k, v = x.split([h, hk, hk], 2)
+        q, k = ops.qk_norm_rope(q.transpose(1, 2), k.transpose(1, 2), w[0], w[1], pos, freqs, [8, 8])
+        means = ops.block_means(k.detach(), lens, block)
+        sel = ops.block_select(q.detach(), means, lens, lens, block, topk)
+        return ops.attn_blocks(q, k, v.transpose(1, 2), sel, lens, lens, block)[0], sel
+
+    out, sel = block_of(x, w)
+    g = torch.randn(out.shape, generator=gen).to(torch.bfloat16).to(DEV)
+    gx, gw = torch.autograd.grad(out, [x, w], g)
+    xc, wc = (t.detach().cpu().double().requires_grad_() for t in (x, w))
+    q, k, v = (t.transpose(1, 2) for t in xc.split([h, hk, hk], 2))
+    th = pos.cpu().double().repeat_interleave(8, -1)[:, None] * freqs.cpu().double()
+
+    def turn(t, wt):
+        t = t / (t.square().mean(-1, keepdim=True) + 1e-6).sqrt() * wt
+        a, c = t[..., :16], t[..., 16:32]
+        return torch.cat([a * th.cos() - c * th.sin(), c * th.cos() + a * th.sin(), t[..., 32:]], -1)
+
+    q, k = turn(q, wc[0]), turn(k, wc[1])
+    k, v = k.repeat_interleave(h // hk, 1), v.repeat_interleave(h // hk, 1)
+    member = torch.arange(s) // block
+    seen = (sel.cpu().repeat_interleave(h // hk, 1)[..., None] == member).any(-2)
+    seen &= torch.arange(s) < lens.cpu()[:, None, None, None]
+    rows = seen.any(-1, keepdim=True)
+    p = torch.softmax((q @ k.transpose(-1, -2) / 8).masked_fill(~seen, -1e30), -1) * rows
+    want = p @ v
+    wx, ww = torch.autograd.grad(want, [xc, wc], g.cpu().double())
+    for got, ref in ((out, want), (gx, wx), (gw, ww)):
+        assert (got.detach().cpu().double() - ref).norm() <= 0.05 * ref.detach().norm()
+
+
+def test_captured():
+    """Means, choice, attention and gradients in a graph, replayed with new inputs and
+    eager work between; two graphs beside each other."""
+    gen = _gen(12)
+    b, h, hk, s, d, block, topk = 2, 4, 2, 130, 64, 16, 4
+    lens = _lens(s, s - 20)
+    new = lambda n: torch.randn(b, n, s, d, generator=gen).to(torch.bfloat16).to(DEV)
+    calls = []
+    for _ in range(2):
+        ins = [new(h), new(hk), new(hk), new(h)]
+
+        def run(ins=ins):
+            q, k, v, g = ins
+            means = ops.block_means(k, lens, block)
+            ops.block_means_update(means, k, lens, block)
+            sel = ops.block_select(q, means, lens, lens, block, topk)
+            out, lse = ops.attn_blocks(q, k, v, sel, lens, lens, block)
+            one = ops.attn_blocks(q[:, :, :1], k, v, sel[:, :, :1], lens, lens, block)
+            return (means, sel, out, lse, *one,
+                    *ops.attn_blocks_backward(g, None, q, k, v, sel, lens, lens, out, lse, block))
+
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run()
+        calls.append((graph, outs, run, ins))
+    for _ in range(3):
+        for *_, ins in calls:
+            for t in ins:
+                t.copy_(new(t.shape[1]))
+        for graph, *_ in calls:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, outs, run, _ in calls:
+            assert all(torch.equal(a, c) for a, c in zip(outs, run()))
+
+
+def test_other_stream():
+    gen = _gen(13)
+    b, h, s, d, block = 2, 2, 100, 64, 16
+    q, k, v = (_heads(gen, b, h, s, d, torch.bfloat16) for _ in range(3))
+    lens = _lens(s, s)
+
+    def run():
+        sel = ops.block_select(q, ops.block_means(k, lens, block), lens, lens, block, 3)
+        return ops.attn_blocks(q, k, v, sel, lens, lens, block)[0]
+
+    want = run()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = run()
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_refused_on_the_device():
+    q = torch.zeros(1, 4, 5, 64, dtype=torch.bfloat16, device=DEV)
+    k = torch.zeros(1, 2, 40, 64, dtype=torch.bfloat16, device=DEV)
+    ql, kl = _lens(5), _lens(40)
+    means = ops.block_means(k, kl, 16)
+    sel = ops.block_select(q, means, ql, kl, 16, 2)
+    good = dict(q=q, k=k, v=k, sel=sel, q_lens=ql, k_lens=kl, block=16)
+    ops.attn_blocks(**good)
+    wrong = (ValueError, TypeError, RuntimeError)
+    for bad in (dict(block=8), dict(block=24), dict(block=0), dict(q=q.float(), k=k.float(), v=k.float()),
+                dict(v=k.half()), dict(v=k[:, :1]), dict(k=k[..., :32]), dict(q=q[:, :3]), dict(sel=sel.long()),
+                dict(sel=sel[:, :1]), dict(sel=sel[..., :0]), dict(sel=sel.repeat(1, 1, 1, 33)), dict(q_lens=kl[:0]),
+                dict(k_lens=kl.float()), dict(k_lens=kl.cpu()), dict(sel=sel.cpu()), dict(k=k.cpu(), v=k.cpu()),
+                dict(q=torch.zeros(1, 130, 5, 64, dtype=torch.bfloat16, device=DEV)),
+                dict(q=torch.zeros(1, 4, 5, 136, dtype=torch.bfloat16, device=DEV))):
+        with pytest.raises(wrong):
+            ops.attn_blocks(**{**good, **bad})
+    pick = dict(q=q, means=means, q_lens=ql, k_lens=kl, block=16, topk=2)
+    for bad in (dict(topk=0), dict(topk=65), dict(block=0), dict(means=means.half()), dict(means=means[:, :, :, :32]),
+                dict(q=q[:, :3]), dict(q=q[0]), dict(q_lens=ql.repeat(2)), dict(means=means.cpu()),
+                dict(q=q.double()), dict(means=torch.zeros(1, 2, 4097, 64, device=DEV))):
+        with pytest.raises(wrong):
+            ops.block_select(**{**pick, **bad})
+    for bad in (dict(block=0), dict(k=k.int()), dict(k=k[0]), dict(k_lens=kl.cpu()),
+                dict(k=torch.zeros(1, 1, 4097, 64, device=DEV), block=1),
+                dict(k=torch.zeros(1, 1, 4, 129, device=DEV))):
+        with pytest.raises(wrong):
+            ops.block_means(**{**dict(k=k, k_lens=kl, block=16), **bad})
+    for bad in (means.half(), means[:, :, :2], means.transpose(2, 3).contiguous().transpose(2, 3), means.cpu()):
+        with pytest.raises(wrong):
+            ops.block_means_update(bad, k, kl, 16)
+    out, lse = ops.attn_blocks(**good)
+    for bad in (dict(g=out[:, :2]), dict(g=out.half()), dict(lse=lse.half()), dict(g_lse=lse[:, :2]),
+                dict(out=out[..., :32])):
+        with pytest.raises(wrong):
+            ops.attn_blocks_backward(**{**dict(g=out, g_lse=None, out=out, lse=lse), **good, **bad})
