@@ -17,8 +17,9 @@
 // staged in LDS and waves never wait for each other.
 //
 // Softmax in base 2 around the running maximum, statistics and accumulators in fp32;
-// the weights are rounded once to the type of V (half a step relative to each
-// weight, as large as the rounding of the result).
+// a weight enters its product as the sum of two numbers of the type of V (one alone put the
+// error against float64 at 2.1e-3 of the result's norm in bf16 and that of dq at 2.5e-3;
+// two at 1.7e-3, the rounding of the result).
 #include "capi.hpp"
 #include "common.hpp"
 
@@ -41,6 +42,19 @@ struct Mma<__bf16> {
   static SHRIMP_DEV f32x4 k32(u32x4 a, u32x4 b, f32x4 c) { return mfma16x16x32(a, b, c); }
   static SHRIMP_DEV f32x4 k16(u32x2 a, u32x2 b, f32x4 c) { return mfma16x16x16(a, b, c); }
   static SHRIMP_DEV unsigned pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  // x as the sum of two numbers, four at a time. The high part is cut below |x|, so the
+  // low part is neither zero nor of the other sign, and an infinity stays one under both.
+  static SHRIMP_DEV void split(const float (&x)[4], u32x2& hi, u32x2& lo) {
+    unsigned t[4];
+    float r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t[i] = __float_as_uint(x[i] * (1.f - 0x1p-16f));
+      r[i] = x[i] - __uint_as_float(t[i] & 0xFFFF0000u);
+    }
+    hi = u32x2{__builtin_amdgcn_perm(t[1], t[0], 0x07060302u), __builtin_amdgcn_perm(t[3], t[2], 0x07060302u)};
+    lo = u32x2{pack(r[0], r[1]), pack(r[2], r[3])};
+  }
 };
 template <>
 struct Mma<_Float16> {
@@ -55,6 +69,14 @@ struct Mma<_Float16> {
   static SHRIMP_DEV unsigned pack(float lo, float hi) {
     const f16x2 v = {(_Float16)lo, (_Float16)hi};
     return __builtin_bit_cast(unsigned, v);
+  }
+  static SHRIMP_DEV void split(const float (&x)[4], u32x2& hi, u32x2& lo) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const auto h = __builtin_amdgcn_cvt_pkrtz(x[i] * (1.f - 0x1p-13f), x[i + 1] * (1.f - 0x1p-13f));
+      hi[i / 2] = __builtin_bit_cast(unsigned, h);
+      lo[i / 2] = pack(x[i] - (float)h[0], x[i + 1] - (float)h[1]);
+    }
   }
 };
 
@@ -142,20 +164,24 @@ struct Turned {
   }
 };
 
-// acc[e] += (dimension-major A of these keys) x (their weights pk of 16 rows); the order of
-// the keys inside a product is that of the lanes' weights, the same on both sides.
+// acc[e] += (dimension-major A of these keys) x (their weights of 16 rows, hi + lo); the order
+// of the keys inside a product is that of the lanes' weights, the same on both sides.
 template <typename T, int D, int KT>
-SHRIMP_DEV void weigh(const Turned<D, KT>& v, const u32x2 (&pk)[KT], f32x4 (&acc)[D / 16]) {
+SHRIMP_DEV void weigh(const Turned<D, KT>& v, const u32x2 (&hi)[KT], const u32x2 (&lo)[KT],
+                      f32x4 (&acc)[D / 16]) {
 #pragma unroll
   for (int e = 0; e < D / 16; ++e) {
     if constexpr (KT == 1) {
-      acc[e] = Mma<T>::k16(v.four(0, e), pk[0], acc[e]);
+      const u32x2 a = v.four(0, e);
+      acc[e] = Mma<T>::k16(a, hi[0], acc[e]);
+      acc[e] = Mma<T>::k16(a, lo[0], acc[e]);
     } else {
 #pragma unroll
       for (int kt = 0; kt < KT; kt += 2) {
         const u32x2 a = v.four(kt, e), b = v.four(kt + 1, e);
-        acc[e] = Mma<T>::k32(u32x4{a[0], a[1], b[0], b[1]},
-                             u32x4{pk[kt][0], pk[kt][1], pk[kt + 1][0], pk[kt + 1][1]}, acc[e]);
+        const u32x4 ab{a[0], a[1], b[0], b[1]};
+        acc[e] = Mma<T>::k32(ab, u32x4{hi[kt][0], hi[kt][1], hi[kt + 1][0], hi[kt + 1][1]}, acc[e]);
+        acc[e] = Mma<T>::k32(ab, u32x4{lo[kt][0], lo[kt][1], lo[kt + 1][0], lo[kt + 1][1]}, acc[e]);
       }
     }
   }
@@ -174,10 +200,11 @@ SHRIMP_DEV void score_start(int key0, int len, int lg, f32x4 (&c)[KT]) {
 }
 
 // One step of the softmax of 16 rows (row lr, keys 16 kt + 4 lg + i at the lane): from
-// scores s and the row's (m, l) the weights pk in T, the factor for what came before,
+// scores s and the row's (m, l) the weights hi + lo in T, the factor for what came before,
 // and the new (m, l).
 template <typename T, int KT>
-SHRIMP_DEV float soft_step(const f32x4 (&s)[KT], float scale2, float& m, float& l, u32x2 (&pk)[KT]) {
+SHRIMP_DEV float soft_step(const f32x4 (&s)[KT], float scale2, float& m, float& l, u32x2 (&hi)[KT],
+                           u32x2 (&lo)[KT]) {
   float mx = s[0][0];
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
@@ -194,7 +221,7 @@ SHRIMP_DEV float soft_step(const f32x4 (&s)[KT], float scale2, float& m, float& 
       w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], scale2, -off));
       sum += w[i];
     }
-    pk[kt] = u32x2{Mma<T>::pack(w[0], w[1]), Mma<T>::pack(w[2], w[3])};
+    Mma<T>::split(w, hi[kt], lo[kt]);
   }
   const float alpha = __builtin_amdgcn_exp2f(m - off);
   l = fmaf(l, alpha, sum_groups_swap(sum));
@@ -329,13 +356,13 @@ __global__ __launch_bounds__(64) void attn_blocks_kernel(const BlocksParams p) {
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], qf[ks], s[kt]);
         }
-        u32x2 pk[KT];
-        const float alpha = soft_step<T, KT>(s, p.scale2, m, l, pk);
+        u32x2 hi[KT], lo[KT];
+        const float alpha = soft_step<T, KT>(s, p.scale2, m, l, hi, lo);
         float* mine = acc_lds + row * RF + lg * EPL * 4;
         f32x4 acc[EPL];
 #pragma unroll
         for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4) * alpha;
-        weigh<T, D, KT>(vf, pk, acc);
+        weigh<T, D, KT>(vf, hi, lo, acc);
         if (on) {
 #pragma unroll
           for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
@@ -420,11 +447,11 @@ __global__ __launch_bounds__(QW * 64) void attn_blocks_query_kernel(const Blocks
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], qf[ks], s[kt]);
-        u32x2 pk[KT];
-        const float alpha = soft_step<T, KT>(s, p.scale2, m, l, pk);
+        u32x2 hi[KT], lo[KT];
+        const float alpha = soft_step<T, KT>(s, p.scale2, m, l, hi, lo);
 #pragma unroll
         for (int e = 0; e < EPL; ++e) acc[e] *= alpha;
-        weigh<T, D, KT>(vf, pk, acc);
+        weigh<T, D, KT>(vf, hi, lo, acc);
       }
     }
     // join: every wave's rows around its own maximum, added in wave order
@@ -473,7 +500,7 @@ __global__ __launch_bounds__(QW * 64) void attn_blocks_query_kernel(const Blocks
 // also leaves every block's row masks and every row's (lse, delta) behind; dk and dv
 // with a workgroup per run of keys, which gathers the rows of those masks, 32 to
 // a product, and keeps both accumulators in registers. Every sum has one order, so
-// gradients repeat bit for bit. p and ds are rounded once to the operands' type.
+// gradients repeat bit for bit. p and ds are the sum of two numbers of the operands' type.
 
 struct GradParams {
   const uint16_t* g;
@@ -569,7 +596,7 @@ __global__ __launch_bounds__(64) void attn_blocks_dq_kernel(const BlocksParams p
         load_row<D>(q + lane_i64(my_row, row), on, p.d, lg, qf);
         load_row<D>(g + lane_i64(my_grad, row), on, p.d, lg, gf);
         const float2 st = stat_lds[row];
-        u32x2 pk[KT];
+        u32x2 hi[KT], lo[KT];
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
           f32x4 s = start_at[kt], dp = {0.f, 0.f, 0.f, 0.f};
@@ -581,13 +608,13 @@ __global__ __launch_bounds__(64) void attn_blocks_dq_kernel(const BlocksParams p
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -st.x)) * gp.scale * (dp[i] - st.y);
-          pk[kt] = u32x2{Mma<T>::pack(w[0], w[1]), Mma<T>::pack(w[2], w[3])};
+          Mma<T>::split(w, hi[kt], lo[kt]);
         }
         float* mine = acc_lds + row * RF + lg * EPL * 4;
         f32x4 acc[EPL];
 #pragma unroll
         for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4);
-        weigh<T, D, KT>(kt_, pk, acc);
+        weigh<T, D, KT>(kt_, hi, lo, acc);
         if (on) {
 #pragma unroll
           for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
@@ -712,7 +739,7 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
         };
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-          u32x4 pp, ds;
+          u32x2 ph[2], pl[2], dh[2], dl[2];
 #pragma unroll
           for (int rt = 0; rt < 2; ++rt) {
             f32x4 s = start_at[kt], dp = {0.f, 0.f, 0.f, 0.f};
@@ -726,15 +753,16 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
               w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -st[rt][i].x));
               x[i] = w[i] * gp.scale * (dp[i] - st[rt][i].y);
             }
-            pp[2 * rt] = Mma<T>::pack(w[0], w[1]);
-            pp[2 * rt + 1] = Mma<T>::pack(w[2], w[3]);
-            ds[2 * rt] = Mma<T>::pack(x[0], x[1]);
-            ds[2 * rt + 1] = Mma<T>::pack(x[2], x[3]);
+            Mma<T>::split(w, ph[rt], pl[rt]);
+            Mma<T>::split(x, dh[rt], dl[rt]);
           }
 #pragma unroll
           for (int e = 0; e < EPL; ++e) {
-            dv[kt][e] = Mma<T>::k32(turn(gt, e), pp, dv[kt][e]);
-            dk[kt][e] = Mma<T>::k32(turn(qt, e), ds, dk[kt][e]);
+            const u32x4 ga = turn(gt, e), qa = turn(qt, e);
+            dv[kt][e] = Mma<T>::k32(ga, u32x4{ph[0][0], ph[0][1], ph[1][0], ph[1][1]}, dv[kt][e]);
+            dk[kt][e] = Mma<T>::k32(qa, u32x4{dh[0][0], dh[0][1], dh[1][0], dh[1][1]}, dk[kt][e]);
+            dv[kt][e] = Mma<T>::k32(ga, u32x4{pl[0][0], pl[0][1], pl[1][0], pl[1][1]}, dv[kt][e]);
+            dk[kt][e] = Mma<T>::k32(qa, u32x4{dl[0][0], dl[0][1], dl[1][0], dl[1][1]}, dk[kt][e]);
           }
         }
       }
