@@ -5,16 +5,15 @@
 //   lse[b, h, i] = log sum_j exp(q . k_j / sqrt(d)). A row without a key: 0 and -inf.
 //
 // Neighbouring queries choose different blocks, so no tile of queries shares its
-// keys. The chunk kernel turns the choice round: a wave owns R rows (queries x the
-// G heads of a key head) and their output accumulators, in LDS, goes through the
-// blocks, and for each gathers the rows that chose it, 16 to a matrix product.
-// Every (row, block) pair is computed once on full tiles but for the last of a block,
-// nothing leaves the chip in between, and a row meets its blocks in ascending order
-// alone, so its bits depend on its own inputs only. Products stay transposed
-// (S^T = K Q^T, O^T = V^T P^T): a lane's scores are already its part of the next
-// product's operand. K rows are MFMA operands as they lie in memory; V^T's are put
-// together from 4 keys x EPL dimensions per lane with byte permutes, so nothing is
-// staged in LDS and waves never wait for each other.
+// keys. The chunk kernel turns the choice round: a wave owns up to 64 rows (queries x
+// the G heads of a key head) with their output accumulators in LDS; its workgroup of four
+// goes through the keys 64 at a time, read once from memory while the ones before are
+// worked on, and for each block a wave gathers those of its rows that chose it, 16 to
+// a matrix product. Every (row, block) pair is computed once, nothing leaves the chip
+// in between, and a row meets its blocks in ascending order alone, so its bits depend on
+// its own inputs only. Products stay transposed (S^T = K Q^T, O^T = V^T P^T): a lane's
+// scores are already its part of the next product's operand; V^T's operands are put
+// together from 4 keys x EPL dimensions per lane with byte permutes.
 //
 // Softmax in base 2 around the running maximum, statistics and accumulators in fp32;
 // a weight enters its product as the sum of two numbers of the type of V (one alone put the
@@ -28,8 +27,16 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr int R = 64;       // rows of a chunk: one bit each in a 64-bit mask
-constexpr int WINDOW = 512; // blocks whose masks are in LDS at a time
+constexpr int WAVES = 4;    // waves of a chunk workgroup
+constexpr int STAGE = 64;   // keys in LDS at a time
+constexpr int WINDOW = 64;  // blocks whose row masks a wave holds at a time, one per lane
+
+// Rows of a wave (one bit each in a 64-bit mask): as many as the LDS of a compute unit
+// holds for four waves beside the keys.
+template <int D, bool BACK>
+constexpr int wave_rows() {
+  return D == 128 || BACK ? 48 : 64;
+}
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -92,8 +99,10 @@ struct BlocksParams {
   float* lse;
   int B, H, Hk, Sq, Sk, d, block, topk;
   int group;    // query heads per key head
-  int queries;  // queries per chunk
-  int chunks;   // chunks per (sequence, key head)
+  int queries;  // queries per wave
+  int chunks;   // waves' runs of queries per (sequence, key head)
+  int groups;   // workgroups of WAVES runs
+  int stage;    // keys per stage: whole blocks, or an equal part of one
   int by_xcd;   // a key head's chunks stay on one XCD
   float scale2; // log2(e) / sqrt(d)
 };
@@ -229,60 +238,7 @@ SHRIMP_DEV float soft_step(const f32x4 (&s)[KT], float scale2, float& m, float& 
   return alpha;
 }
 
-// ---- chunk kernel: R rows per wave ----------------------------------------------------
-
-// Fills the masks of blocks [w0, w0 + n): bit r of mask[block] = row r chose it.
-SHRIMP_DEV void fill_masks(const BlocksParams& p, const int32_t* sel, int rows_q, int w0, int n,
-                           unsigned* mask, int lane) {
-  for (int i = lane; i < 2 * n; i += 64) mask[i] = 0;
-  __syncthreads();
-  const uint64_t ones = p.group >= 64 ? ~0ull : (1ull << p.group) - 1;
-  for (int j = lane; j < rows_q * p.topk; j += 64) {
-    const unsigned blk = (unsigned)(sel[j] - w0);
-    if (sel[j] >= 0 && blk < (unsigned)n) {
-      const uint64_t bits = ones << (j / p.topk * p.group);
-      if ((unsigned)bits) atomicOr(&mask[2 * blk], (unsigned)bits);
-      if ((unsigned)(bits >> 32)) atomicOr(&mask[2 * blk + 1], (unsigned)(bits >> 32));
-    }
-  }
-  __syncthreads();
-}
-
-// f(mask, row_at, block) for every block that a row of the chunk chose, ascending: bit r
-// of the mask is row r, and lane j holds in row_at the j-th row of the mask (lanes from
-// its count on hold the others). `keep`, when given, receives every live block's mask,
-// `keep_stride` apart.
-template <typename F>
-SHRIMP_DEV void each_block(const BlocksParams& p, const int32_t* sel, int asking, int live,
-                           unsigned* mask_lds, int lane, uint64_t* keep, int64_t keep_stride, F f) {
-  for (int w0 = 0; w0 < live; w0 += WINDOW) {
-    const int wn = min(WINDOW, live - w0);
-    fill_masks(p, sel, asking, w0, wn, mask_lds, lane);
-    for (int g0 = 0; g0 < wn; g0 += 64) {
-      unsigned mlo = 0, mhi = 0;
-      if (g0 + lane < wn) {
-        mlo = mask_lds[2 * (g0 + lane)];
-        mhi = mask_lds[2 * (g0 + lane) + 1];
-        if (keep) keep[(w0 + g0 + lane) * keep_stride] = (uint64_t)mhi << 32 | mlo;
-      }
-      uint64_t todo = __ballot((mlo | mhi) != 0);
-      while (todo) {
-        const int at = __builtin_ctzll(todo);
-        todo &= todo - 1;
-        const uint64_t mask = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)mhi, at) << 32 |
-                              (unsigned)__builtin_amdgcn_readlane((int)mlo, at);
-        const bool in = mask >> lane & 1;
-        const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
-                                                     __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
-        const int to = in ? before : __popcll(mask) + lane - before;
-        f(mask, __builtin_amdgcn_ds_permute(to << 2, lane), w0 + g0 + at);
-      }
-    }
-    __syncthreads();
-  }
-}
-
-// 64-bit value of lane `src` (byte address 4 src) for every lane.
+// 64-bit value of lane `src` for every lane.
 SHRIMP_DEV int64_t lane_i64(int64_t v, int src) {
   return (int64_t)(unsigned)__builtin_amdgcn_ds_bpermute(src << 2, (int)v) |
          (int64_t)__builtin_amdgcn_ds_bpermute(src << 2, (int)(v >> 32)) << 32;
@@ -303,101 +259,314 @@ constexpr int row_floats() {
   return D + 4;  // rows 16 bytes apart in the banks
 }
 
-template <typename T, int D, int KT>
-__global__ __launch_bounds__(64) void attn_blocks_kernel(const BlocksParams p) {
-  extern __shared__ char lds[];
-  constexpr int RF = row_floats<D>(), EPL = D / 16, KS = D / 32;
-  float* acc_lds = reinterpret_cast<float*>(lds);  // [R][RF], per row: lane group, e, i
-  float* m_lds = acc_lds + R * RF;
-  float* l_lds = m_lds + R;
-  unsigned* mask_lds = reinterpret_cast<unsigned*>(l_lds + R);  // [WINDOW][2]
-  const int lane = threadIdx.x, lr = lane & 15, lg = lane >> 4;
+// ---- chunk kernel ------------------------------------------------------------------------
+
+struct GradParams {
+  const uint16_t* g;
+  const float* g_lse;  // or null
+  int64_t g_sb, g_sh, g_sn;
+  uint16_t* dq;
+  uint16_t* dk;
+  uint16_t* dv;
+  float2* stat;     // (B, H, Sq): lse log2(e) (+inf: no key), delta
+  uint64_t* masks;  // (B, Hk, NB, chunks): row masks of the dq kernel's waves
+  float scale;
+  int nb, segments; // blocks; runs of keys per (sequence, key head)
+};
+
+template <typename T>
+SHRIMP_DEV float elem(unsigned word, int hi);
+template <>
+SHRIMP_DEV float elem<__bf16>(unsigned word, int hi) {
+  return hi ? bf16_hi(word) : bf16_lo(word);
+}
+template <>
+SHRIMP_DEV float elem<_Float16>(unsigned word, int hi) {
+  return (float)__builtin_bit_cast(f16x2, word)[hi];
+}
+
+// LDS of a chunk workgroup, in this order.
+template <int D, bool BACK>
+struct ChunkLds {
+  static constexpr int R = wave_rows<D, BACK>(), RF = row_floats<D>();
+  static constexpr int RS = D + 8;             // 16-bit elements of a staged row
+  static constexpr bool ROWS = D <= 64;        // q (and g) rows are kept, else gathered from memory
+  static constexpr int acc = 0;                                      // [WAVES][R][RF] fp32
+  static constexpr int stat = acc + WAVES * R * RF * 4;              // [WAVES][R] float2
+  static constexpr int mask = stat + WAVES * R * 8;                  // [WAVES][WINDOW] u64
+  static constexpr int keys = mask + WAVES * WINDOW * 8;             // [2][STAGE][RS]
+  static constexpr int rows = keys + 2 * STAGE * RS * 2;             // [1 or 2][WAVES][R][RS]
+  static constexpr int bytes = rows + (ROWS ? (BACK ? 2 : 1) * WAVES * R * RS * 2 : 0);
+  static_assert(bytes <= 160 * 1024, "a compute unit's LDS");
+};
+
+// The masks of blocks [w0, w0 + WINDOW): bit r of mask[block] = the wave's row r chose it.
+SHRIMP_DEV void fill_masks(const BlocksParams& p, const int32_t* sel, int asking, int w0,
+                           unsigned* mask, int lane) {
+  mask[2 * lane] = mask[2 * lane + 1] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  const uint64_t ones = (1ull << p.group) - 1;
+  for (int j = lane; j < asking * p.topk; j += 64) {
+    const int s = sel[j];
+    const unsigned blk = (unsigned)s - (unsigned)w0;
+    if (s >= w0 && blk < (unsigned)WINDOW) {
+      const uint64_t bits = ones << (j / p.topk * p.group);
+      if ((unsigned)bits) atomicOr(&mask[2 * blk], (unsigned)bits);
+      if ((unsigned)(bits >> 32)) atomicOr(&mask[2 * blk + 1], (unsigned)(bits >> 32));
+    }
+  }
+}
+
+// The forward, and with BACK the gradient of q (see there).
+template <typename T, int D, int KT, bool BACK>
+__global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const BlocksParams p, const GradParams gp) {
+  extern __shared__ __align__(16) char lds[];
+  using L = ChunkLds<D, BACK>;
+  constexpr int R = L::R, RF = L::RF, RS = L::RS, EPL = D / 16, KS = D / 32, W = EPL / 2;
+  constexpr int LPR = D / 4;                                 // lanes of a row, four dimensions each
+  constexpr int PIECES = STAGE * (D / 8) / (WAVES * 64);     // 16-byte pieces of a stage per thread
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4, wave = wave_id();
+  float* acc_lds = reinterpret_cast<float*>(lds + L::acc) + wave * R * RF;
+  float2* stat_lds = reinterpret_cast<float2*>(lds + L::stat) + wave * R;
+  unsigned* mask_lds = reinterpret_cast<unsigned*>(lds + L::mask);
+  uint16_t* k_lds = reinterpret_cast<uint16_t*>(lds + L::keys);
+  uint16_t* v_lds = k_lds + STAGE * RS;
+  uint16_t* q_lds = reinterpret_cast<uint16_t*>(lds + L::rows) + wave * R * RS;
+  uint16_t* g_lds = q_lds + WAVES * R * RS;
   int64_t bh;
-  int chunk;
-  if (!place_chunk(p, p.chunks, bh, chunk)) return;
+  int grp;
+  if (!place_chunk(p, p.groups, bh, grp)) return;
   const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
   const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
-  const int q0 = chunk * p.queries;
-  const int queries = min(p.queries, p.Sq - q0);          // written
-  const int asking = min(queries, max(q_len - q0, 0));    // with a choice
+  const int chunk = grp * WAVES + wave;
+  const int q0 = min(chunk * p.queries, p.Sq);
+  const int queries = min(p.queries, p.Sq - q0);        // written
+  const int asking = min(queries, max(q_len - q0, 0));  // with a choice
   const int live = (k_len + p.block - 1) / p.block;
-
-  for (int i = lane; i < R * RF; i += 64) acc_lds[i] = 0.f;
-  m_lds[lane] = -INFINITY;
-  l_lds[lane] = 0.f;
-
-  // row `lane` of the chunk: query lane / G, head lane % G
-  const int my_query = lane / p.group, my_head = hk * p.group + lane - my_query * p.group;
-  const int64_t my_row = my_head * p.q_sh + (int64_t)(q0 + my_query) * p.q_sn;
   const uint16_t* q = p.q + b * p.q_sb;
+  const uint16_t* g = BACK ? gp.g + b * gp.g_sb : nullptr;
   const uint16_t* k = p.k + b * p.k_sb + hk * p.k_sh;
   const uint16_t* v = p.v + b * p.v_sb + hk * p.v_sh;
   const int32_t* sel = p.sel + (bh * p.Sq + q0) * p.topk;
 
-  each_block(p, sel, asking, live, mask_lds, lane, nullptr, 0, [&](uint64_t mask, int row_at, int blk) {
-    const int count = __popcll(mask), start = blk * p.block;
-    for (int key0 = start; key0 < min(start + p.block, k_len); key0 += KT * 16) {
-      u32x4 kf[KT][KS];
-      load_rows<D, KT>(k, p.k_sn, key0, k_len, p.d, lr, lg, kf);
-      Turned<D, KT> vf;
-      vf.load(v, p.v_sn, key0, k_len, p.d, lr, lg);
-      f32x4 start_at[KT];
-      score_start<KT>(key0, k_len, lg, start_at);
-      for (int t = 0; t < count; t += 16) {
-        const int row = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at);
-        const bool on = t + lr < count;
-        u32x4 qf[KS];
-        load_row<D>(q + lane_i64(my_row, row), on, p.d, lg, qf);
-        float m = on ? m_lds[row] : -INFINITY, l = on ? l_lds[row] : 0.f;
-        f32x4 s[KT];
+  // rows of the wave: query r / G, head r % G
+  for (int i = lane; i < R * RF; i += 64) acc_lds[i] = 0.f;
+  if constexpr (BACK) {
+    for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
+      const int r = r0 + lane / LPR, c = lane % LPR;
+      const bool on = r < queries * p.group;
+      const int query = on ? r / p.group : 0, head = hk * p.group + (on ? r - query * p.group : 0);
+      const int64_t o = ((int64_t)b * p.H + head) * p.Sq + q0 + query;
+      float delta = 0.f;
+      if (on && c * 4 < p.d) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p.out + o * p.d + c * 4);
+        const u32x2 y = *reinterpret_cast<const u32x2*>(g + head * gp.g_sh + (int64_t)(q0 + query) * gp.g_sn + c * 4);
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          s[kt] = start_at[kt];
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], qf[ks], s[kt]);
-        }
-        u32x2 hi[KT], lo[KT];
-        const float alpha = soft_step<T, KT>(s, p.scale2, m, l, hi, lo);
-        float* mine = acc_lds + row * RF + lg * EPL * 4;
-        f32x4 acc[EPL];
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4) * alpha;
-        weigh<T, D, KT>(vf, hi, lo, acc);
-        if (on) {
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
-          if (lg == 0) {
-            m_lds[row] = m;
-            l_lds[row] = l;
-          }
-        }
-        __syncthreads();  // (one wave: the rows' state is read again by other lanes)
+        for (int e = 0; e < 4; ++e) delta = fmaf(elem<T>(x[e >> 1], e & 1), elem<T>(y[e >> 1], e & 1), delta);
+      }
+      for (int m = 1; m < LPR; m <<= 1) delta += xor_shfl(delta, m);
+      if (on && c == 0) {
+        if (gp.g_lse) delta -= gp.g_lse[o];
+        const float lse = p.lse[o];
+        const float2 st = {lse == -INFINITY ? INFINITY : lse * LOG2E, delta};
+        stat_lds[r] = st;
+        gp.stat[o] = st;
       }
     }
-  });
+  } else {
+    for (int r = lane; r < R; r += 64) stat_lds[r] = float2{-INFINITY, 0.f};  // maximum, sum
+  }
+  const int my_query = lane / p.group, my_head = hk * p.group + lane - my_query * p.group;
+  const int64_t my_row = my_head * p.q_sh + (int64_t)(q0 + my_query) * p.q_sn;
+  const int64_t my_grad = BACK ? my_head * gp.g_sh + (int64_t)(q0 + my_query) * gp.g_sn : 0;
+  if constexpr (L::ROWS) {
+    for (int i = lane; i < R * (D / 8); i += 64) {
+      const int r = i / (D / 8), c = i % (D / 8);
+      const bool on = r < asking * p.group && c * 8 < p.d;
+      const int query = on ? r / p.group : 0, head = hk * p.group + (on ? r - query * p.group : 0);
+      const u32x4 none = {0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(q_lds + r * RS + c * 8) =
+          on ? *reinterpret_cast<const u32x4*>(q + head * p.q_sh + (int64_t)(q0 + query) * p.q_sn + c * 8) : none;
+      if constexpr (BACK)
+        *reinterpret_cast<u32x4*>(g_lds + r * RS + c * 8) =
+            on ? *reinterpret_cast<const u32x4*>(g + head * gp.g_sh + (int64_t)(q0 + query) * gp.g_sn + c * 8) : none;
+    }
+  }
 
-  // 16 lanes per row (D >= 64; four dimensions each), the rows' result and lse
-  constexpr int LPR = D / 4;  // lanes per row
+  // stage of keys from key0: requested into registers, put into LDS by `store`
+  u32x4 kr[PIECES], vr[PIECES];
+  auto request = [&](int key0) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int row = (tid + i * WAVES * 64) / (D / 8), c = (tid + i * WAVES * 64) % (D / 8);
+      const bool on = row < p.stage && key0 + row < k_len && c * 8 < p.d;
+      const u32x4 none = {0, 0, 0, 0};
+      kr[i] = on ? *reinterpret_cast<const u32x4*>(k + (int64_t)(key0 + row) * p.k_sn + c * 8) : none;
+      vr[i] = on ? *reinterpret_cast<const u32x4*>(v + (int64_t)(key0 + row) * p.v_sn + c * 8) : none;
+    }
+  };
+  auto store = [&]() {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int row = (tid + i * WAVES * 64) / (D / 8), c = (tid + i * WAVES * 64) % (D / 8);
+      *reinterpret_cast<u32x4*>(k_lds + row * RS + c * 8) = kr[i];
+      *reinterpret_cast<u32x4*>(v_lds + row * RS + c * 8) = vr[i];
+    }
+  };
+
+  // the wave's rows of `mask` against `keys` keys at row `at` of the stage (key0 of the sequence)
+  auto work = [&](uint64_t mask, int at, int keys, int key0) {
+    const int count = __popcll(mask);
+    // lane j: the j-th row of the mask (the others behind them)
+    const bool in = mask >> lane & 1;
+    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+    const int row_at = __builtin_amdgcn_ds_permute((in ? before : count + lane - before) << 2, lane);
+    for (int t = 0; t < count; t += 16) {
+      const bool on = t + lr < count;
+      const int listed = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at), row = on ? listed : 0;
+      u32x4 qf[KS], gf[KS];
+      if constexpr (L::ROWS) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          qf[ks] = *reinterpret_cast<const u32x4*>(q_lds + row * RS + ks * 32 + lg * 8);
+          if constexpr (BACK) gf[ks] = *reinterpret_cast<const u32x4*>(g_lds + row * RS + ks * 32 + lg * 8);
+        }
+      } else {
+        load_row<D>(q + lane_i64(my_row, row), on, p.d, lg, qf);
+        if constexpr (BACK) load_row<D>(g + lane_i64(my_grad, row), on, p.d, lg, gf);
+      }
+      float2 st = stat_lds[row];
+      float* mine = acc_lds + row * RF + lg * EPL * 4;
+      f32x4 acc[EPL];
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4);
+      for (int kk = 0; kk < keys; kk += KT * 16) {
+        const uint16_t* kp = k_lds + (at + kk) * RS;
+        const uint16_t* vp = v_lds + (at + kk) * RS;
+        f32x4 s[KT];
+        score_start<KT>(key0 + kk, k_len, lg, s);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            s[kt] = Mma<T>::k32(*reinterpret_cast<const u32x4*>(kp + (kt * 16 + lr) * RS + ks * 32 + lg * 8),
+                                qf[ks], s[kt]);
+        Turned<D, KT> turned;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            turned.raw[kt][j] = *reinterpret_cast<const Words<W>*>((BACK ? kp : vp) + (kt * 16 + lg * 4 + j) * RS + lr * EPL);
+        u32x2 hi[KT], lo[KT];
+        if constexpr (BACK) {
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            f32x4 dp = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+              dp = Mma<T>::k32(*reinterpret_cast<const u32x4*>(vp + (kt * 16 + lr) * RS + ks * 32 + lg * 8),
+                               gf[ks], dp);
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], p.scale2, -st.x)) * gp.scale * (dp[i] - st.y);
+            Mma<T>::split(w, hi[kt], lo[kt]);
+          }
+        } else {
+          const float alpha = soft_step<T, KT>(s, p.scale2, st.x, st.y, hi, lo);
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) acc[e] *= alpha;
+        }
+        weigh<T, D, KT>(turned, hi, lo, acc);
+      }
+      if (on) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
+        if (!BACK && lg == 0) stat_lds[row] = st;
+      }
+      // (the rows' state is read again by other lanes of the wave)
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+  };
+
   __syncthreads();
+  const int per_stage = p.stage > p.block ? p.stage / p.block : 1;  // blocks of a stage
+  for (int w0 = 0; w0 < live; w0 += WINDOW) {
+    fill_masks(p, sel, asking, w0, mask_lds + wave * 2 * WINDOW, lane);
+    __syncthreads();
+    uint64_t any = 0, mine = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const uint64_t m = reinterpret_cast<const uint64_t*>(mask_lds)[w * WINDOW + lane];
+      any |= m;
+      if (w == wave) mine = m;
+    }
+    const bool here = w0 + lane < live;
+    if constexpr (BACK)
+      if (here && chunk < p.chunks) gp.masks[(bh * gp.nb + w0 + lane) * p.chunks + chunk] = mine;
+    uint64_t todo = __ballot(here && any != 0);
+    // stages that hold a chosen block, ascending
+    const uint64_t stage_bits = per_stage >= 64 ? ~0ull : (1ull << per_stage) - 1;
+    int at = 0, key0 = 0;  // first block (of the window) and key of the stage
+    auto first_of = [&]() {
+      at = __builtin_ctzll(todo) / per_stage * per_stage;
+      key0 = (w0 + at) * p.block;
+    };
+    if (todo) {
+      first_of();
+      request(key0);
+    }
+    while (todo) {
+      __syncthreads();  // the stage before is done with
+      store();
+      const int now = at, now_key = key0;
+      // the next stage: of the same block, or of the next chosen one
+      key0 += p.stage;
+      if (p.stage >= p.block || key0 >= min((w0 + at + 1) * p.block, k_len)) {
+        todo &= ~(stage_bits << at);
+        if (todo) first_of();
+      }
+      if (todo) request(key0);
+      __syncthreads();
+      if (p.stage > p.block) {
+        for (int i = 0; i < per_stage && now + i < WINDOW; ++i) {
+          const uint64_t mask = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), now + i) << 32 |
+                                (unsigned)__builtin_amdgcn_readlane((int)mine, now + i);
+          if (mask && w0 + now + i < live) work(mask, i * p.block, p.block, now_key + i * p.block);
+        }
+      } else {
+        const uint64_t mask = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), now) << 32 |
+                              (unsigned)__builtin_amdgcn_readlane((int)mine, now);
+        if (mask) work(mask, 0, p.stage, now_key);
+      }
+    }
+    __syncthreads();  // the masks are read
+  }
+
   for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
     const int r = r0 + lane / LPR, c = lane % LPR;
     if (r >= queries * p.group) continue;
     const int query = r / p.group, head = hk * p.group + r - query * p.group;
     const int64_t o = ((int64_t)b * p.H + head) * p.Sq + q0 + query;
-    const float l = l_lds[r], m = m_lds[r];
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float2 st = stat_lds[r];
+    const float inv = BACK ? 1.f : st.y == 0.f ? 0.f : 1.f / st.y;
     if (c * 4 < p.d) {
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        // dimension c 4 + e is element x % EPL of MFMA row x / EPL = 4 lg + i
+        // dimension 4 c + e is element dim % EPL of the product's row dim / EPL = 4 lg + i
         const int dim = c * 4 + e, rr = dim / EPL, ee = dim % EPL;
         x[e] = acc_lds[r * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3)] * inv;
       }
-      *reinterpret_cast<u32x2*>(p.out + o * p.d + c * 4) =
+      *reinterpret_cast<u32x2*>((BACK ? gp.dq : p.out) + o * p.d + c * 4) =
           u32x2{Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3])};
     }
-    if (c == 0) p.lse[o] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (!BACK && c == 0) p.lse[o] = st.y == 0.f ? -INFINITY : (st.x + __builtin_amdgcn_logf(st.y)) * LN2;
   }
 }
 
@@ -496,155 +665,16 @@ __global__ __launch_bounds__(QW * 64) void attn_blocks_query_kernel(const Blocks
 // ds_ij = p_ij (sum_d g_id v_jd - delta_i) / sqrt(d):
 //   dq_i = sum_j ds_ij k_j,   dk_j = sum_i ds_ij q_i,   dv_j = sum_i p_ij g_i,
 // the sums over a shared key head's queries of all its heads. Two kernels, each
-// computing the scores again: dq in the forward's chunks (accumulators in LDS), which
+// computing the scores again: dq in the chunk kernel (BACK), which
 // also leaves every block's row masks and every row's (lse, delta) behind; dk and dv
 // with a workgroup per run of keys, which gathers the rows of those masks, 32 to
 // a product, and keeps both accumulators in registers. Every sum has one order, so
 // gradients repeat bit for bit. p and ds are the sum of two numbers of the operands' type.
 
-struct GradParams {
-  const uint16_t* g;
-  const float* g_lse;  // or null
-  int64_t g_sb, g_sh, g_sn;
-  uint16_t* dq;
-  uint16_t* dk;
-  uint16_t* dv;
-  float2* stat;     // (B, H, Sq): lse log2(e) (+inf: no key), delta
-  uint64_t* masks;  // (B, Hk, NB, chunks)
-  float scale;
-  int nb, segments; // blocks; runs of keys per (sequence, key head)
-};
-
-template <typename T>
-SHRIMP_DEV float elem(unsigned word, int hi);
-template <>
-SHRIMP_DEV float elem<__bf16>(unsigned word, int hi) {
-  return hi ? bf16_hi(word) : bf16_lo(word);
-}
-template <>
-SHRIMP_DEV float elem<_Float16>(unsigned word, int hi) {
-  return (float)__builtin_bit_cast(f16x2, word)[hi];
-}
-
-template <typename T, int D, int KT>
-__global__ __launch_bounds__(64) void attn_blocks_dq_kernel(const BlocksParams p, const GradParams gp) {
-  extern __shared__ char lds[];
-  constexpr int RF = row_floats<D>(), EPL = D / 16, KS = D / 32;
-  float* acc_lds = reinterpret_cast<float*>(lds);
-  float2* stat_lds = reinterpret_cast<float2*>(acc_lds + R * RF);
-  unsigned* mask_lds = reinterpret_cast<unsigned*>(stat_lds + R);
-  const int lane = threadIdx.x, lr = lane & 15, lg = lane >> 4;
-  int64_t bh;
-  int chunk;
-  if (!place_chunk(p, p.chunks, bh, chunk)) return;
-  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
-  const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
-  const int q0 = chunk * p.queries;
-  const int queries = min(p.queries, p.Sq - q0);
-  const int asking = min(queries, max(q_len - q0, 0));
-  const int live = (k_len + p.block - 1) / p.block;
-  const uint16_t* g = gp.g + b * gp.g_sb;
-
-  for (int i = lane; i < R * RF; i += 64) acc_lds[i] = 0.f;
-  constexpr int LPR = D / 4;  // lanes per row, four dimensions each
-  for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
-    const int r = r0 + lane / LPR, c = lane % LPR;
-    const bool on = r < queries * p.group;
-    const int query = on ? r / p.group : 0, head = hk * p.group + (on ? r - query * p.group : 0);
-    const int64_t o = ((int64_t)b * p.H + head) * p.Sq + q0 + query;
-    float delta = 0.f;
-    if (on && c * 4 < p.d) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(p.out + o * p.d + c * 4);
-      const u32x2 y = *reinterpret_cast<const u32x2*>(g + head * gp.g_sh + (int64_t)(q0 + query) * gp.g_sn + c * 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) delta = fmaf(elem<T>(x[e >> 1], e & 1), elem<T>(y[e >> 1], e & 1), delta);
-    }
-    for (int m = 1; m < LPR; m <<= 1) delta += xor_shfl(delta, m);
-    if (on && c == 0) {
-      if (gp.g_lse) delta -= gp.g_lse[o];
-      const float lse = p.lse[o];
-      const float2 st = {lse == -INFINITY ? INFINITY : lse * LOG2E, delta};
-      stat_lds[r] = st;
-      gp.stat[o] = st;
-    }
-  }
-  __syncthreads();
-
-  const int my_query = lane / p.group, my_head = hk * p.group + lane - my_query * p.group;
-  const int64_t my_row = my_head * p.q_sh + (int64_t)(q0 + my_query) * p.q_sn;
-  const int64_t my_grad = my_head * gp.g_sh + (int64_t)(q0 + my_query) * gp.g_sn;
-  const uint16_t* q = p.q + b * p.q_sb;
-  const uint16_t* k = p.k + b * p.k_sb + hk * p.k_sh;
-  const uint16_t* v = p.v + b * p.v_sb + hk * p.v_sh;
-  const int32_t* sel = p.sel + (bh * p.Sq + q0) * p.topk;
-  uint64_t* keep = gp.masks + bh * gp.nb * p.chunks + chunk;
-
-  each_block(p, sel, asking, live, mask_lds, lane, keep, p.chunks, [&](uint64_t mask, int row_at, int blk) {
-    const int count = __popcll(mask), start = blk * p.block;
-    for (int key0 = start; key0 < min(start + p.block, k_len); key0 += KT * 16) {
-      u32x4 kf[KT][KS], vf[KT][KS];
-      load_rows<D, KT>(k, p.k_sn, key0, k_len, p.d, lr, lg, kf);
-      load_rows<D, KT>(v, p.v_sn, key0, k_len, p.d, lr, lg, vf);
-      Turned<D, KT> kt_;
-      kt_.load(k, p.k_sn, key0, k_len, p.d, lr, lg);
-      f32x4 start_at[KT];
-      score_start<KT>(key0, k_len, lg, start_at);
-      for (int t = 0; t < count; t += 16) {
-        const int row = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at);
-        const bool on = t + lr < count;
-        u32x4 qf[KS], gf[KS];
-        load_row<D>(q + lane_i64(my_row, row), on, p.d, lg, qf);
-        load_row<D>(g + lane_i64(my_grad, row), on, p.d, lg, gf);
-        const float2 st = stat_lds[row];
-        u32x2 hi[KT], lo[KT];
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          f32x4 s = start_at[kt], dp = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) s = Mma<T>::k32(kf[kt][ks], qf[ks], s);
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) dp = Mma<T>::k32(vf[kt][ks], gf[ks], dp);
-          float w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -st.x)) * gp.scale * (dp[i] - st.y);
-          Mma<T>::split(w, hi[kt], lo[kt]);
-        }
-        float* mine = acc_lds + row * RF + lg * EPL * 4;
-        f32x4 acc[EPL];
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4);
-        weigh<T, D, KT>(kt_, hi, lo, acc);
-        if (on) {
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
-        }
-        __syncthreads();
-      }
-    }
-  });
-
-  __syncthreads();
-  for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
-    const int r = r0 + lane / LPR, c = lane % LPR;
-    if (r >= queries * p.group || c * 4 >= p.d) continue;
-    const int query = r / p.group, head = hk * p.group + r - query * p.group;
-    const int64_t o = ((int64_t)b * p.H + head) * p.Sq + q0 + query;
-    float x[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int dim = c * 4 + e, rr = dim / EPL, ee = dim % EPL;
-      x[e] = acc_lds[r * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3)];
-    }
-    *reinterpret_cast<u32x2*>(gp.dq + o * p.d + c * 4) =
-        u32x2{Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3])};
-  }
-}
-
 constexpr int GW = 4;  // waves of a workgroup at most
 
 // One workgroup: KT tiles of 16 keys of one block. Its waves take every GW-th word of the
-// block's row masks (a word: the 64 rows of a chunk), 64 words at a time, list their
+// block's row masks (a word: the rows of one wave of the dq kernel), 64 words at a time, list their
 // rows in LDS and go through them 32 at a time; at the end the waves' sums are added in
 // wave order.
 template <typename T, int D, int KT>
@@ -813,8 +843,9 @@ int check_blocks(const shrimp_attn_blocks_args* a, bool back, const char* what) 
   SHRIMP_REQUIRE(a != nullptr, "%s: null arguments", what);
   SHRIMP_REQUIRE(a->dt == SHRIMP_DT_BF16 || a->dt == SHRIMP_DT_F16, "%s: element type %d", what, a->dt);
   SHRIMP_REQUIRE(a->B >= 0 && a->H >= 0 && a->Sq >= 0 && a->Sk >= 0, "%s: negative size", what);
-  SHRIMP_REQUIRE(a->Hk >= 1 && a->H % a->Hk == 0 && a->H / a->Hk <= R,
-                 "%s: %d query heads for %d key heads (at most %d each)", what, a->H, a->Hk, R);
+  SHRIMP_REQUIRE(a->Hk >= 1 && a->H % a->Hk == 0 && a->H / a->Hk <= SHRIMP_BLOCK_MAX_GROUP,
+                 "%s: %d query heads for %d key heads (at most %d each)", what, a->H, a->Hk,
+                 SHRIMP_BLOCK_MAX_GROUP);
   SHRIMP_REQUIRE(a->d >= 8 && a->d <= SHRIMP_BLOCK_MAX_D && a->d % 8 == 0,
                  "%s: head dim %d is not a multiple of 8 in [8, %d]", what, a->d, SHRIMP_BLOCK_MAX_D);
   SHRIMP_REQUIRE(a->block >= 16 && a->block % 16 == 0 && a->block <= (1 << 20),
@@ -837,7 +868,10 @@ int check_blocks(const shrimp_attn_blocks_args* a, bool back, const char* what) 
   return SHRIMP_OK;
 }
 
-BlocksParams blocks_params(const shrimp_attn_blocks_args* a) {
+// Keys that a wave scores at once (16 KT): the most of 64, 32 and 16 that divide a block.
+int key_step(int block) { return block % 64 == 0 ? 64 : block % 32 == 0 ? 32 : 16; }
+
+BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
   BlocksParams p{};
   p.q = static_cast<const uint16_t*>(a->q);
   p.k = static_cast<const uint16_t*>(a->k);
@@ -853,12 +887,35 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a) {
   p.B = a->B, p.H = a->H, p.Hk = a->Hk, p.Sq = a->Sq, p.Sk = a->Sk;
   p.d = a->d, p.block = a->block, p.topk = a->topk;
   p.group = a->H / a->Hk;
-  p.queries = p.group > 0 ? R / p.group : R;
+  const int rows = back || a->d > 64 ? 48 : 64;  // wave_rows
+  p.queries = p.group > 0 ? rows / p.group : rows;
   p.chunks = (a->Sq + p.queries - 1) / p.queries;
+  p.groups = (p.chunks + WAVES - 1) / WAVES;
+  // whole blocks of up to 64 keys together, or the largest part of a longer block that a
+  // product's key_step divides
+  const int step = key_step(a->block);
+  p.stage = step;
+  if (a->block <= STAGE)
+    p.stage = STAGE / a->block * a->block;
+  else
+    for (int keys = STAGE; keys > step; keys -= step)
+      if (a->block % keys == 0) {
+        p.stage = keys;
+        break;
+      }
   const int64_t pairs = (int64_t)a->B * a->Hk;
   p.by_xcd = pairs % 8 == 0 || pairs >= 64;
   p.scale2 = a->scale * LOG2E;
   return p;
+}
+
+template <typename T, int D, int KT, bool BACK>
+int launch_chunk(const BlocksParams& p, const GradParams& gp, unsigned blocks, hipStream_t st) {
+  constexpr int bytes = ChunkLds<D, BACK>::bytes;
+  SHRIMP_REQUIRE(bytes <= max_lds_per_block(), "attn_blocks: %d bytes of LDS, %d available", bytes,
+                 max_lds_per_block());
+  hipLaunchKernelGGL((attn_blocks_kernel<T, D, KT, BACK>), dim3(blocks), dim3(WAVES * 64), bytes, st, p, gp);
+  return SHRIMP_OK;
 }
 
 template <typename T, int D, int KT>
@@ -870,17 +927,15 @@ int launch_forward(const BlocksParams& p, hipStream_t st) {
     return SHRIMP_OK;
   }
   const int64_t pairs = (int64_t)p.B * p.Hk;
-  const int64_t n = (p.by_xcd ? (pairs + 7) / 8 * 8 : pairs) * p.chunks;
-  SHRIMP_REQUIRE(n <= INT32_MAX, "attn_blocks: %lld chunks of queries", (long long)n);
-  const size_t lds = (size_t)R * (row_floats<D>() + 2) * 4 + (size_t)WINDOW * 8;
-  hipLaunchKernelGGL((attn_blocks_kernel<T, D, KT>), dim3((unsigned)n), dim3(64), lds, st, p);
-  return SHRIMP_OK;
+  const int64_t n = (p.by_xcd ? (pairs + 7) / 8 * 8 : pairs) * p.groups;
+  SHRIMP_REQUIRE(n <= INT32_MAX, "attn_blocks: %lld groups of queries", (long long)n);
+  return launch_chunk<T, D, KT, false>(p, GradParams{}, (unsigned)n, st);
 }
 
 template <typename T, int D>
 int launch_forward_kt(const BlocksParams& p, hipStream_t st) {
-  if (p.block % 64 == 0) return launch_forward<T, D, 4>(p, st);
-  if (p.block % 32 == 0) return launch_forward<T, D, 2>(p, st);
+  if (key_step(p.block) == 64) return launch_forward<T, D, 4>(p, st);
+  if (key_step(p.block) == 32) return launch_forward<T, D, 2>(p, st);
   return launch_forward<T, D, 1>(p, st);
 }
 
@@ -895,7 +950,7 @@ int64_t grad_stat_bytes(const shrimp_attn_blocks_args* a) {
   return mul_sat({a->B, a->H, a->Sq, 8});
 }
 int64_t grad_mask_bytes(const shrimp_attn_blocks_args* a) {
-  const BlocksParams p = blocks_params(a);
+  const BlocksParams p = blocks_params(a, true);
   return mul_sat({a->B, a->Hk, ((int64_t)a->Sk + a->block - 1) / a->block, p.chunks, 8});
 }
 
@@ -909,14 +964,15 @@ template <typename T, int D, int KT>
 int launch_backward(const BlocksParams& p, GradParams gp, hipStream_t st) {
   constexpr int KG = key_tiles<D, KT>();
   const int64_t pairs = (int64_t)p.B * p.Hk, sets = p.by_xcd ? (pairs + 7) / 8 * 8 : pairs;
-  const int64_t n = sets * p.chunks;
+  const int64_t n = sets * p.groups;
   gp.segments = (p.Sk + KG * 16 - 1) / (KG * 16);
   const int64_t m = sets * gp.segments;
   SHRIMP_REQUIRE(n <= INT32_MAX && m <= INT32_MAX, "attn_blocks_backward: %lld chunks of queries, %lld of keys",
                  (long long)n, (long long)m);
-  const size_t lds = (size_t)R * (row_floats<D>() + 2) * 4 + (size_t)WINDOW * 8;
-  if (n > 0)
-    hipLaunchKernelGGL((attn_blocks_dq_kernel<T, D, KT>), dim3((unsigned)n), dim3(64), lds, st, p, gp);
+  if (n > 0) {
+    const int rc = launch_chunk<T, D, KT, true>(p, gp, (unsigned)n, st);
+    if (rc != SHRIMP_OK) return rc;
+  }
   if (m > 0) {
     // waves by the rows that a block has on average: tiles of 32 that stay full
     const int64_t rows = (int64_t)p.Sq * p.group * p.topk / (gp.nb > 0 ? gp.nb : 1);
@@ -930,8 +986,8 @@ int launch_backward(const BlocksParams& p, GradParams gp, hipStream_t st) {
 
 template <typename T, int D>
 int launch_backward_kt(const BlocksParams& p, const GradParams& gp, hipStream_t st) {
-  if (p.block % 64 == 0) return launch_backward<T, D, 4>(p, gp, st);
-  if (p.block % 32 == 0) return launch_backward<T, D, 2>(p, gp, st);
+  if (key_step(p.block) == 64) return launch_backward<T, D, 4>(p, gp, st);
+  if (key_step(p.block) == 32) return launch_backward<T, D, 2>(p, gp, st);
   return launch_backward<T, D, 1>(p, gp, st);
 }
 
@@ -950,7 +1006,7 @@ extern "C" int shrimp_attn_blocks(const shrimp_attn_blocks_args* a, void* stream
   const int rc = check_blocks(a, false, "attn_blocks");
   if (rc != SHRIMP_OK) return rc;
   if (a->B == 0 || a->H == 0 || a->Sq == 0) return SHRIMP_OK;
-  const BlocksParams p = blocks_params(a);
+  const BlocksParams p = blocks_params(a, false);
   const int e = a->dt == SHRIMP_DT_F16 ? launch_forward_d<_Float16>(p, as_stream(stream))
                                        : launch_forward_d<__bf16>(p, as_stream(stream));
   if (e != SHRIMP_OK) return e;
@@ -983,7 +1039,7 @@ extern "C" int shrimp_attn_blocks_backward(const shrimp_attn_blocks_args* a,
                      (g->workspace || stat + mask == 0) && reinterpret_cast<uintptr_t>(g->workspace) % 8 == 0,
                  "attn_blocks_backward: workspace of %lld bytes, %lld + %lld needed",
                  (long long)g->workspace_bytes, (long long)stat, (long long)mask);
-  const BlocksParams p = blocks_params(a);
+  const BlocksParams p = blocks_params(a, true);
   GradParams gp{};
   gp.g = static_cast<const uint16_t*>(g->g);
   gp.g_lse = g->g_lse;

@@ -33,7 +33,7 @@ from ._oplib import below, define
 MAX_HEAD_DIM = 128
 MAX_TOPK = 64
 MAX_BLOCKS = 4096
-MAX_GROUP = 64
+MAX_GROUP = 48
 
 _DT = {
     torch.float32: _lib.DT_F32,

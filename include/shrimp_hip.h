@@ -833,6 +833,7 @@ int shrimp_qk_norm_rope_backward(const shrimp_rope_args* a, void* dw_q, void* dw
 #define SHRIMP_BLOCK_MAX_D 128
 #define SHRIMP_BLOCK_MAX_TOPK 64
 #define SHRIMP_BLOCK_MAX_BLOCKS 4096
+#define SHRIMP_BLOCK_MAX_GROUP 48
 
 typedef struct {
   const void* q;
@@ -854,7 +855,7 @@ int shrimp_block_select(const shrimp_block_select_args* a, void* stream);
  * shrimp::attn_blocks: softmax attention of every query over its own blocks of keys
  * (no counterpart in the reference; shrimp_attn reads all of them).
  *   q (B, H, Sq, d), k, v (B, Hk, Sk, d) of type dt (SHRIMP_DT_BF16 / F16), Hk
- *     divides H, at most 64 query heads per key head; strides in elements,
+ *     divides H, at most SHRIMP_BLOCK_MAX_GROUP query heads per key head; strides in elements,
  *     multiples of 8, the last one 1, rows on 16-byte boundaries; d a multiple of
  *     8 up to SHRIMP_BLOCK_MAX_D. block a multiple of 16.
  *   sel (B, Hk, Sq, topk) int32 contiguous: a row's blocks in any order; entries

@@ -199,7 +199,7 @@ ATTN = [
     (2, 8, 8, 40, 264, 16, 16, 8, "bshd"),    # the benchmark's
     (1, 6, 2, 129, 300, 64, 48, 3, "odd"),    # groups of three, blocks of three tiles
     (1, 5, 1, 20, 70, 20, 16, 2, "odd"),      # a head dim of no vector
-    (1, 64, 1, 10, 64, 64, 16, 2, "bhsd"),    # the largest group
+    (1, 48, 1, 10, 64, 64, 16, 2, "bhsd"),    # the largest group
     (1, 40, 1, 11, 64, 8, 16, 2, "bhsd"),
     (2, 2, 2, 20, 20, 64, 64, 3, "bhsd"),     # one block, shorter than itself
     (3, 4, 1, 1, 300, 128, 64, 3, "bshd"),    # one new token
@@ -207,6 +207,10 @@ ATTN = [
     (1, 2, 2, 8, 1100, 32, 16, 64, "bhsd"),   # the most blocks a query can name
     (1, 1, 1, 70, 9000, 16, 16, 8, "bhsd"),   # more blocks than masks are held for
     (2, 2, 1, 33, 256, 128, 128, 1, "bshd"),
+    (1, 2, 1, 300, 333, 32, 96, 2, "bhsd"),   # blocks of two stages of 48
+    (1, 2, 2, 150, 700, 64, 112, 3, "bshd"),  # of seven of 16
+    (1, 48, 1, 20, 200, 128, 64, 2, "bhsd"),
+    (1, 3, 3, 270, 2300, 24, 32, 5, "bhsd"),  # two windows of masks
 ]
 
 
