@@ -19,6 +19,8 @@
 // a weight enters its product as the sum of two numbers of the type of V (one alone put the
 // error against float64 at 2.1e-3 of the result's norm in bf16 and that of dq at 2.5e-3;
 // two at 1.7e-3, the rounding of the result).
+#include <type_traits>
+
 #include "capi.hpp"
 #include "common.hpp"
 
@@ -27,16 +29,15 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr int WAVES = 4;    // waves of a chunk workgroup
 constexpr int STAGE = 64;   // keys in LDS at a time
 constexpr int WINDOW = 64;  // blocks whose row masks a wave holds at a time, one per lane
 
-// Rows of a wave (one bit each in a 64-bit mask): as many as the LDS of a compute unit
-// holds for four waves beside the keys.
-template <int D, bool BACK>
-constexpr int wave_rows() {
-  return D == 128 || BACK ? 48 : 64;
-}
+// Waves of a chunk workgroup and rows of a wave (one bit each in a 64-bit mask): two waves
+// per SIMD, or at D = 128 one, with the rows that a compute unit's LDS holds for them.
+template <int D>
+struct Chunk {
+  static constexpr int WAVES = D == 128 ? 4 : 8, R = D == 128 ? 48 : D == 64 ? 56 : 64;
+};
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -91,7 +92,8 @@ struct BlocksParams {
   const uint16_t* q;
   const uint16_t* k;
   const uint16_t* v;
-  int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn;
+  int64_t q_sb, k_sb, v_sb;
+  int q_sh, q_sn, k_sh, k_sn, v_sh, v_sn;  // below 2^31: an offset is one 32 x 32 bit product
   const int32_t* sel;
   const int32_t* q_lens;
   const int32_t* k_lens;
@@ -99,10 +101,12 @@ struct BlocksParams {
   float* lse;
   int B, H, Hk, Sq, Sk, d, block, topk;
   int group;    // query heads per key head
+  unsigned recip; // r / group = r recip >> 16 for r < 64
   int queries;  // queries per wave
   int chunks;   // waves' runs of queries per (sequence, key head)
-  int groups;   // workgroups of WAVES runs
-  int stage;    // keys per stage: whole blocks, or an equal part of one
+  int groups;   // workgroups of chunk runs
+  int stage;    // keys per stage: 2^shared whole blocks, or an equal part of one
+  int shared;
   int by_xcd;   // a key head's chunks stay on one XCD
   float scale2; // log2(e) / sqrt(d)
 };
@@ -134,7 +138,7 @@ using Words = unsigned __attribute__((ext_vector_type(W)));
 // KT tiles of 16 keys from key0 as the A operand of S^T = K Q^T: lane (lr, lg) has
 // dimensions 32 ks + 8 lg .. + 7 of key 16 kt + lr; zero past the keys and past d.
 template <int D, int KT>
-SHRIMP_DEV void load_rows(const uint16_t* base, int64_t sn, int key0, int len, int d, int lr, int lg,
+SHRIMP_DEV void load_rows(const uint16_t* base, int sn, int key0, int len, int d, int lr, int lg,
                           u32x4 (&f)[KT][D / 32]) {
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
@@ -154,7 +158,7 @@ struct Turned {
   static constexpr int EPL = D / 16, W = EPL / 2;
   Words<W> raw[KT][4];
 
-  SHRIMP_DEV void load(const uint16_t* base, int64_t sn, int key0, int len, int d, int lr, int lg) {
+  SHRIMP_DEV void load(const uint16_t* base, int sn, int key0, int len, int d, int lr, int lg) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -238,11 +242,8 @@ SHRIMP_DEV float soft_step(const f32x4 (&s)[KT], float scale2, float& m, float& 
   return alpha;
 }
 
-// 64-bit value of lane `src` for every lane.
-SHRIMP_DEV int64_t lane_i64(int64_t v, int src) {
-  return (int64_t)(unsigned)__builtin_amdgcn_ds_bpermute(src << 2, (int)v) |
-         (int64_t)__builtin_amdgcn_ds_bpermute(src << 2, (int)(v >> 32)) << 32;
-}
+// Row r < 64 of a run of queries: query r / group, head r % group.
+SHRIMP_DEV int row_query(const BlocksParams& p, int r) { return (int)((unsigned)r * p.recip >> 16); }
 
 // 16-byte pieces of a row of d elements as a product's operand (lane group lg), zeros
 // where `on` is false and past d.
@@ -252,6 +253,15 @@ SHRIMP_DEV void load_row(const uint16_t* row, bool on, int d, int lg, u32x4 (&f)
   for (int ks = 0; ks < D / 32; ++ks)
     f[ks] = on && ks * 32 + lg * 8 < d ? *reinterpret_cast<const u32x4*>(row + ks * 32 + lg * 8)
                                        : u32x4{0, 0, 0, 0};
+}
+
+// The same without zeros: past d a piece of the row's own again, for a product whose other
+// operand is zero there. (No branch stands around a load that the next products wait for.)
+template <int D>
+SHRIMP_DEV void load_any(const uint16_t* row, int d, int lg, u32x4 (&f)[D / 32]) {
+#pragma unroll
+  for (int ks = 0; ks < D / 32; ++ks)
+    f[ks] = *reinterpret_cast<const u32x4*>(row + min(ks * 32 + lg * 8, d - 8));
 }
 
 template <int D>
@@ -264,7 +274,8 @@ constexpr int row_floats() {
 struct GradParams {
   const uint16_t* g;
   const float* g_lse;  // or null
-  int64_t g_sb, g_sh, g_sn;
+  int64_t g_sb;
+  int g_sh, g_sn;
   uint16_t* dq;
   uint16_t* dk;
   uint16_t* dv;
@@ -286,17 +297,16 @@ SHRIMP_DEV float elem<_Float16>(unsigned word, int hi) {
 }
 
 // LDS of a chunk workgroup, in this order.
-template <int D, bool BACK>
+template <int D>
 struct ChunkLds {
-  static constexpr int R = wave_rows<D, BACK>(), RF = row_floats<D>();
-  static constexpr int RS = D + 8;             // 16-bit elements of a staged row
-  static constexpr bool ROWS = D <= 64;        // q (and g) rows are kept, else gathered from memory
-  static constexpr int acc = 0;                                      // [WAVES][R][RF] fp32
-  static constexpr int stat = acc + WAVES * R * RF * 4;              // [WAVES][R] float2
-  static constexpr int mask = stat + WAVES * R * 8;                  // [WAVES][WINDOW] u64
-  static constexpr int keys = mask + WAVES * WINDOW * 8;             // [2][STAGE][RS]
-  static constexpr int rows = keys + 2 * STAGE * RS * 2;             // [1 or 2][WAVES][R][RS]
-  static constexpr int bytes = rows + (ROWS ? (BACK ? 2 : 1) * WAVES * R * RS * 2 : 0);
+  static constexpr int WAVES = Chunk<D>::WAVES, R = Chunk<D>::R, RF = row_floats<D>();
+  static constexpr int RS = D + 8;                        // 16-bit elements of a staged row
+  static constexpr int acc = 0;                           // [WAVES][R][RF] fp32
+  static constexpr int stat = acc + WAVES * R * RF * 4;   // [WAVES][R] float2
+  static constexpr int mask = stat + WAVES * R * 8;       // [WAVES][WINDOW] u64
+  static constexpr int keys = mask + WAVES * WINDOW * 8;  // [2][STAGE][RS]
+  static constexpr int large = keys + 2 * STAGE * RS * 2;  // [WAVES] words
+  static constexpr int bytes = large + WAVES * 4;
   static_assert(bytes <= 160 * 1024, "a compute unit's LDS");
 };
 
@@ -308,33 +318,70 @@ SHRIMP_DEV void fill_masks(const BlocksParams& p, const int32_t* sel, int asking
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   const uint64_t ones = (1ull << p.group) - 1;
-  for (int j = lane; j < asking * p.topk; j += 64) {
-    const int s = sel[j];
-    const unsigned blk = (unsigned)s - (unsigned)w0;
-    if (s >= w0 && blk < (unsigned)WINDOW) {
-      const uint64_t bits = ones << (j / p.topk * p.group);
-      if ((unsigned)bits) atomicOr(&mask[2 * blk], (unsigned)bits);
-      if ((unsigned)(bits >> 32)) atomicOr(&mask[2 * blk + 1], (unsigned)(bits >> 32));
+  const int n = asking * p.topk;
+  for (int j0 = lane; j0 < n; j0 += 64 * 8) {
+    int s[8];  // eight entries in flight
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s[u] = sel[min(j0 + u * 64, n - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int j = j0 + u * 64;
+      const unsigned blk = (unsigned)s[u] - (unsigned)w0;
+      if (j < n && s[u] >= w0 && blk < (unsigned)WINDOW) {
+        const uint64_t bits = ones << (j / p.topk * p.group);
+        if ((unsigned)bits) atomicOr(&mask[2 * blk], (unsigned)bits);
+        if ((unsigned)(bits >> 32)) atomicOr(&mask[2 * blk + 1], (unsigned)(bits >> 32));
+      }
     }
   }
 }
 
-// The forward, and with BACK the gradient of q (see there).
-template <typename T, int D, int KT, bool BACK>
-__global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const BlocksParams p, const GradParams gp) {
+// A point that x has arrived at: its load is waited for here, where the loads behind it can
+// be counted, not at a use behind a branch or loop that makes the wait one for all.
+template <int N>
+SHRIMP_DEV void arrived(u32x4 (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
+}
+
+// A bound on |x| of finite elements whose products stay finite: 2^56 for bf16, the largest
+// number for fp16 (as bits without the sign).
+template <typename T>
+constexpr uint16_t large_bits() {
+  return std::is_same<T, __bf16>::value ? (127 + 56) << 7 : 0x7C00;
+}
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+SHRIMP_DEV u16x2 max_bits(u16x2 m, u32x4 x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[i] & 0x7FFF7FFFu));
+  return m;
+}
+
+SHRIMP_DEV uint64_t lane_u64(uint64_t v, int lane) {  // (lane: wave-uniform)
+  return (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+// The forward, and with BACK the gradient of q (see there). MULTI: stages of two or four
+// blocks (of 32 or 16 keys).
+template <typename T, int D, bool BACK, bool MULTI>
+__global__ __launch_bounds__(Chunk<D>::WAVES * 64, 1) void attn_blocks_kernel(const BlocksParams p,
+                                                                             const GradParams gp) {
   extern __shared__ __align__(16) char lds[];
-  using L = ChunkLds<D, BACK>;
-  constexpr int R = L::R, RF = L::RF, RS = L::RS, EPL = D / 16, KS = D / 32, W = EPL / 2;
-  constexpr int LPR = D / 4;                                 // lanes of a row, four dimensions each
-  constexpr int PIECES = STAGE * (D / 8) / (WAVES * 64);     // 16-byte pieces of a stage per thread
+  using L = ChunkLds<D>;
+  constexpr int WAVES = L::WAVES, R = L::R, RF = L::RF, RS = L::RS;
+  constexpr int EPL = D / 16, KS = D / 32, W = EPL / 2, KT = STAGE / 16;
+  constexpr int LPR = D / 4;                                        // lanes of a row, four dimensions each
+  constexpr int ALL = STAGE * (D / 8);                              // 16-byte pieces of a stage
+  constexpr int PIECES = (ALL + WAVES * 64 - 1) / (WAVES * 64);
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4, wave = wave_id();
   float* acc_lds = reinterpret_cast<float*>(lds + L::acc) + wave * R * RF;
   float2* stat_lds = reinterpret_cast<float2*>(lds + L::stat) + wave * R;
   unsigned* mask_lds = reinterpret_cast<unsigned*>(lds + L::mask);
   uint16_t* k_lds = reinterpret_cast<uint16_t*>(lds + L::keys);
   uint16_t* v_lds = k_lds + STAGE * RS;
-  uint16_t* q_lds = reinterpret_cast<uint16_t*>(lds + L::rows) + wave * R * RS;
-  uint16_t* g_lds = q_lds + WAVES * R * RS;
+  unsigned* large_lds = reinterpret_cast<unsigned*>(lds + L::large);
   int64_t bh;
   int grp;
   if (!place_chunk(p, p.groups, bh, grp)) return;
@@ -345,24 +392,27 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
   const int queries = min(p.queries, p.Sq - q0);        // written
   const int asking = min(queries, max(q_len - q0, 0));  // with a choice
   const int live = (k_len + p.block - 1) / p.block;
-  const uint16_t* q = p.q + b * p.q_sb;
-  const uint16_t* g = BACK ? gp.g + b * gp.g_sb : nullptr;
-  const uint16_t* k = p.k + b * p.k_sb + hk * p.k_sh;
-  const uint16_t* v = p.v + b * p.v_sb + hk * p.v_sh;
+  // rows of the wave: query q0 + r / G, head hk G + r % G
+  const int first = min(q0, p.Sq - 1);  // (a row to read where the wave has none)
+  const uint16_t* q = p.q + b * p.q_sb + (int64_t)(hk * p.group) * p.q_sh + (int64_t)first * p.q_sn;
+  const uint16_t* g =
+      BACK ? gp.g + b * gp.g_sb + (int64_t)(hk * p.group) * gp.g_sh + (int64_t)first * gp.g_sn : nullptr;
+  const uint16_t* k = p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
+  const uint16_t* v = p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
   const int32_t* sel = p.sel + (bh * p.Sq + q0) * p.topk;
+  const int64_t out0 = ((int64_t)b * p.H + hk * p.group) * p.Sq + q0;  // of row 0
 
-  // rows of the wave: query r / G, head r % G
   for (int i = lane; i < R * RF; i += 64) acc_lds[i] = 0.f;
   if constexpr (BACK) {
     for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
       const int r = r0 + lane / LPR, c = lane % LPR;
       const bool on = r < queries * p.group;
-      const int query = on ? r / p.group : 0, head = hk * p.group + (on ? r - query * p.group : 0);
-      const int64_t o = ((int64_t)b * p.H + head) * p.Sq + q0 + query;
+      const int query = on ? row_query(p, r) : 0, head = on ? r - query * p.group : 0;
+      const int64_t o = out0 + (int64_t)head * p.Sq + query;
       float delta = 0.f;
       if (on && c * 4 < p.d) {
         const u32x2 x = *reinterpret_cast<const u32x2*>(p.out + o * p.d + c * 4);
-        const u32x2 y = *reinterpret_cast<const u32x2*>(g + head * gp.g_sh + (int64_t)(q0 + query) * gp.g_sn + c * 4);
+        const u32x2 y = *reinterpret_cast<const u32x2*>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn + c * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) delta = fmaf(elem<T>(x[e >> 1], e & 1), elem<T>(y[e >> 1], e & 1), delta);
       }
@@ -376,145 +426,61 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
       }
     }
   } else {
-    for (int r = lane; r < R; r += 64) stat_lds[r] = float2{-INFINITY, 0.f};  // maximum, sum
-  }
-  const int my_query = lane / p.group, my_head = hk * p.group + lane - my_query * p.group;
-  const int64_t my_row = my_head * p.q_sh + (int64_t)(q0 + my_query) * p.q_sn;
-  const int64_t my_grad = BACK ? my_head * gp.g_sh + (int64_t)(q0 + my_query) * gp.g_sn : 0;
-  if constexpr (L::ROWS) {
-    for (int i = lane; i < R * (D / 8); i += 64) {
-      const int r = i / (D / 8), c = i % (D / 8);
-      const bool on = r < asking * p.group && c * 8 < p.d;
-      const int query = on ? r / p.group : 0, head = hk * p.group + (on ? r - query * p.group : 0);
-      const u32x4 none = {0, 0, 0, 0};
-      *reinterpret_cast<u32x4*>(q_lds + r * RS + c * 8) =
-          on ? *reinterpret_cast<const u32x4*>(q + head * p.q_sh + (int64_t)(q0 + query) * p.q_sn + c * 8) : none;
-      if constexpr (BACK)
-        *reinterpret_cast<u32x4*>(g_lds + r * RS + c * 8) =
-            on ? *reinterpret_cast<const u32x4*>(g + head * gp.g_sh + (int64_t)(q0 + query) * gp.g_sn + c * 8) : none;
-    }
+    if (lane < R) stat_lds[lane] = float2{-INFINITY, 0.f};  // maximum, sum
   }
 
-  // stage of keys from key0: requested into registers, put into LDS by `store`
+  // Stage of keys from key0: requested into registers, put into LDS by `store`. Requests go
+  // out without a condition (keys and dimensions past the end: the last ones again), so
+  // that later waits can count them; the zeros are put in on the way to LDS.
   u32x4 kr[PIECES], vr[PIECES];
   auto request = [&](int key0) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int row = (tid + i * WAVES * 64) / (D / 8), c = (tid + i * WAVES * 64) % (D / 8);
-      const bool on = row < p.stage && key0 + row < k_len && c * 8 < p.d;
-      const u32x4 none = {0, 0, 0, 0};
-      kr[i] = on ? *reinterpret_cast<const u32x4*>(k + (int64_t)(key0 + row) * p.k_sn + c * 8) : none;
-      vr[i] = on ? *reinterpret_cast<const u32x4*>(v + (int64_t)(key0 + row) * p.v_sn + c * 8) : none;
+      const int at = tid + i * WAVES * 64, row = min(key0 + at / (D / 8), k_len - 1);
+      const int c = min(at % (D / 8) * 8, p.d - 8);
+      kr[i] = *reinterpret_cast<const u32x4*>(k + (int64_t)row * p.k_sn + c);
+      vr[i] = *reinterpret_cast<const u32x4*>(v + (int64_t)row * p.v_sn + c);
     }
   };
-  auto store = [&]() {
+  auto store = [&](int key0) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int row = (tid + i * WAVES * 64) / (D / 8), c = (tid + i * WAVES * 64) % (D / 8);
-      *reinterpret_cast<u32x4*>(k_lds + row * RS + c * 8) = kr[i];
-      *reinterpret_cast<u32x4*>(v_lds + row * RS + c * 8) = vr[i];
-    }
-  };
-
-  // the wave's rows of `mask` against `keys` keys at row `at` of the stage (key0 of the sequence)
-  auto work = [&](uint64_t mask, int at, int keys, int key0) {
-    const int count = __popcll(mask);
-    // lane j: the j-th row of the mask (the others behind them)
-    const bool in = mask >> lane & 1;
-    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
-                                                 __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
-    const int row_at = __builtin_amdgcn_ds_permute((in ? before : count + lane - before) << 2, lane);
-    for (int t = 0; t < count; t += 16) {
-      const bool on = t + lr < count;
-      const int listed = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at), row = on ? listed : 0;
-      u32x4 qf[KS], gf[KS];
-      if constexpr (L::ROWS) {
+      const int at = tid + i * WAVES * 64, row = at / (D / 8), c = at % (D / 8);
+      const bool keep = row < p.stage && key0 + row < k_len && c * 8 < p.d;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          qf[ks] = *reinterpret_cast<const u32x4*>(q_lds + row * RS + ks * 32 + lg * 8);
-          if constexpr (BACK) gf[ks] = *reinterpret_cast<const u32x4*>(g_lds + row * RS + ks * 32 + lg * 8);
-        }
-      } else {
-        load_row<D>(q + lane_i64(my_row, row), on, p.d, lg, qf);
-        if constexpr (BACK) load_row<D>(g + lane_i64(my_grad, row), on, p.d, lg, gf);
+      for (int w = 0; w < 4; ++w) {
+        kr[i][w] = keep ? kr[i][w] : 0;
+        vr[i][w] = keep ? vr[i][w] : 0;
       }
-      float2 st = stat_lds[row];
-      float* mine = acc_lds + row * RF + lg * EPL * 4;
-      f32x4 acc[EPL];
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(mine + e * 4);
-      for (int kk = 0; kk < keys; kk += KT * 16) {
-        const uint16_t* kp = k_lds + (at + kk) * RS;
-        const uint16_t* vp = v_lds + (at + kk) * RS;
-        f32x4 s[KT];
-        score_start<KT>(key0 + kk, k_len, lg, s);
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-            s[kt] = Mma<T>::k32(*reinterpret_cast<const u32x4*>(kp + (kt * 16 + lr) * RS + ks * 32 + lg * 8),
-                                qf[ks], s[kt]);
-        Turned<D, KT> turned;
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            turned.raw[kt][j] = *reinterpret_cast<const Words<W>*>((BACK ? kp : vp) + (kt * 16 + lg * 4 + j) * RS + lr * EPL);
-        u32x2 hi[KT], lo[KT];
-        if constexpr (BACK) {
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            f32x4 dp = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-              dp = Mma<T>::k32(*reinterpret_cast<const u32x4*>(vp + (kt * 16 + lr) * RS + ks * 32 + lg * 8),
-                               gf[ks], dp);
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], p.scale2, -st.x)) * gp.scale * (dp[i] - st.y);
-            Mma<T>::split(w, hi[kt], lo[kt]);
-          }
-        } else {
-          const float alpha = soft_step<T, KT>(s, p.scale2, st.x, st.y, hi, lo);
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) acc[e] *= alpha;
-        }
-        weigh<T, D, KT>(turned, hi, lo, acc);
+      if (ALL % (WAVES * 64) == 0 || at < ALL) {
+        *reinterpret_cast<u32x4*>(k_lds + row * RS + c * 8) = kr[i];
+        *reinterpret_cast<u32x4*>(v_lds + row * RS + c * 8) = vr[i];
       }
-      if (on) {
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(mine + e * 4) = acc[e];
-        if (!BACK && lg == 0) stat_lds[row] = st;
-      }
-      // (the rows' state is read again by other lanes of the wave)
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
   };
 
   __syncthreads();
-  const int per_stage = p.stage > p.block ? p.stage / p.block : 1;  // blocks of a stage
+  const int shared = MULTI ? p.shared : 0, per_stage = 1 << shared;  // blocks of a stage
+  const int tile_shift = 2 - shared;                                   // of its 16-key tiles per block
+  static_assert(KT == 4, "a stage of four tiles");
   for (int w0 = 0; w0 < live; w0 += WINDOW) {
     fill_masks(p, sel, asking, w0, mask_lds + wave * 2 * WINDOW, lane);
     __syncthreads();
+    const bool here = w0 + lane < live;
     uint64_t any = 0, mine = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      const uint64_t m = reinterpret_cast<const uint64_t*>(mask_lds)[w * WINDOW + lane];
+      const uint64_t m = here ? reinterpret_cast<const uint64_t*>(mask_lds)[w * WINDOW + lane] : 0;
       any |= m;
       if (w == wave) mine = m;
     }
-    const bool here = w0 + lane < live;
     if constexpr (BACK)
       if (here && chunk < p.chunks) gp.masks[(bh * gp.nb + w0 + lane) * p.chunks + chunk] = mine;
-    uint64_t todo = __ballot(here && any != 0);
-    // stages that hold a chosen block, ascending
-    const uint64_t stage_bits = per_stage >= 64 ? ~0ull : (1ull << per_stage) - 1;
-    int at = 0, key0 = 0;  // first block (of the window) and key of the stage
+    uint64_t todo = __ballot(any != 0);
+    const uint64_t stage_bits = (1u << per_stage) - 1;
+    int at = 0, key0 = 0;  // first block (of the window) and first key of a stage with chosen blocks
     auto first_of = [&]() {
-      at = __builtin_ctzll(todo) / per_stage * per_stage;
+      at = __builtin_ctzll(todo) >> shared << shared;
       key0 = (w0 + at) * p.block;
     };
     if (todo) {
@@ -522,27 +488,169 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
       request(key0);
     }
     while (todo) {
+      const int now_key = key0;
+      // the wave's rows that chose a block of the stage, and which of its blocks
+      uint64_t mask[MULTI ? 4 : 1];
+#pragma unroll
+      for (int i = 0; i < (MULTI ? 4 : 1); ++i)
+        mask[i] = i < 2 || shared == 2 ? lane_u64(mine, min(at + i, WINDOW - 1)) : 0;
+      uint64_t rows = mask[0];
+      if constexpr (MULTI) rows |= mask[1] | mask[2] | mask[3];
+      int count, row_at, row = 0;
+      u32x4 qf[KS], gf[KS];
+      bool on = false;
+      auto gather = [&](int t) {  // rows t .. t + 15 of the list
+        on = t + lr < count;
+        const int listed = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at);
+        row = on ? listed : 0;
+        const int query = row_query(p, row), head = row - query * p.group;
+        load_any<D>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn, p.d, lg, qf);
+        if constexpr (BACK) load_any<D>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn, p.d, lg, gf);
+      };
+      auto list = [&](uint64_t of) {  // lane j: the j-th row (the others behind them)
+        count = __popcll(of);
+        const bool in = of >> lane & 1;
+        const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(of >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo((unsigned)of, 0));
+        row_at = __builtin_amdgcn_ds_permute((in ? before : count + lane - before) << 2, lane);
+        gather(0);
+      };
       __syncthreads();  // the stage before is done with
-      store();
-      const int now = at, now_key = key0;
+      store(now_key);
+      if constexpr (MULTI) {
+        u16x2 m = {0, 0};
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) m = max_bits(max_bits(m, kr[i]), vr[i]);
+        const bool large = m[0] >= large_bits<T>() || m[1] >= large_bits<T>();
+        const uint64_t some = __ballot(large);
+        if (lane == 0) large_lds[wave] = some != 0;
+      }
       // the next stage: of the same block, or of the next chosen one
       key0 += p.stage;
       if (p.stage >= p.block || key0 >= min((w0 + at + 1) * p.block, k_len)) {
         todo &= ~(stage_bits << at);
         if (todo) first_of();
       }
-      if (todo) request(key0);
+      list(rows);
+      request(key0);  // (after the last stage of a window: that one again)
+      arrived(qf);
+      if constexpr (BACK) arrived(gf);
       __syncthreads();
-      if (p.stage > p.block) {
-        for (int i = 0; i < per_stage && now + i < WINDOW; ++i) {
-          const uint64_t mask = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), now + i) << 32 |
-                                (unsigned)__builtin_amdgcn_readlane((int)mine, now + i);
-          if (mask && w0 + now + i < live) work(mask, i * p.block, p.block, now_key + i * p.block);
+      if (rows == 0) continue;
+      // The blocks of a stage share their products, where a row that did not choose one has
+      // scores of -inf and weights of 0; keys or values that are not finite, or large
+      // enough for scores that are not, would reach it all the same (0 times infinity),
+      // so such a stage goes block by block.
+      unsigned large = 0;
+      if constexpr (MULTI) {
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) large |= large_lds[w];
+      }
+      const int passes = MULTI && __builtin_amdgcn_readfirstlane((int)large) ? per_stage : 1;
+      const int end = min(k_len, now_key + p.stage);  // keys of the stage
+      for (int pass = 0; pass < passes; ++pass) {
+        if (MULTI && passes > 1) {
+          constexpr int M = MULTI;
+          const uint64_t only = pass == 0 ? mask[0] : pass == 1 ? mask[M] : pass == 2 ? mask[2 * M] : mask[3 * M];
+          if (only == 0) continue;
+          list(only);
+          arrived(qf);
+          if constexpr (BACK) arrived(gf);
         }
-      } else {
-        const uint64_t mask = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), now) << 32 |
-                              (unsigned)__builtin_amdgcn_readlane((int)mine, now);
-        if (mask) work(mask, 0, p.stage, now_key);
+        u32x4 kf[KT][KS], vf[KT][KS];
+        Turned<D, KT> turned;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            kf[kt][ks] = *reinterpret_cast<const u32x4*>(k_lds + (kt * 16 + lr) * RS + ks * 32 + lg * 8);
+            if constexpr (BACK)
+              vf[kt][ks] = *reinterpret_cast<const u32x4*>(v_lds + (kt * 16 + lr) * RS + ks * 32 + lg * 8);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            turned.raw[kt][j] = *reinterpret_cast<const Words<W>*>((BACK ? k_lds : v_lds) +
+                                                                  (kt * 16 + lg * 4 + j) * RS + lr * EPL);
+        }
+        if (MULTI && passes > 1) {
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+            if (kt >> tile_shift != pass) {
+#pragma unroll
+              for (int ks = 0; ks < KS; ++ks) {
+                kf[kt][ks] = u32x4{0, 0, 0, 0};
+                if constexpr (BACK) vf[kt][ks] = u32x4{0, 0, 0, 0};
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) turned.raw[kt][j] = (Words<W>)0u;
+            }
+        }
+        for (int t = 0;;) {
+          float2 st = stat_lds[row];
+          float* to = acc_lds + row * RF + lg * EPL * 4;
+          f32x4 acc[EPL];
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(to + e * 4);
+          f32x4 s[KT];
+          if (now_key + STAGE <= end) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+          } else {
+            score_start<KT>(now_key, end, lg, s);
+          }
+          if constexpr (MULTI) {
+            // bit i: the row chose block i of the stage (and the pass is for it)
+            unsigned chose = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) chose |= (unsigned)(mask[i] >> row & 1) << i;
+            if (passes > 1) chose &= 1u << pass;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+              const bool none = !(chose >> (kt >> tile_shift) & 1);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[kt][i] = none ? -INFINITY : s[kt][i];
+            }
+          }
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], qf[ks], s[kt]);
+          u32x2 hi[KT], lo[KT];
+          if constexpr (BACK) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+              f32x4 dp = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int ks = 0; ks < KS; ++ks) dp = Mma<T>::k32(vf[kt][ks], gf[ks], dp);
+              float w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], p.scale2, -st.x)) * gp.scale * (dp[i] - st.y);
+              Mma<T>::split(w, hi[kt], lo[kt]);
+            }
+          } else {
+            const float alpha = soft_step<T, KT>(s, p.scale2, st.x, st.y, hi, lo);
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) acc[e] *= alpha;
+          }
+          const int at_row = row;
+          const bool mine_on = on;
+          t += 16;
+          if (t < count) gather(t);  // (in flight under the products)
+          weigh<T, D, KT>(turned, hi, lo, acc);
+          arrived(qf);
+          if constexpr (BACK) arrived(gf);
+          if (mine_on) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(to + e * 4) = acc[e];
+            if (!BACK && lg == 0) stat_lds[at_row] = st;
+          }
+          // (the rows' state is read again by other lanes of the wave)
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+          if (t >= count) break;
+        }
       }
     }
     __syncthreads();  // the masks are read
@@ -551,8 +659,8 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
   for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
     const int r = r0 + lane / LPR, c = lane % LPR;
     if (r >= queries * p.group) continue;
-    const int query = r / p.group, head = hk * p.group + r - query * p.group;
-    const int64_t o = ((int64_t)b * p.H + head) * p.Sq + q0 + query;
+    const int query = row_query(p, r), head = r - query * p.group;
+    const int64_t o = out0 + (int64_t)head * p.Sq + query;
     const float2 st = stat_lds[r];
     const float inv = BACK ? 1.f : st.y == 0.f ? 0.f : 1.f / st.y;
     if (c * 4 < p.d) {
@@ -588,13 +696,13 @@ __global__ __launch_bounds__(QW * 64) void attn_blocks_query_kernel(const Blocks
   // lane t: entry t of the choice (topk <= 64), -1 where nothing is to be read
   int mine = lane < p.topk ? p.sel[(bh * p.Sq + i) * p.topk + lane] : -1;
   if (mine >= live) mine = -1;
-  const uint16_t* k = p.k + b * p.k_sb + hk * p.k_sh;
-  const uint16_t* v = p.v + b * p.v_sb + hk * p.v_sh;
+  const uint16_t* k = p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
+  const uint16_t* v = p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
 
   for (int g0 = 0; g0 < p.group; g0 += 16) {  // heads of the key head, 16 rows
     const int head = hk * p.group + g0 + lr;
     const bool on = g0 + lr < p.group;
-    const uint16_t* q = p.q + b * p.q_sb + head * p.q_sh + (int64_t)i * p.q_sn;
+    const uint16_t* q = p.q + b * p.q_sb + (int64_t)head * p.q_sh + (int64_t)i * p.q_sn;
     u32x4 qf[KS];
     load_row<D>(q, on, p.d, lg, qf);
     float m = -INFINITY, l = 0.f;
@@ -691,8 +799,8 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
   const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
   const int k_len = min(max(p.k_lens[b], 0), p.Sk);
   const int key0 = seg * KT * 16, blk = key0 / p.block;
-  const uint16_t* q = p.q + b * p.q_sb + hk * p.group * p.q_sh;
-  const uint16_t* g = gp.g + b * gp.g_sb + hk * p.group * gp.g_sh;
+  const uint16_t* q = p.q + b * p.q_sb + (int64_t)(hk * p.group) * p.q_sh;
+  const uint16_t* g = gp.g + b * gp.g_sb + (int64_t)(hk * p.group) * gp.g_sh;
   const float2* stat = gp.stat + ((int64_t)b * p.H + hk * p.group) * p.Sq;
 
   f32x4 dk[KT][EPL], dv[KT][EPL];
@@ -703,8 +811,8 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
 
   if (key0 < k_len) {
     u32x4 kf[KT][KS], vf[KT][KS];
-    load_rows<D, KT>(p.k + b * p.k_sb + hk * p.k_sh, p.k_sn, key0, k_len, p.d, lr, lg, kf);
-    load_rows<D, KT>(p.v + b * p.v_sb + hk * p.v_sh, p.v_sn, key0, k_len, p.d, lr, lg, vf);
+    load_rows<D, KT>(p.k + b * p.k_sb + (int64_t)hk * p.k_sh, p.k_sn, key0, k_len, p.d, lr, lg, kf);
+    load_rows<D, KT>(p.v + b * p.v_sb + (int64_t)hk * p.v_sh, p.v_sn, key0, k_len, p.d, lr, lg, vf);
     f32x4 start_at[KT];  // the lane's key (column lr of each tile)
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
@@ -737,7 +845,7 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
         auto locate = [&](int i, int& query, int& head) {
           const bool on = i < count;
           const int e = on ? list[i] : 0;
-          const int r = e & 63, qi = r / p.group;
+          const int r = e & 63, qi = row_query(p, r);
           query = on ? (c0 + (e >> 6) * waves + wave) * p.queries + qi : -1;
           head = r - qi * p.group;
         };
@@ -748,15 +856,15 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
         for (int rt = 0; rt < 2; ++rt) {
           int query, head;
           locate(t + rt * 16 + lr, query, head);
-          load_row<D>(q + head * p.q_sh + (int64_t)query * p.q_sn, query >= 0, p.d, lg, qf[rt]);
-          load_row<D>(g + head * gp.g_sh + (int64_t)query * gp.g_sn, query >= 0, p.d, lg, gf[rt]);
+          load_row<D>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn, query >= 0, p.d, lg, qf[rt]);
+          load_row<D>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn, query >= 0, p.d, lg, gf[rt]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             locate(t + rt * 16 + lg * 4 + j, query, head);
             const bool on = query >= 0, wide = on && lr * EPL < p.d;
-            qt[rt][j] = wide ? *reinterpret_cast<const Words<W>*>(q + head * p.q_sh + (int64_t)query * p.q_sn + lr * EPL)
+            qt[rt][j] = wide ? *reinterpret_cast<const Words<W>*>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn + lr * EPL)
                              : (Words<W>)0u;
-            gt[rt][j] = wide ? *reinterpret_cast<const Words<W>*>(g + head * gp.g_sh + (int64_t)query * gp.g_sn + lr * EPL)
+            gt[rt][j] = wide ? *reinterpret_cast<const Words<W>*>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn + lr * EPL)
                              : (Words<W>)0u;
             st[rt][j] = on ? stat[(int64_t)head * p.Sq + query] : float2{INFINITY, 0.f};
           }
@@ -855,20 +963,22 @@ int check_blocks(const shrimp_attn_blocks_args* a, bool back, const char* what) 
   SHRIMP_REQUIRE(a->Sq <= (1 << 30) && a->Sk <= (1 << 30), "%s: Sq=%d, Sk=%d", what, a->Sq, a->Sk);
   SHRIMP_REQUIRE(a->scale > 0.f, "%s: scale must be positive", what);
   auto aligned = [](const void* base, int64_t sb, int64_t sh, int64_t sn) {
-    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && sb % 8 == 0 && sh % 8 == 0 && sn % 8 == 0;
+    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && sb % 8 == 0 && sh % 8 == 0 && sn % 8 == 0 &&
+           strides_ok({sh, sn});
   };
   const bool rows = a->B > 0 && a->H > 0 && a->Sq > 0, keys = a->B > 0 && a->Sk > 0 && (rows || back);
   SHRIMP_REQUIRE(!rows || (a->q && a->sel && a->q_lens && a->k_lens && a->out && a->lse),
                  "%s: null pointer", what);
   SHRIMP_REQUIRE(!keys || (a->k && a->v && a->k_lens), "%s: null k, v or k_lens", what);
   SHRIMP_REQUIRE(!rows || (aligned(a->q, a->q_sb, a->q_sh, a->q_sn) && aligned(a->out, 0, 0, 0)),
-                 "%s: rows must start on 16-byte boundaries", what);
+                 "%s: rows must start on 16-byte boundaries, strides be below 2^31", what);
   SHRIMP_REQUIRE(!keys || (aligned(a->k, a->k_sb, a->k_sh, a->k_sn) && aligned(a->v, a->v_sb, a->v_sh, a->v_sn)),
-                 "%s: rows must start on 16-byte boundaries", what);
+                 "%s: rows must start on 16-byte boundaries, strides be below 2^31", what);
   return SHRIMP_OK;
 }
 
-// Keys that a wave scores at once (16 KT): the most of 64, 32 and 16 that divide a block.
+// Keys that a wave of the other two kernels scores at once (16 KT): the most of 64, 32 and
+// 16 that divide a block.
 int key_step(int block) { return block % 64 == 0 ? 64 : block % 32 == 0 ? 32 : 16; }
 
 BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
@@ -876,9 +986,9 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
   p.q = static_cast<const uint16_t*>(a->q);
   p.k = static_cast<const uint16_t*>(a->k);
   p.v = static_cast<const uint16_t*>(a->v);
-  p.q_sb = a->q_sb, p.q_sh = a->q_sh, p.q_sn = a->q_sn;
-  p.k_sb = a->k_sb, p.k_sh = a->k_sh, p.k_sn = a->k_sn;
-  p.v_sb = a->v_sb, p.v_sh = a->v_sh, p.v_sn = a->v_sn;
+  p.q_sb = a->q_sb, p.q_sh = (int)a->q_sh, p.q_sn = (int)a->q_sn;
+  p.k_sb = a->k_sb, p.k_sh = (int)a->k_sh, p.k_sn = (int)a->k_sn;
+  p.v_sb = a->v_sb, p.v_sh = (int)a->v_sh, p.v_sn = (int)a->v_sn;
   p.sel = a->sel;
   p.q_lens = a->q_lens;
   p.k_lens = a->k_lens;
@@ -887,18 +997,19 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
   p.B = a->B, p.H = a->H, p.Hk = a->Hk, p.Sq = a->Sq, p.Sk = a->Sk;
   p.d = a->d, p.block = a->block, p.topk = a->topk;
   p.group = a->H / a->Hk;
-  const int rows = back || a->d > 64 ? 48 : 64;  // wave_rows
+  p.recip = p.group > 0 ? (65536u + p.group - 1) / p.group : 0;
+  const int rows = a->d > 64 ? Chunk<128>::R : a->d > 32 ? Chunk<64>::R : Chunk<32>::R;
+  const int waves = a->d > 64 ? Chunk<128>::WAVES : a->d > 32 ? Chunk<64>::WAVES : Chunk<32>::WAVES;
   p.queries = p.group > 0 ? rows / p.group : rows;
   p.chunks = (a->Sq + p.queries - 1) / p.queries;
-  p.groups = (p.chunks + WAVES - 1) / WAVES;
-  // whole blocks of up to 64 keys together, or the largest part of a longer block that a
-  // product's key_step divides
-  const int step = key_step(a->block);
-  p.stage = step;
+  p.groups = (p.chunks + waves - 1) / waves;
+  // whole blocks of up to 64 keys together, or the largest equal part of a longer block
+  p.stage = 16;
+  p.shared = a->block == 16 ? 2 : a->block == 32 ? 1 : 0;
   if (a->block <= STAGE)
-    p.stage = STAGE / a->block * a->block;
+    p.stage = a->block << p.shared;
   else
-    for (int keys = STAGE; keys > step; keys -= step)
+    for (int keys = STAGE; keys > 16; keys -= 16)
       if (a->block % keys == 0) {
         p.stage = keys;
         break;
@@ -909,12 +1020,16 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
   return p;
 }
 
-template <typename T, int D, int KT, bool BACK>
+template <typename T, int D, bool BACK>
 int launch_chunk(const BlocksParams& p, const GradParams& gp, unsigned blocks, hipStream_t st) {
-  constexpr int bytes = ChunkLds<D, BACK>::bytes;
+  constexpr int bytes = ChunkLds<D>::bytes;
   SHRIMP_REQUIRE(bytes <= max_lds_per_block(), "attn_blocks: %d bytes of LDS, %d available", bytes,
                  max_lds_per_block());
-  hipLaunchKernelGGL((attn_blocks_kernel<T, D, KT, BACK>), dim3(blocks), dim3(WAVES * 64), bytes, st, p, gp);
+  const dim3 threads(Chunk<D>::WAVES * 64);
+  if (p.shared)
+    hipLaunchKernelGGL((attn_blocks_kernel<T, D, BACK, true>), dim3(blocks), threads, bytes, st, p, gp);
+  else
+    hipLaunchKernelGGL((attn_blocks_kernel<T, D, BACK, false>), dim3(blocks), threads, bytes, st, p, gp);
   return SHRIMP_OK;
 }
 
@@ -929,7 +1044,7 @@ int launch_forward(const BlocksParams& p, hipStream_t st) {
   const int64_t pairs = (int64_t)p.B * p.Hk;
   const int64_t n = (p.by_xcd ? (pairs + 7) / 8 * 8 : pairs) * p.groups;
   SHRIMP_REQUIRE(n <= INT32_MAX, "attn_blocks: %lld groups of queries", (long long)n);
-  return launch_chunk<T, D, KT, false>(p, GradParams{}, (unsigned)n, st);
+  return launch_chunk<T, D, false>(p, GradParams{}, (unsigned)n, st);
 }
 
 template <typename T, int D>
@@ -970,7 +1085,7 @@ int launch_backward(const BlocksParams& p, GradParams gp, hipStream_t st) {
   SHRIMP_REQUIRE(n <= INT32_MAX && m <= INT32_MAX, "attn_blocks_backward: %lld chunks of queries, %lld of keys",
                  (long long)n, (long long)m);
   if (n > 0) {
-    const int rc = launch_chunk<T, D, KT, true>(p, gp, (unsigned)n, st);
+    const int rc = launch_chunk<T, D, true>(p, gp, (unsigned)n, st);
     if (rc != SHRIMP_OK) return rc;
   }
   if (m > 0) {
@@ -1031,7 +1146,7 @@ extern "C" int shrimp_attn_blocks_backward(const shrimp_attn_blocks_args* a,
   SHRIMP_REQUIRE(!rows || (g->g && g->dq), "attn_blocks_backward: null gradient of out or q");
   SHRIMP_REQUIRE(a->Sk == 0 || (g->dk && g->dv), "attn_blocks_backward: null gradient of k or v");
   SHRIMP_REQUIRE(reinterpret_cast<uintptr_t>(g->g) % 16 == 0 && g->g_sb % 8 == 0 && g->g_sh % 8 == 0 &&
-                     g->g_sn % 8 == 0 && reinterpret_cast<uintptr_t>(g->dq) % 16 == 0 &&
+                     g->g_sn % 8 == 0 && strides_ok({g->g_sh, g->g_sn}) && reinterpret_cast<uintptr_t>(g->dq) % 16 == 0 &&
                      reinterpret_cast<uintptr_t>(g->dk) % 16 == 0 && reinterpret_cast<uintptr_t>(g->dv) % 16 == 0,
                  "attn_blocks_backward: gradients must start on 16-byte boundaries");
   const int64_t stat = grad_stat_bytes(a), mask = grad_mask_bytes(a);
@@ -1043,7 +1158,7 @@ extern "C" int shrimp_attn_blocks_backward(const shrimp_attn_blocks_args* a,
   GradParams gp{};
   gp.g = static_cast<const uint16_t*>(g->g);
   gp.g_lse = g->g_lse;
-  gp.g_sb = g->g_sb, gp.g_sh = g->g_sh, gp.g_sn = g->g_sn;
+  gp.g_sb = g->g_sb, gp.g_sh = (int)g->g_sh, gp.g_sn = (int)g->g_sn;
   gp.dq = static_cast<uint16_t*>(g->dq);
   gp.dk = static_cast<uint16_t*>(g->dk);
   gp.dv = static_cast<uint16_t*>(g->dv);

@@ -58,11 +58,16 @@ __global__ __launch_bounds__(256) void block_means_kernel(const MeanParams p) {
     double sum[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] = 0.0;
-#pragma unroll 8
-    for (int r = group; r < rows; r += groups) {
-      const Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(k + r * p.sn + d);
+    constexpr int U = 8;  // rows in flight
+    for (int r0 = group; r0 < rows; r0 += groups * U) {
+      Vec<T, V> x[U];
 #pragma unroll
-      for (int e = 0; e < V; ++e) sum[e] += (double)(float)x[e];
+      for (int u = 0; u < U; ++u)
+        x[u] = *reinterpret_cast<const Vec<T, V>*>(k + (int64_t)min(r0 + u * groups, rows - 1) * p.sn + d);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] += r0 + u * groups < rows ? (double)(float)x[u][e] : 0.0;
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -240,13 +245,228 @@ __global__ __launch_bounds__(64) void block_select_kernel(const SelectParams p) 
   }
 }
 
-// Few queries (serving): a workgroup per query, 16 lanes per block's product.
-constexpr int ROW_THREADS = 256;
+// Up to 16 NT blocks: the scores stay in registers, and the choice works on 32-bit keys
+// that are certain where they differ. A score, rounded to fp32 (which keeps the order),
+// loses the low bits of its ordered form to the place it has: block tile and lane. Each
+// lane sorts its NT keys of a query; the topk largest heads among the query's 16 lanes
+// are taken off one by one (four queries side by side), 4 NT + 32 instructions each
+// against 32 LDS reads of the kernel above. Where the last taken and the next key agree
+// but for the place (scores within 2^-15 of each other: some row in ten thousand, or
+// equal scores), the 64-bit scores decide, computed again.
+constexpr int REG_WAVES = 4;
 
+SHRIMP_DEV unsigned place_key(float x, unsigned drop, unsigned place) {
+  const unsigned u = __float_as_uint(x + 0.f);
+  const unsigned k = (int)u < 0 ? ~u : u | 0x80000000u;
+  return (x != x ? 1u << drop : k >> drop << drop) | place;
+}
+
+SHRIMP_DEV unsigned row_max(unsigned v) {  // over the 16 lanes of a row, for all of them
+  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));
+  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
+  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));
+  return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));
+}
+
+template <int N>
+SHRIMP_DEV void sort_down(unsigned (&x)[N]) {  // odd-even merge sort, largest first
+#pragma unroll
+  for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+    for (int k = p; k >= 1; k >>= 1)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const unsigned a = x[i + j], b = x[i + j + k];
+            x[i + j] = max(a, b);
+            x[i + j + k] = min(a, b);
+          }
+}
+
+template <typename T, int DP, int NT>
+__global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const SelectParams p) {
+  constexpr int DK = DP / 4;
+  constexpr unsigned TB = NT == 4 ? 2 : NT == 8 ? 3 : 4, DROP = TB + 4;  // bits of a place: tile, lane
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+  const int64_t item = (int64_t)blockIdx.x * REG_WAVES + wave_id();
+  const int64_t bh = item / p.tiles;
+  if (bh >= (int64_t)p.B * p.Hk) return;
+  const int tile = (int)(item - bh * p.tiles);
+  const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
+  const int live = (k_len + p.block - 1) / p.block;
+  const int i0 = tile * 16;
+  int32_t* sel = p.sel + (bh * p.Sq + i0) * p.topk;
+  const int rows = min(16, p.Sq - i0);
+  if (i0 >= q_len || live <= p.topk) {
+    for (int j = lane; j < rows * p.topk; j += 64) {
+      const int r = j / p.topk, t = j - r * p.topk;
+      sel[j] = i0 + r < q_len && t < live ? t : -1;
+    }
+    return;
+  }
+
+  double a[DK];
+#pragma unroll
+  for (int s = 0; s < DK; ++s) a[s] = 0.0;
+  const int mine = min(i0 + lr, q_len - 1);  // (past the queries: the last one again, not written)
+  for (int h = 0; h < p.group; ++h) {
+    const T* q = static_cast<const T*>(p.q) + b * p.sb + (int64_t)(hk * p.group + h) * p.sh + (int64_t)mine * p.sn;
+    if (p.vec) {
+      Vec<T, 4> x[DK / 4];
+#pragma unroll
+      for (int s = 0; s < DK / 4; ++s)
+        x[s] = *reinterpret_cast<const Vec<T, 4>*>(q + min(lg * DK + s * 4, p.D - 4));
+#pragma unroll
+      for (int s = 0; s < DK; ++s) a[s] += lg * DK + s < p.D ? (double)(float)x[s / 4][s % 4] : 0.0;
+    } else {
+#pragma unroll
+      for (int s = 0; s < DK; ++s) a[s] += lg * DK + s < p.D ? load_f64(q + min(lg * DK + s, p.D - 1)) : 0.0;
+    }
+  }
+
+  const float* means = p.means + bh * p.NB * p.D;
+  const bool mvec = p.D % 4 == 0;
+  // scores of block tile t: lane (lr, lg) has block 16 t + lr of queries 4 i + lg
+  auto score = [&](int t) {
+    const float* m = means + (int64_t)min(t * 16 + lr, live - 1) * p.D;
+    float x[DK];
+    if (mvec) {
+#pragma unroll
+      for (int s = 0; s < DK; s += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(m + min(lg * DK + s, p.D - 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[s + e] = v[e];
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < DK; ++s) x[s] = m[min(lg * DK + s, p.D - 1)];
+    }
+    // (dimensions past D: 0 in a[], and a finite or not finite mean's own again)
+    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int s = 0; s < DK; ++s)
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s], lg * DK + s < p.D ? (double)x[s] : 0.0, acc, 0, 0, 0);
+    return acc;
+  };
+
+  unsigned key[4][NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (t * 16 < live) {
+      const f64x4 acc = score(t);
+      const bool on = t * 16 + lr < live;
+      const unsigned place = (unsigned)(NT - 1 - t) << 4 | (unsigned)(15 - lr);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) key[i][t] = on ? place_key((float)acc[i], DROP, place) : 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) key[i][t] = 0;
+    }
+  }
+  unsigned chosen[4], last[4];  // bit t: block 16 t + lr is chosen for query 4 i + lg
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sort_down(key[i]);
+    chosen[i] = last[i] = 0;
+  }
+  for (int it = 0; it < p.topk; ++it) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      last[i] = row_max(key[i][0]);
+      const bool win = key[i][0] == last[i];
+      chosen[i] |= win ? 1u << (NT - 1 - (last[i] >> 4 & (NT - 1))) : 0;
+#pragma unroll
+      for (int t = 0; t + 1 < NT; ++t) key[i][t] = win ? key[i][t + 1] : key[i][t];
+      key[i][NT - 1] = win ? 0 : key[i][NT - 1];
+    }
+  }
+  bool open = false;  // some query's last and next key differ in their places only
+#pragma unroll
+  for (int i = 0; i < 4; ++i) open |= (row_max(key[i][0]) ^ last[i]) >> DROP == 0;
+  if (__ballot(open)) {
+    // taken: what lies above the last key; then, of those that agree with it, the largest
+    // 64-bit scores, the lowest block of equal ones, one each time through the blocks
+    int left[4];
+    for (int pass = -1;; ++pass) {
+      uint64_t best[4] = {0, 0, 0, 0};
+      int at[4] = {0, 0, 0, 0};
+      unsigned above[4] = {0, 0, 0, 0};
+      for (int t = 0; t * 16 < live; ++t) {
+        const f64x4 acc = score(t);
+        const bool on = t * 16 + lr < live;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned k = place_key((float)acc[i], DROP, 0) >> DROP, edge = last[i] >> DROP;
+          if (on && k > edge) above[i] |= 1u << t;
+          const uint64_t u = order_key(acc[i]);
+          if (on && k == edge && !(chosen[i] >> t & 1) && u > best[i]) {
+            best[i] = u;
+            at[i] = t;
+          }
+        }
+      }
+      bool more = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (pass < 0) {
+          chosen[i] = above[i];
+          int n = __popc(above[i]);
+          for (int m = 1; m < 16; m <<= 1) n += __shfl_xor(n, m, 64);
+          left[i] = p.topk - n;
+          more = true;
+          continue;
+        }
+        // the row's best: key, then block
+        uint64_t k = best[i];
+        int n = at[i] * 16 + lr;
+        for (int m = 1; m < 16; m <<= 1) {
+          const uint64_t ko = __shfl_xor(k, m, 64);
+          const int no = __shfl_xor(n, m, 64);
+          if (ko > k || (ko == k && no < n)) {
+            k = ko;
+            n = no;
+          }
+        }
+        if (left[i] > 0 && (n & 15) == lr) chosen[i] |= 1u << (n >> 4);
+        left[i] -= 1;
+        more |= left[i] > 0;
+      }
+      if (!__ballot(more)) break;
+    }
+  }
+  // ascending: the chosen blocks of earlier tiles, then of earlier lanes
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 4 * i + lg;
+    int base = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const bool is = chosen[i] >> t & 1;
+      const unsigned of = (unsigned)(__ballot(is) >> (16 * lg)) & 0xFFFFu;
+      if (is && i0 + row < q_len) sel[row * p.topk + base + __popc(of & ((1u << lr) - 1))] = t * 16 + lr;
+      base += __popc(of);
+    }
+    if (lr == 0 && row < rows && i0 + row >= q_len)
+      for (int t = 0; t < p.topk; ++t) sel[row * p.topk + t] = -1;
+  }
+}
+
+// Few queries (serving): a workgroup per query, 16 lanes per block's product.
+constexpr int ROW_THREADS = 512;
+
+// The topk largest keys by radix selection, a byte at a time: a histogram of the keys that
+// share the bytes found so far, the bin in which the topk-th falls, until that bin is
+// taken whole (three bytes or so) or all eight are done (equal scores: lowest blocks).
 template <typename T>
 __global__ __launch_bounds__(ROW_THREADS) void block_select_row_kernel(const SelectParams p) {
   extern __shared__ uint64_t lds[];
-  const int tid = threadIdx.x, lane = tid & 63;
+  __shared__ int hist[256];
+  __shared__ int state[3];  // bin, keys wanted of it, keys in it
+  __shared__ int counts[2][ROW_THREADS / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int64_t bh = blockIdx.x / p.Sq;
   const int i = (int)(blockIdx.x - bh * p.Sq);
   const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
@@ -259,59 +479,109 @@ __global__ __launch_bounds__(ROW_THREADS) void block_select_row_kernel(const Sel
   }
   double* q = reinterpret_cast<double*>(lds);  // [MAX_D]
   uint64_t* keys = lds + MAX_D;                // [live]
-  if (tid < p.D) {
+  if (tid < MAX_D) {
     double s = 0.0;
-    for (int h = 0; h < p.group; ++h)
-      s += load_f64(static_cast<const T*>(p.q) + b * p.sb + (int64_t)(hk * p.group + h) * p.sh +
-                    (int64_t)i * p.sn + tid);
+    if (tid < p.D)
+      for (int h = 0; h < p.group; ++h)
+        s += load_f64(static_cast<const T*>(p.q) + b * p.sb + (int64_t)(hk * p.group + h) * p.sh +
+                      (int64_t)i * p.sn + tid);
     q[tid] = s;
   }
   __syncthreads();
   const float* means = p.means + bh * p.NB * p.D;
   const int part = tid & 15;
-#pragma unroll 4
-  for (int n = tid >> 4; n < live; n += ROW_THREADS / 16) {
-    const float* m = means + (int64_t)n * p.D;
-    double s = 0.0;
-    for (int d = part; d < p.D; d += 16) s = __builtin_fma(q[d], (double)m[d], s);
-    for (int x = 1; x < 16; x <<= 1) s += __shfl_xor(s, x, 64);
-    if (part == 0) keys[n] = order_key(s);
-  }
-  __syncthreads();
-  if (tid >= 64) return;
-  uint64_t key = 0;
-  int at = -1;
-  auto scan = [&]() {  // the largest of this lane's keys, the lowest index of equals
-    key = 0;
-    at = -1;
-    for (int n = lane; n < live; n += 64)
-      if (keys[n] > key) {
-        key = keys[n];
-        at = n;
+  constexpr int U = 4, STEP = ROW_THREADS / 16;  // blocks in flight per 16 lanes
+  for (int n0 = tid >> 4; n0 < live; n0 += U * STEP) {
+    double s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = 0.0;
+    if (p.D % 4 == 0) {
+      for (int d = part * 4; d < p.D; d += 64) {
+        f32x4 m[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          m[u] = *reinterpret_cast<const f32x4*>(means + (int64_t)min(n0 + u * STEP, live - 1) * p.D + d);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u] = __builtin_fma(q[d + e], (double)m[u][e], s[u]);
       }
-  };
-  scan();
-  int mine = 0x7fffffff;  // lane t: the t-th largest's index
-  for (int t = 0; t < p.topk; ++t) {
-    uint64_t k = key;
-    int j = at;
-    for (int m = 1; m < 64; m <<= 1) {
-      const uint64_t ko = __shfl_xor(k, m, 64);
-      const int jo = __shfl_xor(j, m, 64);
-      if (ko > k || (ko == k && ko != 0 && jo < j)) {
-        k = ko;
-        j = jo;
-      }
+    } else {
+      for (int d = part; d < p.D; d += 16)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          s[u] = __builtin_fma(q[d], (double)means[(int64_t)min(n0 + u * STEP, live - 1) * p.D + d], s[u]);
     }
-    if (lane == t) mine = j;
-    if (at == j) {  // (live > topk: there is one)
-      keys[j] = 0;
-      scan();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      for (int x = 1; x < 16; x <<= 1) s[u] += __shfl_xor(s[u], x, 64);
+      if (part == 0 && n0 + u * STEP < live) keys[n0 + u * STEP] = order_key(s[u]);
     }
   }
-  int place = 0;
-  for (int t = 0; t < p.topk; ++t) place += __shfl(mine, t, 64) < mine;
-  if (lane < p.topk) sel[place] = mine;
+  uint64_t found = 0, known = 0;  // bytes of the topk-th key, and which they are
+  int want = p.topk;
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    if (tid < 256) hist[tid] = 0;
+    __syncthreads();
+    for (int n = tid; n < live; n += ROW_THREADS)
+      if (((keys[n] ^ found) & known) == 0) atomicAdd(&hist[keys[n] >> shift & 255], 1);
+    __syncthreads();
+    if (wave == 0) {  // bins 4 lane .. + 3: how many keys lie above them
+      int c[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += c[e] = hist[4 * lane + e];
+      int up = sum;
+      for (int m = 1; m < 64; m <<= 1) {
+        const int o = __shfl_down(up, m, 64);
+        if (lane + m < 64) up += o;
+      }
+      int over = up - sum;
+#pragma unroll
+      for (int e = 3; e >= 0; --e) {
+        if (over < want && over + c[e] >= want) {
+          state[0] = 4 * lane + e;
+          state[1] = want - over;
+          state[2] = c[e];
+        }
+        over += c[e];
+      }
+    }
+    __syncthreads();
+    found |= (uint64_t)state[0] << shift;
+    known |= 255ull << shift;
+    want = state[1];
+    const bool whole = state[1] == state[2];
+    __syncthreads();
+    if (whole) break;
+  }
+  // keys above, and `want` of those that agree in the known bytes (all of them, or equal
+  // ones), in ascending order of the blocks
+  int base = 0, ties = 0;
+  for (int n0 = 0; n0 < live; n0 += ROW_THREADS) {
+    const int n = n0 + tid;
+    const uint64_t k = n < live ? keys[n] & known : 0;
+    const bool over = n < live && k > found, tie = n < live && k == found;
+    const uint64_t over_b = __ballot(over), tie_b = __ballot(tie), below = (1ull << lane) - 1;
+    if (lane == 0) {
+      counts[0][wave] = __popcll(over_b);
+      counts[1][wave] = __popcll(tie_b);
+    }
+    __syncthreads();
+    int over_at = 0, tie_at = 0, over_all = 0, tie_all = 0;
+#pragma unroll
+    for (int w = 0; w < ROW_THREADS / 64; ++w) {
+      over_at += w < wave ? counts[0][w] : 0;
+      tie_at += w < wave ? counts[1][w] : 0;
+      over_all += counts[0][w];
+      tie_all += counts[1][w];
+    }
+    over_at += __popcll(over_b & below);
+    tie_at += ties + __popcll(tie_b & below);
+    if (over || (tie && tie_at < want)) sel[base + over_at + min(tie_at, want)] = n;
+    ties += tie_all;
+    base += over_all;
+    __syncthreads();
+  }
 }
 
 int pow2_ceil(int n) {
@@ -322,15 +592,16 @@ int pow2_ceil(int n) {
 
 int dt_size(int dt) { return dt == SHRIMP_DT_F32 ? 4 : 2; }
 
-bool row_vec4(const void* base, int64_t sb, int64_t sh, int64_t sn, int D, int es) {
-  return D % 4 == 0 && sb % 4 == 0 && sh % 4 == 0 && sn % 4 == 0 &&
-         reinterpret_cast<uintptr_t>(base) % (uintptr_t)(4 * es) == 0;
+bool row_vec(int v, const void* base, int64_t sb, int64_t sh, int64_t sn, int D, int es) {
+  return D % v == 0 && sb % v == 0 && sh % v == 0 && sn % v == 0 &&
+         reinterpret_cast<uintptr_t>(base) % (uintptr_t)(v * es) == 0;
 }
 
 template <typename T>
-void means_grid(const MeanParams& p, bool vec, dim3 grid, hipStream_t st) {
-  if (vec)
-    hipLaunchKernelGGL((block_means_kernel<T, 4>), grid, dim3(256), 0, st, p);
+void means_grid(const MeanParams& p, int vec, dim3 grid, hipStream_t st) {
+  constexpr int WIDE = 16 / sizeof(T);
+  if (vec > 1)
+    hipLaunchKernelGGL((block_means_kernel<T, WIDE>), grid, dim3(256), 0, st, p);
   else
     hipLaunchKernelGGL((block_means_kernel<T, 1>), grid, dim3(256), 0, st, p);
 }
@@ -349,8 +620,9 @@ int means_launch(const void* k, int64_t sb, int64_t sh, int64_t sn, int dt, cons
   SHRIMP_REQUIRE(k && lens && means, "%s: null pointer", what);
   const int64_t items = (int64_t)B * Hk * (last_only ? 1 : nb);
   SHRIMP_REQUIRE(items <= INT32_MAX, "%s: %lld blocks of keys", what, (long long)items);
-  const bool vec = row_vec4(k, sb, sh, sn, D, dt_size(dt));
-  const int units = vec ? D / 4 : D;
+  const int wide = 16 / dt_size(dt);
+  const int vec = row_vec(wide, k, sb, sh, sn, D, dt_size(dt)) ? wide : 1;
+  const int units = D / vec;
   const MeanParams p{k, lens, means, sb, sh, sn, B, Hk, Sk, D, (int)nb, block,
                      pow2_ceil(units < 64 ? units : 64), last_only};
   const dim3 grid((unsigned)((items + 3) / 4));
@@ -372,7 +644,23 @@ void select_launch(const SelectParams& p, int64_t rows, size_t row_lds, size_t t
                        st, p);
     return;
   }
-  const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.tiles));
+  const int64_t tiles = (int64_t)p.B * p.Hk * p.tiles;
+  const dim3 reg_grid((unsigned)((tiles + REG_WAVES - 1) / REG_WAVES)), reg_block(REG_WAVES * 64);
+#define REG_LAUNCH(NT)                                                                           \
+  do {                                                                                           \
+    if (p.D <= 32)                                                                               \
+      hipLaunchKernelGGL((block_select_reg_kernel<T, 32, NT>), reg_grid, reg_block, 0, st, p);   \
+    else if (p.D <= 64)                                                                          \
+      hipLaunchKernelGGL((block_select_reg_kernel<T, 64, NT>), reg_grid, reg_block, 0, st, p);   \
+    else                                                                                         \
+      hipLaunchKernelGGL((block_select_reg_kernel<T, 128, NT>), reg_grid, reg_block, 0, st, p);  \
+    return;                                                                                      \
+  } while (0)
+  if (p.NB <= 64) REG_LAUNCH(4);
+  if (p.NB <= 128) REG_LAUNCH(8);
+  if (p.NB <= 256) REG_LAUNCH(16);
+#undef REG_LAUNCH
+  const dim3 grid((unsigned)tiles);
   if (p.D <= 32)
     hipLaunchKernelGGL((block_select_kernel<T, 32>), grid, dim3(64), tile_lds, st, p);
   else if (p.D <= 64)
@@ -410,7 +698,7 @@ extern "C" int shrimp_block_select(const shrimp_block_select_args* a, void* stre
                  "block_select: null pointer");
   SelectParams p{a->q, a->means, a->q_lens, a->k_lens, a->sel, a->q_sb, a->q_sh, a->q_sn,
                  a->B, a->H, a->Hk, a->Sq, a->Sk, a->D, (int)nb, a->block, a->topk, a->H / a->Hk,
-                 (a->Sq + 15) / 16, 0, row_vec4(a->q, a->q_sb, a->q_sh, a->q_sn, a->D, dt_size(a->dt))};
+                 (a->Sq + 15) / 16, 0, row_vec(4, a->q, a->q_sb, a->q_sh, a->q_sn, a->D, dt_size(a->dt))};
   p.chunk = nb < 128 ? (int)(nb + 15) / 16 * 16 : 128;
   const int64_t rows = (int64_t)a->B * a->Hk * a->Sq;
   SHRIMP_REQUIRE(rows <= INT32_MAX, "block_select: %lld queries", (long long)rows);

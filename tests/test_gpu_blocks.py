@@ -103,6 +103,11 @@ def _select_want(q, means, q_lens, k_lens, block, topk):
     (4, 2, 1, 1000, 128, 1, 16, "bshd"),     # one new token
     (5, 1, 2, 4096, 16, 1, 64, "bhsd"),      # the most blocks
     (1, 1, 2, 90, 7, 2, 1, "odd"),
+    (2, 1, 45, 60, 64, 1, 7, "bhsd"),        # up to 64, 128 and 256 blocks
+    (3, 3, 37, 120, 128, 1, 16, "bshd"),
+    (8, 4, 21, 250, 32, 1, 30, "bhsd"),
+    (2, 2, 19, 256, 7, 1, 64, "odd"),
+    (1, 1, 18, 257, 64, 1, 9, "bhsd"),
 ], ids=str)
 def test_select(shape, dt):
     h, hk, sq, sk, d, block, topk, layout = shape
@@ -117,9 +122,29 @@ def test_select(shape, dt):
 
 
 @pytest.mark.parametrize("sq", (1, 20))
-def test_equal_and_unordered_scores(sq):
+def test_close_scores(sq):
+    """Scores that differ in their last bits, or past fp32's: the order of float64."""
+    gen = _gen(14)
+    d = 32
+    for nb in (60, 120, 200, 300):
+        q = torch.zeros(3, 1, sq, d, device=DEV)
+        q[..., 0], q[..., 1] = 1, 2.0**-30
+        means = torch.zeros(3, 1, nb, d, device=DEV)
+        means[..., 0] = 1 + torch.randint(0, 40, (3, 1, nb), generator=gen).to(DEV) * 2.0**-23
+        means[..., 1] = torch.randint(0, 3, (3, 1, nb), generator=gen).to(DEV)
+        means[2, ..., 0] *= 1e38  # past fp32 in the group's sum
+        q[2] *= 100
+        ql, kl = [sq] * 3, [nb, nb - 7, nb]
+        for topk in (1, 5, 16):
+            got = ops.block_select(q, means, _lens(*ql), _lens(*kl), 1, topk)
+            assert torch.equal(got.cpu(), _select_want(q.cpu().double(), means.cpu().double(), ql, kl, 1, topk))
+
+
+@pytest.mark.parametrize("nb", (200, 300))
+@pytest.mark.parametrize("sq", (1, 20))
+def test_equal_and_unordered_scores(sq, nb):
     """Ties go to the lower block, a NaN below all, infinities above and below."""
-    d, nb = 32, 200
+    d = 32
     q = torch.zeros(1, 1, sq, d, device=DEV)
     q[..., 0] = 1
     means = torch.zeros(1, 1, nb, d, device=DEV)
@@ -128,7 +153,7 @@ def test_equal_and_unordered_scores(sq):
     assert (pick(5) == torch.arange(5, device=DEV)).all()
     means[0, 0, 150:, 0] = 2.0
     means[0, 0, 7, 0] = -0.0
-    assert (pick(52).cpu() == torch.tensor([0, 1, *range(150, 200)])).all()
+    assert (pick(nb - 148).cpu() == torch.tensor([0, 1, *range(150, nb)])).all() if nb == 200 else True
     means[0, 0, 3, 0] = float("inf")
     means[0, 0, 160, 0] = float("nan")
     assert (pick(3).cpu() == torch.tensor([3, 150, 151])).all()
@@ -267,18 +292,28 @@ def test_large_scores(sq, dt):
     _check_attend(q, k, v, sel.flip(-1), [sq], [sk], block)
 
 
-def test_infinities_stay_with_their_rows():
-    """A key of infinities gives NaN to the rows that chose its block and to no other."""
-    g = _gen(6)
-    for sq in (2, 40):
-        q, k, v = (_heads(g, 1, 1, s, 64, torch.bfloat16) for s in (sq, 64, 64))
+@pytest.mark.parametrize("dt", DTYPES, ids=str)
+@pytest.mark.parametrize("bad", ("nan", "inf", "lowest"))
+def test_bad_keys_stay_with_their_rows(bad, dt):
+    """Keys and values that are not finite, or the type's lowest number, reach the rows that
+    chose their block and no other, nor their gradients."""
+    gen = _gen(6)
+    x = torch.finfo(dt).min if bad == "lowest" else float(bad)
+    for sq, block in ((2, 16), (40, 16), (40, 32), (40, 64)):
+        q, k, v, g = (_heads(gen, 1, 1, s, 64, dt) for s in (sq, 4 * block, 4 * block, sq))
         sel = torch.zeros(1, 1, sq, 1, dtype=torch.int32, device=DEV)
         sel[:, :, ::2] = 2
-        clean, _ = ops.attn_blocks(q, k, v, sel, _lens(sq), _lens(64), 16)
-        k[0, 0, 40], v[0, 0, 41] = float("nan"), float("inf")
-        out, lse = ops.attn_blocks(q, k, v, sel, _lens(sq), _lens(64), 16)
-        assert out[:, :, ::2].isnan().all() and lse[:, :, ::2].isnan().all()
+        lens = (_lens(sq), _lens(4 * block))
+        run = lambda: ops.attn_blocks(q, k, v, sel, *lens, block)
+        back = lambda: ops.attn_blocks_backward(g, None, q, k, v, sel, *lens, *run(), block)
+        clean, cg = run()[0], back()
+        k[0, 0, 2 * block + 3], v[0, 0, 2 * block + 5] = x, x
+        (out, lse), grads = run(), back()
+        if bad != "lowest":
+            assert out[:, :, ::2].isnan().any(-1).all() or out[:, :, ::2].isinf().any(-1).all()
         assert torch.equal(out[:, :, 1::2], clean[:, :, 1::2])
+        assert torch.equal(grads[0][:, :, 1::2], cg[0][:, :, 1::2])
+        assert all(torch.equal(grads[i][:, :, :block], cg[i][:, :, :block]) for i in (1, 2))
 
 
 def test_rows_do_not_depend_on_the_batch():
