@@ -38,8 +38,9 @@ struct MeanParams {
   int last_only;
 };
 
-// One wave per block of keys: lanes take a row's dimensions, groups of lanes rows.
-template <typename T, int V>
+// One wave per block of keys: lanes take a row's dimensions, groups of lanes rows, U of
+// them in flight.
+template <typename T, int V, int U>
 __global__ __launch_bounds__(256) void block_means_kernel(const MeanParams p) {
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * 4 + wave_id();
@@ -58,7 +59,6 @@ __global__ __launch_bounds__(256) void block_means_kernel(const MeanParams p) {
     double sum[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] = 0.0;
-    constexpr int U = 8;  // rows in flight
     for (int r0 = group; r0 < rows; r0 += groups * U) {
       Vec<T, V> x[U];
 #pragma unroll
@@ -285,7 +285,8 @@ SHRIMP_DEV void sort_down(unsigned (&x)[N]) {  // odd-even merge sort, largest f
           }
 }
 
-template <typename T, int DP, int NT>
+// FULL: heads of exactly DP dimensions, rows readable four at a time.
+template <typename T, int DP, int NT, bool FULL>
 __global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const SelectParams p) {
   constexpr int DK = DP / 4;
   constexpr unsigned TB = NT == 4 ? 2 : NT == 8 ? 3 : 4, DROP = TB + 4;  // bits of a place: tile, lane
@@ -308,35 +309,15 @@ __global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const 
     return;
   }
 
-  double a[DK];
-#pragma unroll
-  for (int s = 0; s < DK; ++s) a[s] = 0.0;
-  const int mine = min(i0 + lr, q_len - 1);  // (past the queries: the last one again, not written)
-  for (int h = 0; h < p.group; ++h) {
-    const T* q = static_cast<const T*>(p.q) + b * p.sb + (int64_t)(hk * p.group + h) * p.sh + (int64_t)mine * p.sn;
-    if (p.vec) {
-      Vec<T, 4> x[DK / 4];
-#pragma unroll
-      for (int s = 0; s < DK / 4; ++s)
-        x[s] = *reinterpret_cast<const Vec<T, 4>*>(q + min(lg * DK + s * 4, p.D - 4));
-#pragma unroll
-      for (int s = 0; s < DK; ++s) a[s] += lg * DK + s < p.D ? (double)(float)x[s / 4][s % 4] : 0.0;
-    } else {
-#pragma unroll
-      for (int s = 0; s < DK; ++s) a[s] += lg * DK + s < p.D ? load_f64(q + min(lg * DK + s, p.D - 1)) : 0.0;
-    }
-  }
-
+  // mean rows: lane (lr, lg) supplies dimensions lg DK .. of block 16 t + lr (past the
+  // blocks the last one again, its scores not used)
   const float* means = p.means + bh * p.NB * p.D;
-  const bool mvec = p.D % 4 == 0;
-  // scores of block tile t: lane (lr, lg) has block 16 t + lr of queries 4 i + lg
-  auto score = [&](int t) {
+  auto load = [&](int t, float (&x)[DK]) {
     const float* m = means + (int64_t)min(t * 16 + lr, live - 1) * p.D;
-    float x[DK];
-    if (mvec) {
+    if (FULL || p.D % 4 == 0) {
 #pragma unroll
       for (int s = 0; s < DK; s += 4) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(m + min(lg * DK + s, p.D - 4));
+        const f32x4 v = *reinterpret_cast<const f32x4*>(m + (FULL ? lg * DK + s : min(lg * DK + s, p.D - 4)));
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[s + e] = v[e];
       }
@@ -344,19 +325,62 @@ __global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const 
 #pragma unroll
       for (int s = 0; s < DK; ++s) x[s] = m[min(lg * DK + s, p.D - 1)];
     }
-    // (dimensions past D: 0 in a[], and a finite or not finite mean's own again)
-    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+  };
+  float x[DK];
+  load(0, x);
+
+  double a[DK];
 #pragma unroll
-    for (int s = 0; s < DK; ++s)
-      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s], lg * DK + s < p.D ? (double)x[s] : 0.0, acc, 0, 0, 0);
-    return acc;
+  for (int s = 0; s < DK; ++s) a[s] = 0.0;
+  const int mine = min(i0 + lr, q_len - 1);  // (past the queries: the last one again, not written)
+  const T* q0 = static_cast<const T*>(p.q) + b * p.sb + (int64_t)(hk * p.group) * p.sh + (int64_t)mine * p.sn;
+  if (FULL || p.vec) {
+    Vec<T, 4> v[DK / 4], w[DK / 4];
+    auto row = [&](int h, Vec<T, 4> (&y)[DK / 4]) {
+#pragma unroll
+      for (int s = 0; s < DK / 4; ++s)
+        y[s] = *reinterpret_cast<const Vec<T, 4>*>(q0 + h * p.sh +
+                                                   (FULL ? lg * DK + s * 4 : min(lg * DK + s * 4, p.D - 4)));
+    };
+    row(0, v);
+    for (int h = 0; h < p.group; ++h) {  // the next head's row in flight
+      row(min(h + 1, p.group - 1), w);
+#pragma unroll
+      for (int s = 0; s < DK; ++s) {
+        const double y = (double)(float)v[s / 4][s % 4];
+        a[s] += FULL || lg * DK + s < p.D ? y : 0.0;
+      }
+#pragma unroll
+      for (int s = 0; s < DK / 4; ++s) v[s] = w[s];
+    }
+  } else {
+    for (int h = 0; h < p.group; ++h)
+#pragma unroll
+      for (int s = 0; s < DK; ++s)
+        a[s] += lg * DK + s < p.D ? load_f64(q0 + h * p.sh + min(lg * DK + s, p.D - 1)) : 0.0;
+  }
+
+  // scores of a block tile: lane (lr, lg) has block lr of queries 4 i + lg. Two chains of
+  // products, so that one need not wait for the other.
+  auto score = [&](const float (&m)[DK]) {
+    f64x4 even = {0.0, 0.0, 0.0, 0.0}, odd = even;
+#pragma unroll
+    for (int s = 0; s < DK; s += 2) {
+      const double y = FULL || lg * DK + s < p.D ? (double)m[s] : 0.0;
+      const double z = FULL || lg * DK + s + 1 < p.D ? (double)m[s + 1] : 0.0;
+      even = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s], y, even, 0, 0, 0);
+      odd = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s + 1], z, odd, 0, 0, 0);
+    }
+    return even + odd;
   };
 
   unsigned key[4][NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
+    float next[DK];
+    if (t + 1 < NT) load(t + 1, next);
     if (t * 16 < live) {
-      const f64x4 acc = score(t);
+      const f64x4 acc = score(x);
       const bool on = t * 16 + lr < live;
       const unsigned place = (unsigned)(NT - 1 - t) << 4 | (unsigned)(15 - lr);
 #pragma unroll
@@ -364,6 +388,10 @@ __global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const 
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) key[i][t] = 0;
+    }
+    if (t + 1 < NT) {
+#pragma unroll
+      for (int s = 0; s < DK; ++s) x[s] = next[s];
     }
   }
   unsigned chosen[4], last[4];  // bit t: block 16 t + lr is chosen for query 4 i + lg
@@ -395,7 +423,8 @@ __global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const 
       int at[4] = {0, 0, 0, 0};
       unsigned above[4] = {0, 0, 0, 0};
       for (int t = 0; t * 16 < live; ++t) {
-        const f64x4 acc = score(t);
+        load(t, x);
+        const f64x4 acc = score(x);
         const bool on = t * 16 + lr < live;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -600,10 +629,14 @@ bool row_vec(int v, const void* base, int64_t sb, int64_t sh, int64_t sn, int D,
 template <typename T>
 void means_grid(const MeanParams& p, int vec, dim3 grid, hipStream_t st) {
   constexpr int WIDE = 16 / sizeof(T);
-  if (vec > 1)
-    hipLaunchKernelGGL((block_means_kernel<T, WIDE>), grid, dim3(256), 0, st, p);
-  else
-    hipLaunchKernelGGL((block_means_kernel<T, 1>), grid, dim3(256), 0, st, p);
+  if (vec > 1) {
+    if (p.block * p.lanes > 4 * 64)
+      hipLaunchKernelGGL((block_means_kernel<T, WIDE, 8>), grid, dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((block_means_kernel<T, WIDE, 2>), grid, dim3(256), 0, st, p);
+  } else {
+    hipLaunchKernelGGL((block_means_kernel<T, 1, 4>), grid, dim3(256), 0, st, p);
+  }
 }
 
 int means_launch(const void* k, int64_t sb, int64_t sh, int64_t sn, int dt, const int32_t* lens,
@@ -646,19 +679,24 @@ void select_launch(const SelectParams& p, int64_t rows, size_t row_lds, size_t t
   }
   const int64_t tiles = (int64_t)p.B * p.Hk * p.tiles;
   const dim3 reg_grid((unsigned)((tiles + REG_WAVES - 1) / REG_WAVES)), reg_block(REG_WAVES * 64);
-#define REG_LAUNCH(NT)                                                                           \
-  do {                                                                                           \
-    if (p.D <= 32)                                                                               \
-      hipLaunchKernelGGL((block_select_reg_kernel<T, 32, NT>), reg_grid, reg_block, 0, st, p);   \
-    else if (p.D <= 64)                                                                          \
-      hipLaunchKernelGGL((block_select_reg_kernel<T, 64, NT>), reg_grid, reg_block, 0, st, p);   \
-    else                                                                                         \
-      hipLaunchKernelGGL((block_select_reg_kernel<T, 128, NT>), reg_grid, reg_block, 0, st, p);  \
-    return;                                                                                      \
+#define REG_LAUNCH(DP, NT)                                                                              \
+  do {                                                                                                  \
+    if (p.D == DP && p.vec)                                                                             \
+      hipLaunchKernelGGL((block_select_reg_kernel<T, DP, NT, true>), reg_grid, reg_block, 0, st, p);    \
+    else                                                                                                \
+      hipLaunchKernelGGL((block_select_reg_kernel<T, DP, NT, false>), reg_grid, reg_block, 0, st, p);   \
+    return;                                                                                             \
   } while (0)
-  if (p.NB <= 64) REG_LAUNCH(4);
-  if (p.NB <= 128) REG_LAUNCH(8);
-  if (p.NB <= 256) REG_LAUNCH(16);
+#define REG_LAUNCH_D(NT)                 \
+  do {                                   \
+    if (p.D <= 32) REG_LAUNCH(32, NT);   \
+    if (p.D <= 64) REG_LAUNCH(64, NT);   \
+    REG_LAUNCH(128, NT);                 \
+  } while (0)
+  if (p.NB <= 64) REG_LAUNCH_D(4);
+  if (p.NB <= 128) REG_LAUNCH_D(8);
+  if (p.NB <= 256) REG_LAUNCH_D(16);
+#undef REG_LAUNCH_D
 #undef REG_LAUNCH
   const dim3 grid((unsigned)tiles);
   if (p.D <= 32)
