@@ -32,12 +32,12 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int STAGE = 64;   // keys in LDS at a time
 constexpr int WINDOW = 64;  // blocks whose row masks a wave holds at a time, one per lane
 
-// Waves of a chunk workgroup and rows of a wave (one bit each in a 64-bit mask): two waves
-// per SIMD, or at D = 128 one, with the rows that a compute unit's LDS holds for them.
-template <int D>
-struct Chunk {
-  static constexpr int WAVES = D == 128 ? 4 : 8, R = D == 128 ? 48 : D == 64 ? 56 : 64;
-};
+// Rows of a wave (one bit each in a 64-bit mask): what a compute unit's LDS holds of their
+// accumulators for one workgroup of four or eight waves, at D = 32 for three.
+template <int D, int WAVES>
+constexpr int wave_rows() {
+  return D == 128 ? 48 : WAVES == 8 ? 56 : 64;
+}
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -104,7 +104,8 @@ struct BlocksParams {
   unsigned recip; // r / group = r recip >> 16 for r < 64
   int queries;  // queries per wave
   int chunks;   // waves' runs of queries per (sequence, key head)
-  int groups;   // workgroups of chunk runs
+  int waves;    // of a chunk workgroup: a run of queries each
+  int groups;   // chunk workgroups per (sequence, key head)
   int stage;    // keys per stage: 2^shared whole blocks, or an equal part of one
   int shared;
   int by_xcd;   // a key head's chunks stay on one XCD
@@ -297,15 +298,16 @@ SHRIMP_DEV float elem<_Float16>(unsigned word, int hi) {
 }
 
 // LDS of a chunk workgroup, in this order.
-template <int D>
+template <int D, int WAVES>
 struct ChunkLds {
-  static constexpr int WAVES = Chunk<D>::WAVES, R = Chunk<D>::R, RF = row_floats<D>();
+  static constexpr int R = wave_rows<D, WAVES>(), RF = row_floats<D>();
   static constexpr int RS = D + 8;                        // 16-bit elements of a staged row
   static constexpr int acc = 0;                           // [WAVES][R][RF] fp32
   static constexpr int stat = acc + WAVES * R * RF * 4;   // [WAVES][R] float2
   static constexpr int mask = stat + WAVES * R * 8;       // [WAVES][WINDOW] u64
   static constexpr int keys = mask + WAVES * WINDOW * 8;  // [2][STAGE][RS]
-  static constexpr int large = keys + 2 * STAGE * RS * 2;  // [WAVES] words
+  static constexpr int start = keys + 2 * STAGE * RS * 2;  // [STAGE] fp32: 0, -inf past the keys
+  static constexpr int large = start + STAGE * 4;          // [WAVES] words
   static constexpr int bytes = large + WAVES * 4;
   static_assert(bytes <= 160 * 1024, "a compute unit's LDS");
 };
@@ -365,12 +367,12 @@ SHRIMP_DEV uint64_t lane_u64(uint64_t v, int lane) {  // (lane: wave-uniform)
 
 // The forward, and with BACK the gradient of q (see there). MULTI: stages of two or four
 // blocks (of 32 or 16 keys).
-template <typename T, int D, bool BACK, bool MULTI>
-__global__ __launch_bounds__(Chunk<D>::WAVES * 64, 1) void attn_blocks_kernel(const BlocksParams p,
-                                                                             const GradParams gp) {
+template <typename T, int D, int WAVES, bool BACK, bool MULTI>
+__global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const BlocksParams p,
+                                                                   const GradParams gp) {
   extern __shared__ __align__(16) char lds[];
-  using L = ChunkLds<D>;
-  constexpr int WAVES = L::WAVES, R = L::R, RF = L::RF, RS = L::RS;
+  using L = ChunkLds<D, WAVES>;
+  constexpr int R = L::R, RF = L::RF, RS = L::RS;
   constexpr int EPL = D / 16, KS = D / 32, W = EPL / 2, KT = STAGE / 16;
   constexpr int LPR = D / 4;                                        // lanes of a row, four dimensions each
   constexpr int ALL = STAGE * (D / 8);                              // 16-byte pieces of a stage
@@ -381,6 +383,7 @@ __global__ __launch_bounds__(Chunk<D>::WAVES * 64, 1) void attn_blocks_kernel(co
   unsigned* mask_lds = reinterpret_cast<unsigned*>(lds + L::mask);
   uint16_t* k_lds = reinterpret_cast<uint16_t*>(lds + L::keys);
   uint16_t* v_lds = k_lds + STAGE * RS;
+  float* start_lds = reinterpret_cast<float*>(lds + L::start);
   unsigned* large_lds = reinterpret_cast<unsigned*>(lds + L::large);
   int64_t bh;
   int grp;
@@ -457,6 +460,14 @@ __global__ __launch_bounds__(Chunk<D>::WAVES * 64, 1) void attn_blocks_kernel(co
         *reinterpret_cast<u32x4*>(v_lds + row * RS + c * 8) = vr[i];
       }
     }
+    if (tid < STAGE) start_lds[tid] = tid < p.stage && key0 + tid < k_len ? 0.f : -INFINITY;
+    if constexpr (MULTI) {
+      u16x2 m = {0, 0};
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) m = max_bits(max_bits(m, kr[i]), vr[i]);
+      const uint64_t some = __ballot(m[0] >= large_bits<T>() || m[1] >= large_bits<T>());
+      if (lane == 0) large_lds[wave] = some != 0;
+    }
   };
 
   __syncthreads();
@@ -483,177 +494,202 @@ __global__ __launch_bounds__(Chunk<D>::WAVES * 64, 1) void attn_blocks_kernel(co
       at = __builtin_ctzll(todo) >> shared << shared;
       key0 = (w0 + at) * p.block;
     };
-    if (todo) {
+    if (todo == 0) {
+      __syncthreads();  // the masks are read
+      continue;
+    }
+    // to the stage behind (at, key0): of the same block, or of the next chosen one; false
+    // behind the last, which is then left as it is
+    auto advance = [&]() {
+      if (p.stage < p.block && key0 + p.stage < min((w0 + at + 1) * p.block, k_len)) {
+        key0 += p.stage;
+        return true;
+      }
+      todo &= ~(stage_bits << at);
+      if (todo == 0) return false;
       first_of();
-      request(key0);
-    }
-    while (todo) {
-      const int now_key = key0;
-      // the wave's rows that chose a block of the stage, and which of its blocks
-      uint64_t mask[MULTI ? 4 : 1];
+      return true;
+    };
+    // the wave's rows that chose a block of a stage, and which of its blocks; their list:
+    // lane j has the j-th row (the others behind them)
+    constexpr int M = MULTI ? 4 : 1;
+    auto choice = [&](int first_block, uint64_t (&mask)[M]) {
+      uint64_t rows = 0;
 #pragma unroll
-      for (int i = 0; i < (MULTI ? 4 : 1); ++i)
-        mask[i] = i < 2 || shared == 2 ? lane_u64(mine, min(at + i, WINDOW - 1)) : 0;
-      uint64_t rows = mask[0];
-      if constexpr (MULTI) rows |= mask[1] | mask[2] | mask[3];
-      int count, row_at, row = 0;
-      u32x4 qf[KS], gf[KS];
-      bool on = false;
-      auto gather = [&](int t) {  // rows t .. t + 15 of the list
-        on = t + lr < count;
-        const int listed = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at);
-        row = on ? listed : 0;
-        const int query = row_query(p, row), head = row - query * p.group;
-        load_any<D>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn, p.d, lg, qf);
-        if constexpr (BACK) load_any<D>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn, p.d, lg, gf);
-      };
-      auto list = [&](uint64_t of) {  // lane j: the j-th row (the others behind them)
-        count = __popcll(of);
-        const bool in = of >> lane & 1;
-        const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(of >> 32),
-                                                     __builtin_amdgcn_mbcnt_lo((unsigned)of, 0));
-        row_at = __builtin_amdgcn_ds_permute((in ? before : count + lane - before) << 2, lane);
-        gather(0);
-      };
-      __syncthreads();  // the stage before is done with
-      store(now_key);
-      if constexpr (MULTI) {
-        u16x2 m = {0, 0};
+      for (int i = 0; i < M; ++i) {
+        mask[i] = i < 2 || shared == 2 ? lane_u64(mine, min(first_block + i, WINDOW - 1)) : 0;
+        rows |= mask[i];
+      }
+      return rows;
+    };
+    auto list = [&](uint64_t of, int& count) {
+      count = __popcll(of);
+      const bool in = of >> lane & 1;
+      const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(of >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo((unsigned)of, 0));
+      return __builtin_amdgcn_ds_permute((in ? before : count + lane - before) << 2, lane);
+    };
+    struct Tile {  // 16 rows of a list: the lane's row and its pieces
+      int row;
+      bool on;
+      u32x4 q[KS], g[BACK ? KS : 1];
+    };
+    auto gather = [&](int row_at, int count, int t, Tile& x) {
+      x.on = t + lr < count;
+      const int listed = __builtin_amdgcn_ds_bpermute((t + lr) << 2, row_at);
+      x.row = x.on ? listed : 0;
+      const int query = row_query(p, x.row), head = x.row - query * p.group;
+      load_any<D>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn, p.d, lg, x.q);
+      if constexpr (BACK) load_any<D>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn, p.d, lg, x.g);
+    };
+
+    // Pipeline: while a stage is worked on, the next one's keys are on their way into
+    // registers, and its first rows too.
+    first_of();
+    request(key0);
+    uint64_t mask[M];
+    int count;
+    Tile tile;
+    uint64_t rows = choice(at, mask);
+    int row_at = list(rows, count);
+    gather(row_at, count, 0, tile);
+    store(key0);
+    bool more = advance();
+    request(key0);
+    __syncthreads();
+    for (;;) {
+      uint64_t next_mask[M];
+      int next_count;
+      Tile next;
+      const uint64_t next_rows = choice(at, next_mask);
+      const int next_at = list(next_rows, next_count);
+      arrived(tile.q);
+      if constexpr (BACK) arrived(tile.g);
+      gather(next_at, next_count, 0, next);
+      if (rows != 0) {
+        // The blocks of a stage share their products, where a row that did not choose one has
+        // scores of -inf and weights of 0; keys or values that are not finite, or large
+        // enough for scores that are not, would reach it all the same (0 times infinity),
+        // so such a stage goes block by block.
+        unsigned large = 0;
+        if constexpr (MULTI) {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) m = max_bits(max_bits(m, kr[i]), vr[i]);
-        const bool large = m[0] >= large_bits<T>() || m[1] >= large_bits<T>();
-        const uint64_t some = __ballot(large);
-        if (lane == 0) large_lds[wave] = some != 0;
-      }
-      // the next stage: of the same block, or of the next chosen one
-      key0 += p.stage;
-      if (p.stage >= p.block || key0 >= min((w0 + at + 1) * p.block, k_len)) {
-        todo &= ~(stage_bits << at);
-        if (todo) first_of();
-      }
-      list(rows);
-      request(key0);  // (after the last stage of a window: that one again)
-      arrived(qf);
-      if constexpr (BACK) arrived(gf);
-      __syncthreads();
-      if (rows == 0) continue;
-      // The blocks of a stage share their products, where a row that did not choose one has
-      // scores of -inf and weights of 0; keys or values that are not finite, or large
-      // enough for scores that are not, would reach it all the same (0 times infinity),
-      // so such a stage goes block by block.
-      unsigned large = 0;
-      if constexpr (MULTI) {
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) large |= large_lds[w];
-      }
-      const int passes = MULTI && __builtin_amdgcn_readfirstlane((int)large) ? per_stage : 1;
-      const int end = min(k_len, now_key + p.stage);  // keys of the stage
-      for (int pass = 0; pass < passes; ++pass) {
-        if (MULTI && passes > 1) {
-          constexpr int M = MULTI;
-          const uint64_t only = pass == 0 ? mask[0] : pass == 1 ? mask[M] : pass == 2 ? mask[2 * M] : mask[3 * M];
-          if (only == 0) continue;
-          list(only);
-          arrived(qf);
-          if constexpr (BACK) arrived(gf);
+          for (int w = 0; w < WAVES; ++w) large |= large_lds[w];
         }
-        u32x4 kf[KT][KS], vf[KT][KS];
-        Turned<D, KT> turned;
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            kf[kt][ks] = *reinterpret_cast<const u32x4*>(k_lds + (kt * 16 + lr) * RS + ks * 32 + lg * 8);
-            if constexpr (BACK)
-              vf[kt][ks] = *reinterpret_cast<const u32x4*>(v_lds + (kt * 16 + lr) * RS + ks * 32 + lg * 8);
+        const int passes = MULTI && __builtin_amdgcn_readfirstlane((int)large) ? per_stage : 1;
+        for (int pass = 0; pass < passes; ++pass) {
+          if (MULTI && passes > 1) {
+            const uint64_t only =
+                pass == 0 ? mask[0] : pass == 1 ? mask[M / 4] : pass == 2 ? mask[M / 4 * 2] : mask[M / 4 * 3];
+            if (only == 0) continue;
+            row_at = list(only, count);
+            gather(row_at, count, 0, tile);
+            arrived(tile.q);
+            if constexpr (BACK) arrived(tile.g);
           }
+          u32x4 kf[KT][KS], vf[KT][KS];
+          Turned<D, KT> turned;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            turned.raw[kt][j] = *reinterpret_cast<const Words<W>*>((BACK ? k_lds : v_lds) +
-                                                                  (kt * 16 + lg * 4 + j) * RS + lr * EPL);
-        }
-        if (MULTI && passes > 1) {
+          for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-            if (kt >> tile_shift != pass) {
+            for (int ks = 0; ks < KS; ++ks) {
+              kf[kt][ks] = *reinterpret_cast<const u32x4*>(k_lds + (kt * 16 + lr) * RS + ks * 32 + lg * 8);
+              if constexpr (BACK)
+                vf[kt][ks] = *reinterpret_cast<const u32x4*>(v_lds + (kt * 16 + lr) * RS + ks * 32 + lg * 8);
+            }
 #pragma unroll
-              for (int ks = 0; ks < KS; ++ks) {
-                kf[kt][ks] = u32x4{0, 0, 0, 0};
-                if constexpr (BACK) vf[kt][ks] = u32x4{0, 0, 0, 0};
+            for (int j = 0; j < 4; ++j)
+              turned.raw[kt][j] = *reinterpret_cast<const Words<W>*>((BACK ? k_lds : v_lds) +
+                                                                    (kt * 16 + lg * 4 + j) * RS + lr * EPL);
+          }
+          if (MULTI && passes > 1) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+              if (kt >> tile_shift != pass) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                  kf[kt][ks] = u32x4{0, 0, 0, 0};
+                  if constexpr (BACK) vf[kt][ks] = u32x4{0, 0, 0, 0};
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) turned.raw[kt][j] = (Words<W>)0u;
               }
+          }
+          for (int t = 0;;) {
+            float2 st = stat_lds[tile.row];
+            float* to = acc_lds + tile.row * RF + lg * EPL * 4;
+            f32x4 acc[EPL];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) turned.raw[kt][j] = (Words<W>)0u;
+            for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(to + e * 4);
+            f32x4 s[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[kt] = *reinterpret_cast<const f32x4*>(start_lds + kt * 16 + lg * 4);
+            if constexpr (MULTI) {
+              // bit i: the row chose block i of the stage (and the pass is for it)
+              unsigned chose = 0;
+#pragma unroll
+              for (int i = 0; i < M; ++i) chose |= (unsigned)(mask[i] >> tile.row & 1) << i;
+              if (passes > 1) chose &= 1u << pass;
+#pragma unroll
+              for (int kt = 0; kt < KT; ++kt) {
+                const bool none = !(chose >> (kt >> tile_shift) & 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[kt][i] = none ? -INFINITY : s[kt][i];
+              }
             }
-        }
-        for (int t = 0;;) {
-          float2 st = stat_lds[row];
-          float* to = acc_lds + row * RF + lg * EPL * 4;
-          f32x4 acc[EPL];
 #pragma unroll
-          for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(to + e * 4);
-          f32x4 s[KT];
-          if (now_key + STAGE <= end) {
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-          } else {
-            score_start<KT>(now_key, end, lg, s);
-          }
-          if constexpr (MULTI) {
-            // bit i: the row chose block i of the stage (and the pass is for it)
-            unsigned chose = 0;
+              for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], tile.q[ks], s[kt]);
+            u32x2 hi[KT], lo[KT];
+            if constexpr (BACK) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) chose |= (unsigned)(mask[i] >> row & 1) << i;
-            if (passes > 1) chose &= 1u << pass;
+              for (int kt = 0; kt < KT; ++kt) {
+                f32x4 dp = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-              const bool none = !(chose >> (kt >> tile_shift) & 1);
+                for (int ks = 0; ks < KS; ++ks) dp = Mma<T>::k32(vf[kt][ks], tile.g[ks], dp);
+                float w[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) s[kt][i] = none ? -INFINITY : s[kt][i];
+                for (int i = 0; i < 4; ++i)
+                  w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], p.scale2, -st.x)) * gp.scale * (dp[i] - st.y);
+                Mma<T>::split(w, hi[kt], lo[kt]);
+              }
+            } else {
+              const float alpha = soft_step<T, KT>(s, p.scale2, st.x, st.y, hi, lo);
+#pragma unroll
+              for (int e = 0; e < EPL; ++e) acc[e] *= alpha;
             }
-          }
+            weigh<T, D, KT>(turned, hi, lo, acc);
+            if (tile.on) {
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[kt] = Mma<T>::k32(kf[kt][ks], qf[ks], s[kt]);
-          u32x2 hi[KT], lo[KT];
-          if constexpr (BACK) {
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-              f32x4 dp = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int ks = 0; ks < KS; ++ks) dp = Mma<T>::k32(vf[kt][ks], gf[ks], dp);
-              float w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], p.scale2, -st.x)) * gp.scale * (dp[i] - st.y);
-              Mma<T>::split(w, hi[kt], lo[kt]);
+              for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(to + e * 4) = acc[e];
+              if (!BACK && lg == 0) stat_lds[tile.row] = st;
             }
-          } else {
-            const float alpha = soft_step<T, KT>(s, p.scale2, st.x, st.y, hi, lo);
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) acc[e] *= alpha;
+            // (the rows' state is read again by other lanes of the wave)
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            t += 16;
+            if (t >= count) break;
+            gather(row_at, count, t, tile);
+            arrived(tile.q);
+            if constexpr (BACK) arrived(tile.g);
           }
-          const int at_row = row;
-          const bool mine_on = on;
-          t += 16;
-          if (t < count) gather(t);  // (in flight under the products)
-          weigh<T, D, KT>(turned, hi, lo, acc);
-          arrived(qf);
-          if constexpr (BACK) arrived(gf);
-          if (mine_on) {
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(to + e * 4) = acc[e];
-            if (!BACK && lg == 0) stat_lds[at_row] = st;
-          }
-          // (the rows' state is read again by other lanes of the wave)
-          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-          if (t >= count) break;
         }
       }
+      __syncthreads();  // the stage is done with
+      if (!more) break;
+      store(key0);
+#pragma unroll
+      for (int i = 0; i < M; ++i) mask[i] = next_mask[i];
+      rows = next_rows;
+      row_at = next_at;
+      count = next_count;
+      tile = next;
+      more = advance();
+      request(key0);
+      __syncthreads();
     }
-    __syncthreads();  // the masks are read
   }
 
   for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
@@ -998,11 +1034,29 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
   p.d = a->d, p.block = a->block, p.topk = a->topk;
   p.group = a->H / a->Hk;
   p.recip = p.group > 0 ? (65536u + p.group - 1) / p.group : 0;
-  const int rows = a->d > 64 ? Chunk<128>::R : a->d > 32 ? Chunk<64>::R : Chunk<32>::R;
-  const int waves = a->d > 64 ? Chunk<128>::WAVES : a->d > 32 ? Chunk<64>::WAVES : Chunk<32>::WAVES;
-  p.queries = p.group > 0 ? rows / p.group : rows;
+  // Four waves of up to 64 rows, or at D = 64 eight of 56 (two per SIMD, which serves 1.4
+  // times the rows in a time, but takes 1.25 times as long for a workgroup): whichever
+  // ends first on 256 compute units. 8 heads of 8100 queries, 16 blocks of 64: 4 x 64
+  // 211 us, 8 x 56 264; the same with 64 heads 1690 and 1320.
+  const int64_t pairs = (int64_t)a->B * a->Hk;
+  auto groups = [&](int waves, int rows) {
+    const int64_t queries = p.group > 0 ? rows / p.group : rows;
+    return (a->Sq + waves * queries - 1) / (waves * queries);
+  };
+  p.waves = 4;
+  int rows = a->d > 64 ? wave_rows<128, 4>() : wave_rows<64, 4>();
+  if (a->d > 32 && a->d <= 64) {
+    const int eight = wave_rows<64, 8>();
+    const int64_t rounds8 = (pairs * groups(8, eight) + 255) / 256, rounds4 = (pairs * groups(4, rows) + 255) / 256;
+    if (5 * rounds8 < 4 * rounds4) {
+      p.waves = 8;
+      rows = eight;
+    }
+  }
+  p.groups = (int)groups(p.waves, rows);
+  // the queries dealt evenly to the waves of all groups
+  p.queries = p.groups > 0 ? (a->Sq + p.groups * p.waves - 1) / (p.groups * p.waves) : 1;
   p.chunks = (a->Sq + p.queries - 1) / p.queries;
-  p.groups = (p.chunks + waves - 1) / waves;
   // whole blocks of up to 64 keys together, or the largest equal part of a longer block
   p.stage = 16;
   p.shared = a->block == 16 ? 2 : a->block == 32 ? 1 : 0;
@@ -1014,23 +1068,29 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
         p.stage = keys;
         break;
       }
-  const int64_t pairs = (int64_t)a->B * a->Hk;
   p.by_xcd = pairs % 8 == 0 || pairs >= 64;
   p.scale2 = a->scale * LOG2E;
   return p;
 }
 
-template <typename T, int D, bool BACK>
-int launch_chunk(const BlocksParams& p, const GradParams& gp, unsigned blocks, hipStream_t st) {
-  constexpr int bytes = ChunkLds<D>::bytes;
+template <typename T, int D, int WAVES, bool BACK>
+int launch_chunk_waves(const BlocksParams& p, const GradParams& gp, unsigned blocks, hipStream_t st) {
+  constexpr int bytes = ChunkLds<D, WAVES>::bytes;
   SHRIMP_REQUIRE(bytes <= max_lds_per_block(), "attn_blocks: %d bytes of LDS, %d available", bytes,
                  max_lds_per_block());
-  const dim3 threads(Chunk<D>::WAVES * 64);
+  const dim3 grid(blocks), threads(WAVES * 64);
   if (p.shared)
-    hipLaunchKernelGGL((attn_blocks_kernel<T, D, BACK, true>), dim3(blocks), threads, bytes, st, p, gp);
+    hipLaunchKernelGGL((attn_blocks_kernel<T, D, WAVES, BACK, true>), grid, threads, bytes, st, p, gp);
   else
-    hipLaunchKernelGGL((attn_blocks_kernel<T, D, BACK, false>), dim3(blocks), threads, bytes, st, p, gp);
+    hipLaunchKernelGGL((attn_blocks_kernel<T, D, WAVES, BACK, false>), grid, threads, bytes, st, p, gp);
   return SHRIMP_OK;
+}
+
+template <typename T, int D, bool BACK>
+int launch_chunk(const BlocksParams& p, const GradParams& gp, unsigned blocks, hipStream_t st) {
+  if constexpr (D == 64)
+    if (p.waves == 8) return launch_chunk_waves<T, D, 8, BACK>(p, gp, blocks, st);
+  return launch_chunk_waves<T, D, 4, BACK>(p, gp, blocks, st);
 }
 
 template <typename T, int D, int KT>
