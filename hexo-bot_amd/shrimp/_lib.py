@@ -366,8 +366,10 @@ def launch(fn, device, what: str, *args) -> None:
 
     import torch
 
-    if device.index in (None, torch.cuda.current_device()):
-        check(fn(*args, stream_handle(device)), what)
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, stream_handle(device)), what)
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if status:
+        check(status, what)

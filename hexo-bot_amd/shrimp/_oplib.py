@@ -4,7 +4,10 @@ call and the launch.
 ``torch.library.custom_op`` costs a small call a third of its time, and its
 generated autograd some 60 us per forward and backward; an operator defined here
 has one Python kernel, and at the autograd key one ``torch.autograd.Function``,
-applied only when a gradient is wanted.
+applied only when a gradient is wanted. The public functions go past the
+dispatcher where nothing listens there (``direct``), and a Function's backward
+starts from its forward's argument struct: it runs on autograd's own thread,
+where every line of Python costs three times as much.
 """
 
 from __future__ import annotations
@@ -37,6 +40,26 @@ def define(schema: str, kernel, fake, function=None):
 
         _LIB.impl(name, autograd, "Autograd")
     return op
+
+
+def direct(*tensors) -> bool:
+    """Plain tensors, no tracing and no dispatch mode: a kernel may be called as it is."""
+
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack():
+        return False
+    for t in tensors:
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return True
+
+
+def wants_grad(*tensors) -> bool:
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t.requires_grad:
+            return True
+    return False
 
 
 def below(op, *args):

@@ -28,7 +28,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._oplib import below, define
+from ._oplib import below, define, direct, wants_grad
 
 MAX_HEAD_DIM = 128
 MAX_TOPK = 64
@@ -114,7 +114,7 @@ def block_means(k: torch.Tensor, k_lens: torch.Tensor, block: int) -> torch.Tens
     summed in float64; zero for a block without one. k (B, Hk, Sk, D) bfloat16, float16 or
     float32. Carries no gradient."""
 
-    return _block_means(k, k_lens, block)
+    return (_means_kernel if direct(k, k_lens) else _block_means)(k, k_lens, block)
 
 
 def _update_kernel(means, k, k_lens, block):
@@ -142,7 +142,7 @@ def block_means_update(means: torch.Tensor, k: torch.Tensor, k_lens: torch.Tenso
     place (block 0 for an empty sequence); the other blocks' means stay. The same bits as
     block_means."""
 
-    _block_means_update(means, k, k_lens, block)
+    (_update_kernel if direct(means, k, k_lens) else _block_means_update)(means, k, k_lens, block)
 
 
 # ---- block_select ----------------------------------------------------------------------------
@@ -189,7 +189,8 @@ def block_select(q: torch.Tensor, means: torch.Tensor, q_lens: torch.Tensor, k_l
     group's queries, ascending, then -1; -1 throughout for later rows. Scores are float64;
     equal ones go to the lower block, NaN ranks lowest. q (B, H, Sq, D); topk <= 64."""
 
-    return _block_select(q, means, q_lens, k_lens, block, topk)
+    run = _select_kernel if direct(q, means, q_lens, k_lens) else _block_select
+    return run(q, means, q_lens, k_lens, block, topk)
 
 
 # ---- attn_blocks -----------------------------------------------------------------------------
@@ -239,7 +240,9 @@ def _attn_struct(q, k, v, sel, ql, kl, out, lse, block, d):
         _DT[q.dtype], 1.0 / math.sqrt(d))
 
 
-def _attn_kernel(q, k, v, sel, q_lens, k_lens, block):
+def _attn_run(q, k, v, sel, q_lens, k_lens, block):
+    """((out, lse), argument struct, tensors it points to)"""
+
     what = "shrimp::attn_blocks"
     d = q.shape[-1]
     q, k, v, sel, ql, kl = _attn_args(what, q, k, v, sel, q_lens, k_lens, block)
@@ -247,7 +250,11 @@ def _attn_kernel(q, k, v, sel, q_lens, k_lens, block):
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
     a = _attn_struct(q, k, v, sel, ql, kl, out, lse, block, d)
     _lib.launch(_lib.load().shrimp_attn_blocks, q.device, what, ctypes.byref(a))
-    return (out if out.shape[3] == d else out[..., :d].contiguous()), lse
+    return (out if out.shape[3] == d else out[..., :d].contiguous(), lse), a, (q, k, v, sel, ql, kl, out)
+
+
+def _attn_kernel(q, k, v, sel, q_lens, k_lens, block):
+    return _attn_run(q, k, v, sel, q_lens, k_lens, block)[0]
 
 
 def _attn_fake(q, k, v, sel, q_lens, k_lens, block):
@@ -257,7 +264,12 @@ def _attn_fake(q, k, v, sel, q_lens, k_lens, block):
 class _AttnBlocks(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, sel, q_lens, k_lens, block):
-        out, lse = below(_attn_blocks, q, k, v, sel, q_lens, k_lens, block)
+        ctx.args = None
+        if direct(q, k, v, sel, q_lens, k_lens):
+            (out, lse), ctx.args, ctx.keep = _attn_run(q, k, v, sel, q_lens, k_lens, block)
+            ctx.keep = ctx.keep[:6] + ((ctx.keep[6],) if out is not ctx.keep[6] else ())
+        else:
+            out, lse = below(_attn_blocks, q, k, v, sel, q_lens, k_lens, block)
         ctx.save_for_backward(q, k, v, sel, q_lens, k_lens, out, lse)
         ctx.block = block
         ctx.set_materialize_grads(False)
@@ -268,10 +280,13 @@ class _AttnBlocks(torch.autograd.Function):
     def backward(ctx, g, g_lse):
         if g is None and g_lse is None:
             return (None,) * 7
-        out = ctx.saved_tensors[6]
+        saved = ctx.saved_tensors
         if g is None:
-            g = torch.zeros_like(out)
-        grads = _attn_blocks_backward(g, g_lse, *ctx.saved_tensors, ctx.block)
+            g = torch.zeros_like(saved[6])
+        if ctx.args is None or not direct(g):
+            grads = _attn_blocks_backward(g, g_lse, *saved, ctx.block)
+        else:
+            grads = _attn_back_run(ctx.args, g, g_lse, *ctx.keep[:2], saved[0].shape[3])
         return (*grads, None, None, None, None)
 
 
@@ -289,7 +304,33 @@ def attn_blocks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sel: torch.Te
     ones count once. Rows from q_lens[b] on, and rows without a key, are 0 and -inf. q, k
     and v bfloat16 or float16, H a multiple of Hk; block a multiple of 16."""
 
+    if direct(q, k, v, sel, q_lens, k_lens):
+        run = _AttnBlocks.apply if wants_grad(q, k, v) else _attn_kernel
+        return run(q, k, v, sel, q_lens, k_lens, block)
     return _attn_blocks(q, k, v, sel, q_lens, k_lens, block)
+
+
+def _attn_back_run(a, g, g_lse, q, k, d):
+    """Gradients from the forward's arguments; q and k as they point to them, d their head
+    dim without padding."""
+
+    g = _aligned(g, q.shape[3])
+    g_lse = None if g_lse is None else g_lse.contiguous()
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    lib = _lib.load()
+    ref = ctypes.byref(a)
+    n = lib.shrimp_attn_blocks_workspace(ref)
+    ws = torch.empty(max(n, 0), dtype=torch.uint8, device=q.device)
+    sb, sh, sn, _ = g.stride()
+    gr = _lib.AttnBlocksGrads(g.data_ptr(), sb, sh, sn, _lib.ptr(g_lse), dq.data_ptr(),
+                              dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n)
+    _lib.launch(lib.shrimp_attn_blocks_backward, q.device, "shrimp::attn_blocks_backward", ref,
+                ctypes.byref(gr))
+    if q.shape[3] == d:
+        return dq, dk, dv
+    return tuple(t[..., :d].contiguous() for t in (dq, dk, dv))
 
 
 def _attn_back_kernel(g, g_lse, q, k, v, sel, q_lens, k_lens, out, lse, block):
@@ -303,20 +344,8 @@ def _attn_back_kernel(g, g_lse, q, k, v, sel, q_lens, k_lens, out, lse, block):
         if t is not None and (t.dtype != torch.float32 or t.shape != q.shape[:3] or t.device != q.device):
             raise ValueError(f"{what}: {name} {t.dtype} {tuple(t.shape)} on {t.device}")
     q, k, v, sel, ql, kl = _attn_args(what, q, k, v, sel, q_lens, k_lens, block)
-    d8 = q.shape[3]
-    g, out = _aligned(g, d8), _aligned(out, d8).contiguous()
-    lse = lse.contiguous()
-    g_lse = None if g_lse is None else g_lse.contiguous()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-    a = _attn_struct(q, k, v, sel, ql, kl, out, lse, block, d)
-    lib = _lib.load()
-    n = lib.shrimp_attn_blocks_workspace(ctypes.byref(a))
-    ws = torch.empty(max(n, 0), dtype=torch.uint8, device=q.device)
-    gr = _lib.AttnBlocksGrads(g.data_ptr(), *g.stride()[:3], _lib.ptr(g_lse), dq.data_ptr(),
-                              dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n)
-    _lib.launch(lib.shrimp_attn_blocks_backward, q.device, what, ctypes.byref(a), ctypes.byref(gr))
-    return tuple(t if d8 == d else t[..., :d].contiguous() for t in (dq, dk, dv))
+    out, lse = _aligned(out, q.shape[3]).contiguous(), lse.contiguous()
+    return _attn_back_run(_attn_struct(q, k, v, sel, ql, kl, out, lse, block, d), g, g_lse, q, k, d)
 
 
 def _attn_back_fake(g, g_lse, q, k, v, sel, q_lens, k_lens, out, lse, block):

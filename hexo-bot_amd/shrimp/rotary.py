@@ -21,7 +21,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._oplib import below, define
+from ._oplib import below, define, direct, wants_grad
 
 MAX_AXES = 4
 MAX_HEAD_DIM = 256
@@ -63,7 +63,8 @@ def _check_heads(what: str, q: torch.Tensor, k: Optional[torch.Tensor]) -> None:
 
 def _args(what, q, k, pos, freqs, sections, interleaved, inverse, eps=0.0, q_w=None, k_w=None,
           gq=None, gk=None):
-    """(argument struct, outputs, tensors that the launch reads) of one call."""
+    """(argument struct, outputs, tensors that the launch reads) of one call; with the
+    gradients gq and gk these are checked, and no outputs made."""
 
     _check_heads(what, q, k)
     b, h, s, d = q.shape
@@ -100,24 +101,24 @@ def _args(what, q, k, pos, freqs, sections, interleaved, inverse, eps=0.0, q_w=N
         if t is not None and t.device != q.device:
             raise ValueError(f"{what}: {name} on {t.device}, q on {q.device}")
     q = _rows(q)
-    q_out = torch.empty((b, h, s, d), dtype=q.dtype, device=q.device)
-    hk, k_st, k_out = 0, (0, 0, 0), None
+    hk, k_st, q_out, k_out = 0, (0, 0, 0), None, None
     if k is not None:
         k = _rows(k)
         hk, k_st = k.shape[1], k.stride()
-        k_out = torch.empty((b, hk, s, d), dtype=q.dtype, device=q.device)
-    gq_st = gk_st = (0, 0, 0)
     if gq is not None:
         for name, g, t in (("gq", gq, q), ("gk", gk, k)):
             if g.shape != t.shape or g.dtype != t.dtype or g.device != t.device:
                 raise ValueError(f"{what}: {name} {g.dtype} {tuple(g.shape)} on {g.device} for "
                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
         gq, gk = _rows(gq), _rows(gk)
-        gq_st, gk_st = gq.stride(), gk.stride()
+    else:
+        q_out = torch.empty((b, h, s, d), dtype=q.dtype, device=q.device)
+        if k is not None:
+            k_out = torch.empty((b, hk, s, d), dtype=q.dtype, device=q.device)
     a = _lib.RopeArgs(
         q.data_ptr(), _lib.ptr(k), *q.stride()[:3], *k_st[:3],
         pos.data_ptr(), *pos.stride(), freqs.data_ptr(), _lib.ptr(q_w), _lib.ptr(k_w),
-        q_out.data_ptr(), _lib.ptr(k_out), _lib.ptr(gq), _lib.ptr(gk), *gq_st[:3], *gk_st[:3],
+        _lib.ptr(q_out), _lib.ptr(k_out), None, None, 0, 0, 0, 0, 0, 0,
         b, s, h, hk, d, axes, (ctypes.c_int32 * MAX_AXES)(*sections), _DT[q.dtype],
         _POS_DT[pos.dtype], int(freqs.dtype == torch.float64), w_dt, int(interleaved),
         int(inverse), eps,
@@ -144,11 +145,27 @@ class _RopeAxes(torch.autograd.Function):
     def forward(ctx, x, pos, freqs, sections, interleaved, inverse):
         ctx.save_for_backward(pos, freqs)
         ctx.turn = (sections, interleaved, not inverse)
-        return below(_rope_axes, x, pos, freqs, sections, interleaved, inverse)
+        ctx.args = None
+        if not direct(x, pos, freqs):
+            return below(_rope_axes, x, pos, freqs, sections, interleaved, inverse)
+        ctx.args, out, _, ctx.keep = _args("shrimp::rope_axes", x, None, pos, freqs, sections,
+                                           interleaved, inverse)
+        _lib.launch(_lib.load().shrimp_rope, x.device, "shrimp::rope_axes", ctypes.byref(ctx.args))
+        ctx.keep = ctx.keep[2:4]  # positions and frequencies as the kernel reads them
+        return out
 
     @staticmethod
     def backward(ctx, g):
-        return _rope_axes(g, *ctx.saved_tensors, *ctx.turn), None, None, None, None, None
+        pos, freqs = ctx.saved_tensors
+        if ctx.args is None or wants_grad(g) or not direct(g):
+            return rope_axes(g, pos, freqs, *ctx.turn), None, None, None, None, None
+        g = _rows(g)
+        out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        a = _lib.RopeArgs.from_buffer_copy(ctx.args)
+        a.q, a.q_out, a.inverse = g.data_ptr(), out.data_ptr(), int(ctx.turn[2])
+        a.q_sb, a.q_sh, a.q_sn, _ = g.stride()
+        _lib.launch(_lib.load().shrimp_rope, g.device, "shrimp::rope_axes", ctypes.byref(a))
+        return out, None, None, None, None, None
 
 
 _rope_axes = define(
@@ -165,6 +182,9 @@ def rope_axes(x: torch.Tensor, pos: torch.Tensor, freqs: torch.Tensor, sections:
     float32; freqs (P,) float32 or float64. Angles are formed in float64. ``inverse`` turns
     back."""
 
+    if direct(x, pos, freqs):
+        run = _RopeAxes.apply if wants_grad(x) else _rope_kernel
+        return run(x, pos, freqs, sections, interleaved, inverse)
     return _rope_axes(x, pos, freqs, sections, interleaved, inverse)
 
 
@@ -189,12 +209,24 @@ class _QkNormRope(torch.autograd.Function):
     def forward(ctx, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved):
         ctx.save_for_backward(q, k, q_weight, k_weight, pos, freqs)
         ctx.rest = (sections, eps, interleaved)
-        return below(_qk_norm_rope, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved)
+        ctx.args = None
+        if not direct(q, k, q_weight, k_weight, pos, freqs):
+            return below(_qk_norm_rope, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved)
+        what = "shrimp::qk_norm_rope"
+        ctx.args, q_out, k_out, ctx.keep = _args(what, q, k, pos, freqs, sections, interleaved, False,
+                                                 eps, q_weight, k_weight)
+        _lib.launch(_lib.load().shrimp_rope, q.device, what, ctypes.byref(ctx.args))
+        return q_out, k_out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        grads = _qk_norm_rope_backward(gq, gk, *ctx.saved_tensors, *ctx.rest)
+        saved = ctx.saved_tensors
+        if ctx.args is None or not direct(gq, gk):
+            grads = _qk_norm_rope_backward(gq, gk, *saved, *ctx.rest)
+        else:
+            a = _lib.RopeArgs.from_buffer_copy(ctx.args)
+            grads = _launch_norm_back(a, _rows(gq), _rows(gk), *saved[:4])
         return (*grads, None, None, None, None, None)
 
 
@@ -211,21 +243,39 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     and k (B, Hk, S, D), then rope_axes, in one launch with fp32 statistics. Weights (D,) of
     one type (bfloat16, float16 or float32)."""
 
+    if direct(q, k, q_weight, k_weight, pos, freqs):
+        run = _QkNormRope.apply if wants_grad(q, k, q_weight, k_weight) else _norm_kernel
+        return run(q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved)
     return _qk_norm_rope(q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved)
+
+
+def _launch_norm_back(a, gq, gk, q, k, q_weight, k_weight):
+    """Gradients from the forward's arguments ``a`` (changed) and those of its results."""
+
+    a.gq, a.gk = gq.data_ptr(), gk.data_ptr()
+    a.gq_sb, a.gq_sh, a.gq_sn, _ = gq.stride()
+    a.gk_sb, a.gk_sh, a.gk_sn, _ = gk.stride()
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    a.q_out, a.k_out = dq.data_ptr(), dk.data_ptr()
+    lib = _lib.load()
+    ref = ctypes.byref(a)
+    n = lib.shrimp_qk_norm_rope_workspace(ref)
+    ws = torch.empty(max(n, 0), dtype=torch.uint8, device=q.device)
+    dqw = torch.empty(q_weight.shape, dtype=q_weight.dtype, device=q.device)
+    dkw = torch.empty(k_weight.shape, dtype=q_weight.dtype, device=q.device)
+    _lib.launch(lib.shrimp_qk_norm_rope_backward, q.device, "shrimp::qk_norm_rope_backward", ref,
+                dqw.data_ptr(), dkw.data_ptr(), ws.data_ptr(), n)
+    return dq, dk, dqw, dkw
 
 
 def _norm_back_kernel(gq, gk, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved):
     what = "shrimp::qk_norm_rope_backward"
-    a, dq, dk, keep = _args(what, q, k, pos, freqs, sections, interleaved, False, eps, q_weight,
-                            k_weight, gq, gk)
-    lib = _lib.load()
-    n = lib.shrimp_qk_norm_rope_workspace(ctypes.byref(a))
-    ws = torch.empty(max(n, 0), dtype=torch.uint8, device=q.device)
-    dqw, dkw = q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
-    _lib.launch(lib.shrimp_qk_norm_rope_backward, q.device, what, ctypes.byref(a), dqw.data_ptr(),
-                dkw.data_ptr(), ws.data_ptr(), n)
+    a, _, _, keep = _args(what, q, k, pos, freqs, sections, interleaved, False, eps, q_weight,
+                          k_weight, gq, gk)
+    grads = _launch_norm_back(a, keep[6], keep[7], q, k, q_weight, k_weight)
     del keep
-    return dq, dk, dqw, dkw
+    return grads
 
 
 def _norm_back_fake(gq, gk, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved):
