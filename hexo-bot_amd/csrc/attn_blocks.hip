@@ -876,35 +876,56 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      for (int t = 0; t < count; t += 32) {
-        // (query, head) of entry i, -1 past the list
-        auto locate = [&](int i, int& query, int& head) {
-          const bool on = i < count;
-          const int e = on ? list[i] : 0;
-          const int r = e & 63, qi = row_query(p, r);
-          query = on ? (c0 + (e >> 6) * waves + wave) * p.queries + qi : -1;
-          head = r - qi * p.group;
-        };
-        u32x4 qf[2][KS], gf[2][KS];
-        Words<W> qt[2][4], gt[2][4];
-        float2 st[2][4];
+      // 32 rows of the list, twice: as they lie for the scores (row 16 rt + lr), and as the
+      // turned operands of the gradients (rows 16 rt + 4 lg + j). Past the list its last
+      // row again, with a weight of 0.
+      auto locate = [&](int i, int& query, int& head) {
+        const int e = list[min(i, count - 1)], r = e & 63;
+        const int qi = row_query(p, r);
+        query = (c0 + (e >> 6) * waves + wave) * p.queries + qi;
+        head = r - qi * p.group;
+      };
+      struct Rows {
+        u32x4 q[2][KS], g[2][KS];
+      };
+      auto load = [&](int t, Rows& x) {
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
           int query, head;
           locate(t + rt * 16 + lr, query, head);
-          load_row<D>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn, query >= 0, p.d, lg, qf[rt]);
-          load_row<D>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn, query >= 0, p.d, lg, gf[rt]);
+          load_any<D>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn, p.d, lg, x.q[rt]);
+          load_any<D>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn, p.d, lg, x.g[rt]);
+        }
+      };
+      // The next tile's rows in flight under the products, where the registers hold them
+      // beside 64 keys' accumulators without a wave less per SIMD (2 x 4096 queries, D = 64:
+      // 99 -> 85 us; blocks of 16 would lose a wave, D = 128 spill).
+      constexpr bool AHEAD = false;
+      Rows next;
+      if (AHEAD && count > 0) load(0, next);
+      for (int t = 0; t < count; t += 32) {
+        Rows now;
+        if constexpr (AHEAD)
+          now = next;
+        else
+          load(t, now);
+        Words<W> qt[2][4], gt[2][4];
+        float2 st[2][4];
+        const int c = min(lr * EPL, p.d - EPL);
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            locate(t + rt * 16 + lg * 4 + j, query, head);
-            const bool on = query >= 0, wide = on && lr * EPL < p.d;
-            qt[rt][j] = wide ? *reinterpret_cast<const Words<W>*>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn + lr * EPL)
-                             : (Words<W>)0u;
-            gt[rt][j] = wide ? *reinterpret_cast<const Words<W>*>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn + lr * EPL)
-                             : (Words<W>)0u;
-            st[rt][j] = on ? stat[(int64_t)head * p.Sq + query] : float2{INFINITY, 0.f};
+            const int i = t + rt * 16 + lg * 4 + j;
+            int query, head;
+            locate(i, query, head);
+            st[rt][j] = stat[(int64_t)head * p.Sq + query];
+            st[rt][j].x = i < count ? st[rt][j].x : INFINITY;
+            qt[rt][j] = *reinterpret_cast<const Words<W>*>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn + c);
+            gt[rt][j] = *reinterpret_cast<const Words<W>*>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn + c);
           }
-        }
+        if constexpr (AHEAD) load(t + 32, next);  // (behind the last tile: its last row)
+        const auto &qf = now.q, &gf = now.g;
         auto turn = [&](const Words<W> (&x)[2][4], int e) {
           const unsigned s = e & 1 ? SEL_HI : SEL_LO;
           const int w = e >> 1;
