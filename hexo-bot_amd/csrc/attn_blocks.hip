@@ -897,18 +897,9 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
           load_any<D>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn, p.d, lg, x.g[rt]);
         }
       };
-      // The next tile's rows in flight under the products, where the registers hold them
-      // beside 64 keys' accumulators without a wave less per SIMD (2 x 4096 queries, D = 64:
-      // 99 -> 85 us; blocks of 16 would lose a wave, D = 128 spill).
-      constexpr bool AHEAD = false;
-      Rows next;
-      if (AHEAD && count > 0) load(0, next);
       for (int t = 0; t < count; t += 32) {
         Rows now;
-        if constexpr (AHEAD)
-          now = next;
-        else
-          load(t, now);
+        load(t, now);
         Words<W> qt[2][4], gt[2][4];
         float2 st[2][4];
         const int c = min(lr * EPL, p.d - EPL);
@@ -924,7 +915,6 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
             qt[rt][j] = *reinterpret_cast<const Words<W>*>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn + c);
             gt[rt][j] = *reinterpret_cast<const Words<W>*>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn + c);
           }
-        if constexpr (AHEAD) load(t + 32, next);  // (behind the last tile: its last row)
         const auto &qf = now.q, &gf = now.g;
         auto turn = [&](const Words<W> (&x)[2][4], int e) {
           const unsigned s = e & 1 ? SEL_HI : SEL_LO;
@@ -1235,7 +1225,8 @@ extern "C" int shrimp_attn_blocks_backward(const shrimp_attn_blocks_args* a,
                      (g->workspace || stat + mask == 0) && reinterpret_cast<uintptr_t>(g->workspace) % 8 == 0,
                  "attn_blocks_backward: workspace of %lld bytes, %lld + %lld needed",
                  (long long)g->workspace_bytes, (long long)stat, (long long)mask);
-  const BlocksParams p = blocks_params(a, true);
+  BlocksParams p = blocks_params(a, true);
+  if (!rows) p.groups = p.chunks = 0;  // (no heads: the keys' gradients are zero)
   GradParams gp{};
   gp.g = static_cast<const uint16_t*>(g->g);
   gp.g_lse = g->g_lse;

@@ -24,6 +24,7 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 constexpr int MAX_TOPK = SHRIMP_BLOCK_MAX_TOPK;
 constexpr int MAX_D = SHRIMP_BLOCK_MAX_D;
 constexpr int MAX_BLOCKS = SHRIMP_BLOCK_MAX_BLOCKS;
+constexpr int MAX_KEYS = 1 << 30;  // (a length and a block add up within an int)
 
 template <typename T, int V>
 using Vec = T __attribute__((ext_vector_type(V)));
@@ -644,7 +645,7 @@ int means_launch(const void* k, int64_t sb, int64_t sh, int64_t sn, int dt, cons
                  "%s: element type %d", what, dt);
   SHRIMP_REQUIRE(B >= 0 && Hk >= 0 && Sk >= 0, "%s: negative size", what);
   SHRIMP_REQUIRE(D >= 1 && D <= MAX_D, "%s: head dim %d outside [1, %d]", what, D, MAX_D);
-  SHRIMP_REQUIRE(block >= 1, "%s: block of %d keys", what, block);
+  SHRIMP_REQUIRE(block >= 1 && block <= MAX_KEYS && Sk <= MAX_KEYS, "%s: block of %d keys of %d", what, block, Sk);
   const int64_t nb = ((int64_t)Sk + block - 1) / block;
   SHRIMP_REQUIRE(nb <= MAX_BLOCKS, "%s: %lld blocks, at most %d", what, (long long)nb, MAX_BLOCKS);
   if (B == 0 || Hk == 0 || nb == 0) return SHRIMP_OK;
@@ -725,17 +726,20 @@ extern "C" int shrimp_block_select(const shrimp_block_select_args* a, void* stre
   SHRIMP_REQUIRE(a->dt == SHRIMP_DT_BF16 || a->dt == SHRIMP_DT_F16 || a->dt == SHRIMP_DT_F32,
                  "block_select: element type %d", a->dt);
   SHRIMP_REQUIRE(a->B >= 0 && a->H >= 0 && a->Sq >= 0 && a->Sk >= 0, "block_select: negative size");
-  SHRIMP_REQUIRE(a->Hk >= 1 && a->H % a->Hk == 0, "block_select: %d query heads for %d key heads",
+  SHRIMP_REQUIRE(a->Hk >= 1 && a->H >= a->Hk && a->H % a->Hk == 0, "block_select: %d query heads for %d key heads",
                  a->H, a->Hk);
   SHRIMP_REQUIRE(a->D >= 1 && a->D <= MAX_D, "block_select: head dim %d outside [1, %d]", a->D, MAX_D);
-  SHRIMP_REQUIRE(a->block >= 1, "block_select: block of %d keys", a->block);
+  SHRIMP_REQUIRE(a->block >= 1 && a->block <= MAX_KEYS && a->Sk <= MAX_KEYS,
+                 "block_select: block of %d keys of %d", a->block, a->Sk);
   SHRIMP_REQUIRE(a->topk >= 1 && a->topk <= MAX_TOPK, "block_select: topk %d outside [1, %d]", a->topk,
                  MAX_TOPK);
   const int64_t nb = ((int64_t)a->Sk + a->block - 1) / a->block;
   SHRIMP_REQUIRE(nb <= MAX_BLOCKS, "block_select: %lld blocks, at most %d", (long long)nb, MAX_BLOCKS);
-  if (a->B == 0 || a->H == 0 || a->Sq == 0) return SHRIMP_OK;
+  if (a->B == 0 || a->Sq == 0) return SHRIMP_OK;
   SHRIMP_REQUIRE(a->q && a->q_lens && a->k_lens && a->sel && (a->means || nb == 0),
                  "block_select: null pointer");
+  SHRIMP_REQUIRE(reinterpret_cast<uintptr_t>(a->means) % 16 == 0,
+                 "block_select: means must start on a 16-byte boundary");
   SelectParams p{a->q, a->means, a->q_lens, a->k_lens, a->sel, a->q_sb, a->q_sh, a->q_sn,
                  a->B, a->H, a->Hk, a->Sq, a->Sk, a->D, (int)nb, a->block, a->topk, a->H / a->Hk,
                  (a->Sq + 15) / 16, 0, row_vec(4, a->q, a->q_sb, a->q_sh, a->q_sn, a->D, dt_size(a->dt))};

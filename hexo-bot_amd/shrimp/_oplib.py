@@ -67,3 +67,22 @@ def below(op, *args):
 
     with torch._C._AutoDispatchBelowAutograd():
         return op(*args)
+
+
+def marks(tensors):
+    """Where each tensor lies and how. A backward may start from its forward's argument
+    struct only if what it saved comes back as it was: a hook on saved tensors (one that
+    moves them to the host, or computes them again) returns others."""
+
+    return [(t.data_ptr(), t.stride()) for t in tensors]
+
+
+def copies(laid, given):
+    """The tensors laid out anew for a launch: a backward holds these beside what it saved."""
+
+    return tuple(a for a, b in zip(laid, given) if a is not b)
+
+
+def check_sizes(what: str, name: str, t: torch.Tensor) -> None:
+    if max(t.shape) >= 2**31:
+        raise ValueError(f"{what}: {name} {tuple(t.shape)}, sizes below 2^31 expected")

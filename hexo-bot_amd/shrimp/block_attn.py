@@ -28,12 +28,14 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._oplib import below, define, direct, wants_grad
+from ._oplib import below, check_sizes, copies, define, direct, marks, wants_grad
 
 MAX_HEAD_DIM = 128
 MAX_TOPK = 64
 MAX_BLOCKS = 4096
 MAX_GROUP = 48
+MAX_KEYS = 2**30
+MAX_ATTN_BLOCK = 2**20
 
 _DT = {
     torch.float32: _lib.DT_F32,
@@ -57,6 +59,7 @@ def _check_heads(what: str, name: str, t: torch.Tensor, types=_DT) -> None:
     if t.dtype not in types:
         raise TypeError(f"{what}: {name} is {t.dtype}, one of "
                         f"{', '.join(str(x) for x in types)} expected")
+    check_sizes(what, name, t)
     if not 1 <= t.shape[3] <= MAX_HEAD_DIM:
         raise ValueError(f"{what}: head dim {t.shape[3]} outside [1, {MAX_HEAD_DIM}]")
 
@@ -67,12 +70,14 @@ def _lens(what: str, name: str, lens: torch.Tensor, like: torch.Tensor) -> torch
                          f"({like.shape[0]},) expected")
     if lens.device != like.device:
         raise ValueError(f"{what}: {name} on {lens.device}, queries or keys on {like.device}")
+    if lens.dtype == torch.int64:
+        lens = lens.clamp(-1, MAX_KEYS)  # (2^32 + 5 is not 5)
     return lens.to(torch.int32).contiguous()
 
 
 def _blocks(what: str, keys: int, block: int) -> int:
-    if block < 1:
-        raise ValueError(f"{what}: block of {block} keys")
+    if not 1 <= block <= MAX_KEYS or keys > MAX_KEYS:
+        raise ValueError(f"{what}: block of {block} keys of {keys}, 1 to {MAX_KEYS} expected")
     nb = -(-keys // block)
     if nb > MAX_BLOCKS:
         raise ValueError(f"{what}: {keys} keys in blocks of {block} are {nb} blocks, at most "
@@ -120,12 +125,15 @@ def block_means(k: torch.Tensor, k_lens: torch.Tensor, block: int) -> torch.Tens
 def _update_kernel(means, k, k_lens, block):
     what = "shrimp::block_means_update"
     _check_heads(what, "k", k)
+    if means.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: means are written in place and carry no gradient")
     want = (k.shape[0], k.shape[1], _blocks(what, k.shape[2], block), k.shape[3])
     if (means.dtype != torch.float32 or tuple(means.shape) != want or not means.is_contiguous()
             or means.device != k.device):
         raise ValueError(f"{what}: means {means.dtype} {tuple(means.shape)} on {means.device}; "
                          f"contiguous float32 {want} on {k.device} expected")
     _launch_means(what, k, k_lens, block, means, 1)
+    torch.autograd.graph.increment_version(means)
 
 
 def _update_fake(means, k, k_lens, block):
@@ -156,18 +164,22 @@ def _select_kernel(q, means, q_lens, k_lens, block, topk):
         raise ValueError(f"{what}: means {means.dtype} {tuple(means.shape)} on {means.device}; "
                          f"float32 (B, Hk, NB, D) on {q.device} expected")
     hk, nb = means.shape[1], means.shape[2]
-    if means.shape[0] != b or means.shape[3] != d or hk < 1 or h % hk:
+    if means.shape[0] != b or means.shape[3] != d or hk < 1 or h < hk or h % hk:
         raise ValueError(f"{what}: means {tuple(means.shape)} for queries {tuple(q.shape)}")
-    if block < 1 or nb > MAX_BLOCKS:
-        raise ValueError(f"{what}: {nb} blocks of {block} keys, at most {MAX_BLOCKS}")
+    if not 1 <= block <= MAX_KEYS or nb > MAX_BLOCKS or (nb - 1) * block >= MAX_KEYS:
+        raise ValueError(f"{what}: {nb} blocks of {block} keys, at most {MAX_BLOCKS} and "
+                         f"{MAX_KEYS} keys")
     if not 1 <= topk <= MAX_TOPK:
         raise ValueError(f"{what}: topk {topk} outside [1, {MAX_TOPK}]")
     q, means = _rows(q), means.contiguous()
+    if means.data_ptr() % 16:
+        means = means.clone()
     ql, kl = _lens(what, "q_lens", q_lens, q), _lens(what, "k_lens", k_lens, q)
     sel = torch.empty((b, hk, sq, topk), dtype=torch.int32, device=q.device)
     # (of the keys only their number is known here: all blocks full)
     a = _lib.BlockSelectArgs(q.data_ptr(), *q.stride()[:3], means.data_ptr(), ql.data_ptr(),
-                             kl.data_ptr(), sel.data_ptr(), b, h, hk, sq, nb * block, d, block, topk,
+                             kl.data_ptr(), sel.data_ptr(), b, h, hk, sq, min(nb * block, MAX_KEYS), d,
+                             block, topk,
                              _DT[q.dtype])
     _lib.launch(_lib.load().shrimp_block_select, q.device, what, ctypes.byref(a))
     return sel
@@ -219,8 +231,9 @@ def _attn_args(what, q, k, v, sel, q_lens, k_lens, block):
         raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     if hk < 1 or h % hk or h // hk > MAX_GROUP:
         raise ValueError(f"{what}: {h} query heads for {hk} key heads (at most {MAX_GROUP} each)")
-    if block < 16 or block % 16:
-        raise ValueError(f"{what}: blocks of {block} keys, a multiple of 16 expected")
+    if not 16 <= block <= MAX_ATTN_BLOCK or block % 16:
+        raise ValueError(f"{what}: blocks of {block} keys, a multiple of 16 up to "
+                         f"{MAX_ATTN_BLOCK} expected")
     if (sel.dtype != torch.int32 or sel.dim() != 4 or tuple(sel.shape[:3]) != (b, hk, sq)
             or not 1 <= sel.shape[3] <= MAX_TOPK):
         raise ValueError(f"{what}: sel {sel.dtype} {tuple(sel.shape)}; int32 ({b}, {hk}, {sq}, 1 to "
@@ -266,8 +279,9 @@ class _AttnBlocks(torch.autograd.Function):
     def forward(ctx, q, k, v, sel, q_lens, k_lens, block):
         ctx.args = None
         if direct(q, k, v, sel, q_lens, k_lens):
-            (out, lse), ctx.args, ctx.keep = _attn_run(q, k, v, sel, q_lens, k_lens, block)
-            ctx.keep = ctx.keep[:6] + ((ctx.keep[6],) if out is not ctx.keep[6] else ())
+            (out, lse), ctx.args, laid = _attn_run(q, k, v, sel, q_lens, k_lens, block)
+            given = (q, k, v, sel, q_lens, k_lens, out)
+            ctx.keep, ctx.marks = copies(laid, given), marks(given + (lse,))
         else:
             out, lse = below(_attn_blocks, q, k, v, sel, q_lens, k_lens, block)
         ctx.save_for_backward(q, k, v, sel, q_lens, k_lens, out, lse)
@@ -283,10 +297,10 @@ class _AttnBlocks(torch.autograd.Function):
         saved = ctx.saved_tensors
         if g is None:
             g = torch.zeros_like(saved[6])
-        if ctx.args is None or not direct(g):
+        if ctx.args is None or not direct(g) or marks(saved) != ctx.marks:
             grads = _attn_blocks_backward(g, g_lse, *saved, ctx.block)
         else:
-            grads = _attn_back_run(ctx.args, g, g_lse, *ctx.keep[:2], saved[0].shape[3])
+            grads = _attn_back_run(ctx.args, g, g_lse, *saved[:2])
         return (*grads, None, None, None, None)
 
 
@@ -302,7 +316,8 @@ def attn_blocks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sel: torch.Te
     below k_lens[b] of the blocks that sel (B, Hk, Sq, topk) names for the row, and the log
     of the softmax's sum. Entries of sel outside the sequence's blocks name none, repeated
     ones count once. Rows from q_lens[b] on, and rows without a key, are 0 and -inf. q, k
-    and v bfloat16 or float16, H a multiple of Hk; block a multiple of 16."""
+    and v bfloat16 or float16, H a multiple of Hk; block a multiple of 16. Strides of heads
+    and rows are below 2^31 elements."""
 
     if direct(q, k, v, sel, q_lens, k_lens):
         run = _AttnBlocks.apply if wants_grad(q, k, v) else _attn_kernel
@@ -310,15 +325,15 @@ def attn_blocks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sel: torch.Te
     return _attn_blocks(q, k, v, sel, q_lens, k_lens, block)
 
 
-def _attn_back_run(a, g, g_lse, q, k, d):
-    """Gradients from the forward's arguments; q and k as they point to them, d their head
-    dim without padding."""
+def _attn_back_run(a, g, g_lse, q, k):
+    """Gradients like q and k from the forward's arguments (whose head dim may be padded)."""
 
-    g = _aligned(g, q.shape[3])
+    d = q.shape[3]
+    g = _aligned(g, a.d)
     g_lse = None if g_lse is None else g_lse.contiguous()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dq = torch.empty((*q.shape[:3], a.d), dtype=q.dtype, device=q.device)
+    dk = torch.empty((*k.shape[:3], a.d), dtype=q.dtype, device=q.device)
+    dv = torch.empty((*k.shape[:3], a.d), dtype=q.dtype, device=q.device)
     lib = _lib.load()
     ref = ctypes.byref(a)
     n = lib.shrimp_attn_blocks_workspace(ref)
@@ -328,7 +343,7 @@ def _attn_back_run(a, g, g_lse, q, k, d):
                               dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n)
     _lib.launch(lib.shrimp_attn_blocks_backward, q.device, "shrimp::attn_blocks_backward", ref,
                 ctypes.byref(gr))
-    if q.shape[3] == d:
+    if a.d == d:
         return dq, dk, dv
     return tuple(t[..., :d].contiguous() for t in (dq, dk, dv))
 
@@ -343,9 +358,9 @@ def _attn_back_kernel(g, g_lse, q, k, v, sel, q_lens, k_lens, out, lse, block):
     for name, t in (("lse", lse), ("g_lse", g_lse)):
         if t is not None and (t.dtype != torch.float32 or t.shape != q.shape[:3] or t.device != q.device):
             raise ValueError(f"{what}: {name} {t.dtype} {tuple(t.shape)} on {t.device}")
-    q, k, v, sel, ql, kl = _attn_args(what, q, k, v, sel, q_lens, k_lens, block)
-    out, lse = _aligned(out, q.shape[3]).contiguous(), lse.contiguous()
-    return _attn_back_run(_attn_struct(q, k, v, sel, ql, kl, out, lse, block, d), g, g_lse, q, k, d)
+    laid = _attn_args(what, q, k, v, sel, q_lens, k_lens, block)
+    out, lse = _aligned(out, laid[0].shape[3]).contiguous(), lse.contiguous()
+    return _attn_back_run(_attn_struct(*laid, out, lse, block, d), g, g_lse, q, k)
 
 
 def _attn_back_fake(g, g_lse, q, k, v, sel, q_lens, k_lens, out, lse, block):

@@ -21,7 +21,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._oplib import below, define, direct, wants_grad
+from ._oplib import below, check_sizes, copies, define, direct, marks, wants_grad
 
 MAX_AXES = 4
 MAX_HEAD_DIM = 256
@@ -51,6 +51,7 @@ def _check_heads(what: str, q: torch.Tensor, k: Optional[torch.Tensor]) -> None:
             raise ValueError(f"{what}: {name} must be (B, heads, S, D), got {tuple(t.shape)}")
         if t.dtype not in _DT:
             raise TypeError(f"{what}: {name} is {t.dtype}; bfloat16, float16 or float32 expected")
+        check_sizes(what, name, t)
     if not 1 <= q.shape[3] <= MAX_HEAD_DIM:
         raise ValueError(f"{what}: head dim {q.shape[3]} outside [1, {MAX_HEAD_DIM}]")
     if k is not None:
@@ -148,16 +149,17 @@ class _RopeAxes(torch.autograd.Function):
         ctx.args = None
         if not direct(x, pos, freqs):
             return below(_rope_axes, x, pos, freqs, sections, interleaved, inverse)
-        ctx.args, out, _, ctx.keep = _args("shrimp::rope_axes", x, None, pos, freqs, sections,
-                                           interleaved, inverse)
+        ctx.args, out, _, laid = _args("shrimp::rope_axes", x, None, pos, freqs, sections,
+                                       interleaved, inverse)
         _lib.launch(_lib.load().shrimp_rope, x.device, "shrimp::rope_axes", ctypes.byref(ctx.args))
-        ctx.keep = ctx.keep[2:4]  # positions and frequencies as the kernel reads them
+        ctx.keep, ctx.marks = copies(laid[2:4], (pos, freqs)), marks((pos, freqs))
         return out
 
     @staticmethod
     def backward(ctx, g):
         pos, freqs = ctx.saved_tensors
-        if ctx.args is None or wants_grad(g) or not direct(g):
+        if (ctx.args is None or wants_grad(g) or not direct(g)
+                or marks((pos, freqs)) != ctx.marks):
             return rope_axes(g, pos, freqs, *ctx.turn), None, None, None, None, None
         g = _rows(g)
         out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
@@ -213,16 +215,19 @@ class _QkNormRope(torch.autograd.Function):
         if not direct(q, k, q_weight, k_weight, pos, freqs):
             return below(_qk_norm_rope, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved)
         what = "shrimp::qk_norm_rope"
-        ctx.args, q_out, k_out, ctx.keep = _args(what, q, k, pos, freqs, sections, interleaved, False,
-                                                 eps, q_weight, k_weight)
+        ctx.args, q_out, k_out, laid = _args(what, q, k, pos, freqs, sections, interleaved, False, eps,
+                                             q_weight, k_weight)
         _lib.launch(_lib.load().shrimp_rope, q.device, what, ctypes.byref(ctx.args))
+        given = (q, k, pos, freqs, q_weight, k_weight)
+        ctx.keep = copies(laid, given)
+        ctx.marks = marks((q, k, q_weight, k_weight, pos, freqs))
         return q_out, k_out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         saved = ctx.saved_tensors
-        if ctx.args is None or not direct(gq, gk):
+        if ctx.args is None or not direct(gq, gk) or marks(saved) != ctx.marks:
             grads = _qk_norm_rope_backward(gq, gk, *saved, *ctx.rest)
         else:
             a = _lib.RopeArgs.from_buffer_copy(ctx.args)

@@ -828,7 +828,8 @@ int shrimp_qk_norm_rope_backward(const shrimp_rope_args* a, void* dw_q, void* dw
  *     H / Hk query heads that share the key head), in fp64; equal scores go to
  *     the lower block, NaN ranks lowest. q (B, H, Sq, D) of type dt.
  * D <= SHRIMP_BLOCK_MAX_D, topk <= SHRIMP_BLOCK_MAX_TOPK, NB <=
- * SHRIMP_BLOCK_MAX_BLOCKS.
+ * SHRIMP_BLOCK_MAX_BLOCKS, block and Sk <= 2^30; the means that a choice reads start
+ * on a 16-byte boundary, and it needs H >= Hk.
  * ---------------------------------------------------------------------- */
 #define SHRIMP_BLOCK_MAX_D 128
 #define SHRIMP_BLOCK_MAX_TOPK 64
@@ -857,7 +858,7 @@ int shrimp_block_select(const shrimp_block_select_args* a, void* stream);
  *   q (B, H, Sq, d), k, v (B, Hk, Sk, d) of type dt (SHRIMP_DT_BF16 / F16), Hk
  *     divides H, at most SHRIMP_BLOCK_MAX_GROUP query heads per key head; strides in elements,
  *     multiples of 8, the last one 1, rows on 16-byte boundaries; d a multiple of
- *     8 up to SHRIMP_BLOCK_MAX_D. block a multiple of 16.
+ *     8 up to SHRIMP_BLOCK_MAX_D. block a multiple of 16 up to 2^20.
  *   sel (B, Hk, Sq, topk) int32 contiguous: a row's blocks in any order; entries
  *     outside [0, ceil(k_lens[b] / block)) name none, repeated ones count once.
  *   out (B, H, Sq, d) of type dt and lse (B, H, Sq) fp32, contiguous: rows from

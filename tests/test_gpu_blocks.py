@@ -612,3 +612,102 @@ def test_refused_on_the_device():
                 dict(out=out[..., :32])):
         with pytest.raises(wrong):
             ops.attn_blocks_backward(**{**dict(g=out, g_lse=None, out=out, lse=lse), **good, **bad})
+
+
+def test_lengths_of_64_bits_and_means_off_a_boundary():
+    g = _gen(41)
+    q, k = _heads(g, 2, 4, 20, 64, torch.bfloat16), _heads(g, 2, 2, 700, 64, torch.bfloat16)
+    ql, kl = _lens(20, 17), _lens(700, 333)
+    means = ops.block_means(k, kl, 16)
+    sel = ops.block_select(q, means, ql, kl, 16, 5)
+    # 2^32 + 5 rows are all of them, not 5
+    far = torch.tensor([2**32 + 5, 333], device=DEV)
+    assert torch.equal(ops.block_means(k, far, 16), means)
+    assert torch.equal(ops.block_select(q, means, ql.long() + torch.tensor([2**32, 0], device=DEV), far, 16, 5), sel)
+    off = torch.empty(means.numel() + 1, device=DEV)[1:].view(means.shape).copy_(means)
+    assert off.data_ptr() % 16 and torch.equal(ops.block_select(q, off, ql, kl, 16, 5), sel)
+
+
+def test_update_counts_as_a_change():
+    k, kl = _heads(_gen(42), 1, 1, 40, 16, torch.float32), _lens(40)
+    means = ops.block_means(k, kl, 16)
+    w = torch.ones_like(means, requires_grad=True)
+    loss = (w * means).sum()
+    ops.block_means_update(means, k, kl, 16)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with pytest.raises(RuntimeError, match="carry no gradient"):
+        ops.block_means_update(means.requires_grad_(), k, kl, 16)
+    with torch.inference_mode():
+        held = torch.zeros(1, 1, 3, 16, device=DEV)
+        ops.block_means_update(held, k, kl, 16)
+    assert torch.equal(held[:, :, 2], means.detach()[:, :, 2])
+
+
+def test_gradients_without_heads():
+    k = _heads(_gen(43), 2, 2, 50, 64, torch.bfloat16)
+    q, sel = k.new_empty(2, 0, 40, 64), torch.zeros(2, 2, 40, 1, dtype=torch.int32, device=DEV)
+    args = q, k, k, sel, _lens(40, 40), _lens(50, 20)
+    out, lse = ops.attn_blocks(*args, 16)
+    dq, dk, dv = ops.attn_blocks_backward(out, None, *args, out, lse, 16)
+    assert out.shape == dq.shape == q.shape
+    for x in (dk, dv):
+        assert x.shape == k.shape and not x.any()
+
+
+@pytest.mark.parametrize("d", (64, 60))
+def test_saved_tensors_that_come_back_elsewhere(d):
+    """Checkpointing and saved-tensor hooks free or replace what the forward read."""
+    from torch.utils.checkpoint import checkpoint
+
+    g = _gen(44)
+    b, h, hk, n, block, topk = 2, 4, 2, 100, 16, 3
+    q0, k0 = _heads(g, b, h, n, d, torch.bfloat16), _heads(g, b, hk, n, d, torch.bfloat16)
+    sel = torch.randint(0, 7, (b, hk, n, topk), generator=g, dtype=torch.int32).to(DEV)
+    ql, kl = _lens(100, 63), _lens(100, 80)
+    w = torch.rand(d, generator=g).to(DEV)
+    pos = torch.arange(n, dtype=torch.int32, device=DEV).unsqueeze(1)
+    freqs = torch.rand(d // 2, generator=g).to(DEV)
+
+    def layer(q, k):
+        qn, kn = ops.qk_norm_rope(q, k, w, w, pos, freqs, [d // 2])
+        qn, kn = ops.rope_axes(qn, pos * 2, freqs * 1.0, [d // 2]), kn * 1.0
+        out, lse = ops.attn_blocks(qn, kn, kn + 1, sel, ql, kl, block)
+        return out * 2.0, lse.clamp(min=-30.0)
+
+    def grads(run):
+        q, k = q0.clone().requires_grad_(), k0.clone().requires_grad_()
+        out, lse = run(q, k)
+        junk = [torch.full_like(out, 5.0) for _ in range(8)]  # over what was freed
+        got = torch.autograd.grad(out.float().square().sum() + lse.sum(), [q, k])
+        del junk
+        return got
+
+    want = grads(layer)
+
+    def moved(q, k):
+        with torch.autograd.graph.save_on_cpu():
+            return layer(q, k)
+
+    for run in (moved, lambda q, k: checkpoint(layer, q, k, use_reentrant=False)):
+        for a, e in zip(grads(run), want):
+            assert torch.equal(a, e)
+
+
+def test_sizes_that_would_wrap_are_refused():
+    k, ql, kl = _heads(_gen(45), 1, 1, 100, 64, torch.bfloat16), _lens(100), _lens(100)
+    means = ops.block_means(k, kl, 16)
+    sel = ops.block_select(k, means, ql, kl, 16, 2)
+    for block in (0, -16, 2**31, 2**32 + 16):
+        for call in (lambda: ops.block_means(k, kl, block), lambda: ops.block_means_update(means, k, kl, block),
+                     lambda: ops.block_select(k, means, ql, kl, block, 2),
+                     lambda: ops.attn_blocks(k, k, k, sel, ql, kl, block)):
+            with pytest.raises(ValueError, match="block"):
+                call()
+    with pytest.raises(ValueError, match="sizes below"):
+        ops.block_means(k[:, :, :1, :1].expand(1, 2**31, 1, 1), kl, 16)
+    with pytest.raises(ValueError, match="sizes below"):
+        ops.rope_axes(k[:, :, :1, :2].expand(1, 2**31, 1, 2), torch.zeros(1, 1, device=DEV), torch.ones(1, device=DEV),
+                      [1])
+    with pytest.raises(ValueError, match="means"):
+        ops.block_select(k[:, :0], means, ql, kl, 16, 2)
