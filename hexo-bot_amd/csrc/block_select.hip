@@ -253,13 +253,20 @@ __global__ __launch_bounds__(64) void block_select_kernel(const SelectParams p) 
 // are taken off one by one (four queries side by side), 4 NT + 32 instructions each
 // against 32 LDS reads of the kernel above. Where the last taken and the next key agree
 // but for the place (scores within 2^-15 of each other: some row in ten thousand, or
-// equal scores), the 64-bit scores decide, computed again.
+// equal scores), float64 scores decide, computed again for that query by the whole wave.
+// (For all 16 of the tile by matrix products, four times through the blocks, the few
+// waves that met one ended 27 of 95 us after the others: 2 x 8000 queries, 125 blocks.)
 constexpr int REG_WAVES = 4;
 
 SHRIMP_DEV unsigned place_key(float x, unsigned drop, unsigned place) {
   const unsigned u = __float_as_uint(x + 0.f);
   const unsigned k = (int)u < 0 ? ~u : u | 0x80000000u;
   return (x != x ? 1u << drop : k >> drop << drop) | place;
+}
+
+SHRIMP_DEV uint64_t lane_u64(uint64_t v, int lane) {  // (lane: wave-uniform)
+  return (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (unsigned)__builtin_amdgcn_readlane((int)v, lane);
 }
 
 SHRIMP_DEV unsigned row_max(unsigned v) {  // over the 16 lanes of a row, for all of them
@@ -412,59 +419,71 @@ __global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const 
       key[i][NT - 1] = win ? 0 : key[i][NT - 1];
     }
   }
-  bool open = false;  // some query's last and next key differ in their places only
+  // Queries whose last and next key differ in their places only are decided by float64
+  // scores, one query at a time (bit r of `open`: query r).
+  unsigned open = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) open |= (row_max(key[i][0]) ^ last[i]) >> DROP == 0;
-  if (__ballot(open)) {
-    // taken: what lies above the last key; then, of those that agree with it, the largest
-    // 64-bit scores, the lowest block of equal ones, one each time through the blocks
-    int left[4];
-    for (int pass = -1;; ++pass) {
-      uint64_t best[4] = {0, 0, 0, 0};
-      int at[4] = {0, 0, 0, 0};
-      unsigned above[4] = {0, 0, 0, 0};
-      for (int t = 0; t * 16 < live; ++t) {
-        load(t, x);
-        const f64x4 acc = score(x);
-        const bool on = t * 16 + lr < live;
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t same = __ballot((row_max(key[i][0]) ^ last[i]) >> DROP == 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned k = place_key((float)acc[i], DROP, 0) >> DROP, edge = last[i] >> DROP;
-          if (on && k > edge) above[i] |= 1u << t;
-          const uint64_t u = order_key(acc[i]);
-          if (on && k == edge && !(chosen[i] >> t & 1) && u > best[i]) {
-            best[i] = u;
-            at[i] = t;
+    for (int g = 0; g < 4; ++g) open |= (unsigned)(same >> (16 * g) & 1) << (4 * i + g);
+  }
+  open &= (1u << min(16, q_len - i0)) - 1;
+  for (unsigned left = open; left != 0; left &= left - 1) {
+    const int r = __builtin_ctz(left);
+    constexpr int NU = NT / 4;  // blocks of a lane: 64 u + lane
+    double sum[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) sum[u] = 0.0;
+#pragma unroll 1
+    for (int part = 0; part < 4; ++part)
+#pragma unroll
+      for (int d0 = 0; d0 < DK; d0 += 4) {
+        if (d0 % 16 == 0) __builtin_amdgcn_sched_barrier(0);  // (no more loads at a time than this)
+        float m[NU][4];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          const float* row = means + (int64_t)min(u * 64 + lane, live - 1) * p.D;
+          const int d = part * DK + d0;
+          if (FULL || p.D % 4 == 0) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(row + (FULL ? d : min(d, p.D - 4)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[u][e] = v[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[u][e] = row[min(d + e, p.D - 1)];
           }
         }
-      }
-      bool more = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (pass < 0) {
-          chosen[i] = above[i];
-          int n = __popc(above[i]);
-          for (int m = 1; m < 16; m <<= 1) n += __shfl_xor(n, m, 64);
-          left[i] = p.topk - n;
-          more = true;
-          continue;
+        for (int e = 0; e < 4; ++e) {
+          const double x = __builtin_bit_cast(double, lane_u64(__builtin_bit_cast(uint64_t, a[d0 + e]), part * 16 + r));
+          const bool in = FULL || part * DK + d0 + e < p.D;
+#pragma unroll
+          for (int u = 0; u < NU; ++u) sum[u] = __builtin_fma(x, in ? (double)m[u][e] : 0.0, sum[u]);
         }
-        // the row's best: key, then block
-        uint64_t k = best[i];
-        int n = at[i] * 16 + lr;
-        for (int m = 1; m < 16; m <<= 1) {
-          const uint64_t ko = __shfl_xor(k, m, 64);
-          const int no = __shfl_xor(n, m, 64);
-          if (ko > k || (ko == k && no < n)) {
-            k = ko;
-            n = no;
-          }
-        }
-        if (left[i] > 0 && (n & 15) == lr) chosen[i] |= 1u << (n >> 4);
-        left[i] -= 1;
-        more |= left[i] > 0;
       }
-      if (!__ballot(more)) break;
+    uint64_t k[NU], edge = 0;  // the topk-th largest key, from its highest bit down
+#pragma unroll
+    for (int u = 0; u < NU; ++u) k[u] = u * 64 + lane < live ? order_key(sum[u]) : 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t next = edge | 1ull << bit;
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) n += __popcll(__ballot(k[u] >= next));
+      if (n >= p.topk) edge = next;
+    }
+    int want = p.topk, at = 0;  // how many of those equal to it: the lowest blocks
+#pragma unroll
+    for (int u = 0; u < NU; ++u) want -= __popcll(__ballot(k[u] > edge));
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const uint64_t ties = __ballot(k[u] == edge);
+      const bool is = k[u] > edge || (k[u] == edge && __popcll(ties & below) < want);
+      const uint64_t of = __ballot(is);
+      if (is) sel[r * p.topk + at + __popcll(of & below)] = u * 64 + lane;
+      at += __popcll(of);
+      want -= min(want, __popcll(ties));
     }
   }
   // ascending: the chosen blocks of earlier tiles, then of earlier lanes
@@ -476,7 +495,7 @@ __global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const 
     for (int t = 0; t < NT; ++t) {
       const bool is = chosen[i] >> t & 1;
       const unsigned of = (unsigned)(__ballot(is) >> (16 * lg)) & 0xFFFFu;
-      if (is && i0 + row < q_len) sel[row * p.topk + base + __popc(of & ((1u << lr) - 1))] = t * 16 + lr;
+      if (is && i0 + row < q_len && !(open >> row & 1)) sel[row * p.topk + base + __popc(of & ((1u << lr) - 1))] = t * 16 + lr;
       base += __popc(of);
     }
     if (lr == 0 && row < rows && i0 + row >= q_len)

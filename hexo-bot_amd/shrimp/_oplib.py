@@ -69,12 +69,18 @@ def below(op, *args):
         return op(*args)
 
 
-def marks(tensors):
-    """Where each tensor lies and how. A backward may start from its forward's argument
-    struct only if what it saved comes back as it was: a hook on saved tensors (one that
-    moves them to the host, or computes them again) returns others."""
+def hooked() -> bool:
+    """Saved tensors go through a hook (checkpointing, offloading): a backward gets others
+    than its forward had, and the forward's may be gone, so it starts anew from them."""
 
-    return [(t.data_ptr(), t.stride()) for t in tensors]
+    return torch._C._autograd._top_saved_tensors_default_hooks(True) is not None
+
+
+def places(tensors):
+    """Where tensors lie. A backward starts from its forward's argument struct only if all
+    that it saved lies where it did (a hook may also have been put on the node itself)."""
+
+    return [t.data_ptr() for t in tensors]
 
 
 def copies(laid, given):

@@ -28,7 +28,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._oplib import below, check_sizes, copies, define, direct, marks, wants_grad
+from ._oplib import below, check_sizes, copies, define, direct, hooked, places, wants_grad
 
 MAX_HEAD_DIM = 128
 MAX_TOPK = 64
@@ -278,10 +278,10 @@ class _AttnBlocks(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, sel, q_lens, k_lens, block):
         ctx.args = None
-        if direct(q, k, v, sel, q_lens, k_lens):
+        if direct(q, k, v, sel, q_lens, k_lens) and not hooked():
             (out, lse), ctx.args, laid = _attn_run(q, k, v, sel, q_lens, k_lens, block)
             given = (q, k, v, sel, q_lens, k_lens, out)
-            ctx.keep, ctx.marks = copies(laid, given), marks(given + (lse,))
+            ctx.keep, ctx.places = copies(laid, given), places(given + (lse,))
         else:
             out, lse = below(_attn_blocks, q, k, v, sel, q_lens, k_lens, block)
         ctx.save_for_backward(q, k, v, sel, q_lens, k_lens, out, lse)
@@ -297,7 +297,7 @@ class _AttnBlocks(torch.autograd.Function):
         saved = ctx.saved_tensors
         if g is None:
             g = torch.zeros_like(saved[6])
-        if ctx.args is None or not direct(g) or marks(saved) != ctx.marks:
+        if ctx.args is None or not direct(g) or places(saved) != ctx.places:
             grads = _attn_blocks_backward(g, g_lse, *saved, ctx.block)
         else:
             grads = _attn_back_run(ctx.args, g, g_lse, *saved[:2])

@@ -21,7 +21,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._oplib import below, check_sizes, copies, define, direct, marks, wants_grad
+from ._oplib import below, check_sizes, copies, define, direct, hooked, places, wants_grad
 
 MAX_AXES = 4
 MAX_HEAD_DIM = 256
@@ -147,19 +147,19 @@ class _RopeAxes(torch.autograd.Function):
         ctx.save_for_backward(pos, freqs)
         ctx.turn = (sections, interleaved, not inverse)
         ctx.args = None
-        if not direct(x, pos, freqs):
+        if not direct(x, pos, freqs) or hooked():
             return below(_rope_axes, x, pos, freqs, sections, interleaved, inverse)
         ctx.args, out, _, laid = _args("shrimp::rope_axes", x, None, pos, freqs, sections,
                                        interleaved, inverse)
         _lib.launch(_lib.load().shrimp_rope, x.device, "shrimp::rope_axes", ctypes.byref(ctx.args))
-        ctx.keep, ctx.marks = copies(laid[2:4], (pos, freqs)), marks((pos, freqs))
+        ctx.keep, ctx.places = copies(laid[2:4], (pos, freqs)), places((pos, freqs))
         return out
 
     @staticmethod
     def backward(ctx, g):
         pos, freqs = ctx.saved_tensors
         if (ctx.args is None or wants_grad(g) or not direct(g)
-                or marks((pos, freqs)) != ctx.marks):
+                or places((pos, freqs)) != ctx.places):
             return rope_axes(g, pos, freqs, *ctx.turn), None, None, None, None, None
         g = _rows(g)
         out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
@@ -212,7 +212,7 @@ class _QkNormRope(torch.autograd.Function):
         ctx.save_for_backward(q, k, q_weight, k_weight, pos, freqs)
         ctx.rest = (sections, eps, interleaved)
         ctx.args = None
-        if not direct(q, k, q_weight, k_weight, pos, freqs):
+        if not direct(q, k, q_weight, k_weight, pos, freqs) or hooked():
             return below(_qk_norm_rope, q, k, q_weight, k_weight, pos, freqs, sections, eps, interleaved)
         what = "shrimp::qk_norm_rope"
         ctx.args, q_out, k_out, laid = _args(what, q, k, pos, freqs, sections, interleaved, False, eps,
@@ -220,14 +220,14 @@ class _QkNormRope(torch.autograd.Function):
         _lib.launch(_lib.load().shrimp_rope, q.device, what, ctypes.byref(ctx.args))
         given = (q, k, pos, freqs, q_weight, k_weight)
         ctx.keep = copies(laid, given)
-        ctx.marks = marks((q, k, q_weight, k_weight, pos, freqs))
+        ctx.places = places((q, k, q_weight, k_weight, pos, freqs))
         return q_out, k_out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         saved = ctx.saved_tensors
-        if ctx.args is None or not direct(gq, gk) or marks(saved) != ctx.marks:
+        if ctx.args is None or not direct(gq, gk) or places(saved) != ctx.places:
             grads = _qk_norm_rope_backward(gq, gk, *saved, *ctx.rest)
         else:
             a = _lib.RopeArgs.from_buffer_copy(ctx.args)
