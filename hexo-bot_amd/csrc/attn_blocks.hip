@@ -6,12 +6,15 @@
 //
 // Neighbouring queries choose different blocks, so no tile of queries shares its
 // keys. The chunk kernel turns the choice round: a wave owns up to 64 rows (queries x
-// the G heads of a key head) with their output accumulators in LDS; its workgroup of four
+// the G heads of a key head) with their output accumulators in LDS; its workgroup
 // goes through the keys 64 at a time, read once from memory while the ones before are
 // worked on, and for each block a wave gathers those of its rows that chose it, 16 to
-// a matrix product. Every (row, block) pair is computed once, nothing leaves the chip
-// in between, and a row meets its blocks in ascending order alone, so its bits depend on
-// its own inputs only. Products stay transposed (S^T = K Q^T, O^T = V^T P^T): a lane's
+// a matrix product. (Where LDS holds the accumulators twice, two waves share the rows and
+// each takes half of the 64 keys; their halves are joined at the end.) Every (row, block)
+// pair is computed once, nothing leaves the chip in between, and a row meets its blocks in
+// ascending order alone, so among launches of one shape its bits depend on its own inputs
+// only (and, with blocks of 16 or 32, on whether a block beside its own holds numbers that
+// are not finite). Products stay transposed (S^T = K Q^T, O^T = V^T P^T): a lane's
 // scores are already its part of the next product's operand; V^T's operands are put
 // together from 4 keys x EPL dimensions per lane with byte permutes.
 //
@@ -32,12 +35,18 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int STAGE = 64;   // keys in LDS at a time
 constexpr int WINDOW = 64;  // blocks whose row masks a wave holds at a time, one per lane
 
-// Rows of a wave (one bit each in a 64-bit mask): what a compute unit's LDS holds of their
-// accumulators for one workgroup of four or eight waves, at D = 32 for three.
-template <int D, int WAVES>
-constexpr int wave_rows() {
-  return D == 128 ? 48 : WAVES == 8 ? 56 : 64;
-}
+// How a chunk workgroup divides: RUNS runs of up to R rows (one bit each in a 64-bit mask),
+// and TEAMS waves per run, each with its part of a stage's keys and accumulators of its own.
+// R is what a compute unit's LDS holds for one workgroup, at D = 32 for three.
+template <int RUNS_, int TEAMS_, int R_>
+struct Shape {
+  static constexpr int RUNS = RUNS_, TEAMS = TEAMS_, R = R_, WAVES = RUNS * TEAMS;
+};
+template <int D>
+struct NarrowShape : Shape<4, 1, D == 128 ? 48 : 64> {};
+template <>
+struct NarrowShape<64> : Shape<4, 2, 64> {};
+typedef Shape<8, 1, 56> WideShape;  // at D = 64
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -102,9 +111,9 @@ struct BlocksParams {
   int B, H, Hk, Sq, Sk, d, block, topk;
   int group;    // query heads per key head
   unsigned recip; // r / group = r recip >> 16 for r < 64
-  int queries;  // queries per wave
-  int chunks;   // waves' runs of queries per (sequence, key head)
-  int waves;    // of a chunk workgroup: a run of queries each
+  int queries;  // queries per run
+  int chunks;   // runs of queries per (sequence, key head)
+  bool wide;    // WideShape
   int groups;   // chunk workgroups per (sequence, key head)
   int stage;    // keys per stage: 2^shared whole blocks, or an equal part of one
   int shared;
@@ -298,14 +307,13 @@ SHRIMP_DEV float elem<_Float16>(unsigned word, int hi) {
 }
 
 // LDS of a chunk workgroup, in this order.
-template <int D, int WAVES>
+template <int D, class S>
 struct ChunkLds {
-  static constexpr int R = wave_rows<D, WAVES>(), RF = row_floats<D>();
+  static constexpr int R = S::R, RF = row_floats<D>(), WAVES = S::WAVES;
   static constexpr int RS = D + 8;                        // 16-bit elements of a staged row
-  static constexpr int acc = 0;                           // [WAVES][R][RF] fp32
-  static constexpr int stat = acc + WAVES * R * RF * 4;   // [WAVES][R] float2
-  static constexpr int mask = stat + WAVES * R * 8;       // [WAVES][WINDOW] u64
-  static constexpr int keys = mask + WAVES * WINDOW * 8;  // [2][STAGE][RS]
+  static constexpr int acc = 0;                           // [WAVES][R][RF] fp32, behind D of them float2 of the row
+  static constexpr int mask = acc + WAVES * R * RF * 4;   // [RUNS][WINDOW] u64
+  static constexpr int keys = mask + S::RUNS * WINDOW * 8;   // [2][STAGE][RS]
   static constexpr int start = keys + 2 * STAGE * RS * 2;  // [STAGE] fp32: 0, -inf past the keys
   static constexpr int large = start + STAGE * 4;          // [WAVES] words
   static constexpr int bytes = large + WAVES * 4;
@@ -367,19 +375,20 @@ SHRIMP_DEV uint64_t lane_u64(uint64_t v, int lane) {  // (lane: wave-uniform)
 
 // The forward, and with BACK the gradient of q (see there). MULTI: stages of two or four
 // blocks (of 32 or 16 keys).
-template <typename T, int D, int WAVES, bool BACK, bool MULTI>
-__global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const BlocksParams p,
-                                                                   const GradParams gp) {
+template <typename T, int D, class S, bool BACK, bool MULTI>
+__global__ __launch_bounds__(S::WAVES * 64, 1) void attn_blocks_kernel(const BlocksParams p,
+                                                                      const GradParams gp) {
   extern __shared__ __align__(16) char lds[];
-  using L = ChunkLds<D, WAVES>;
-  constexpr int R = L::R, RF = L::RF, RS = L::RS;
-  constexpr int EPL = D / 16, KS = D / 32, W = EPL / 2, KT = STAGE / 16;
+  using L = ChunkLds<D, S>;
+  constexpr int R = L::R, RF = L::RF, RS = L::RS, RUNS = S::RUNS, TEAMS = S::TEAMS, WAVES = S::WAVES;
+  constexpr int EPL = D / 16, KS = D / 32, W = EPL / 2, KT = STAGE / 16 / TEAMS;
   constexpr int LPR = D / 4;                                        // lanes of a row, four dimensions each
   constexpr int ALL = STAGE * (D / 8);                              // 16-byte pieces of a stage
   constexpr int PIECES = (ALL + WAVES * 64 - 1) / (WAVES * 64);
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4, wave = wave_id();
+  const int run = wave % RUNS, team = TEAMS > 1 ? wave / RUNS : 0;  // (the teams of a run on one SIMD)
   float* acc_lds = reinterpret_cast<float*>(lds + L::acc) + wave * R * RF;
-  float2* stat_lds = reinterpret_cast<float2*>(lds + L::stat) + wave * R;
+  auto stat_of = [&](int row) -> float2& { return *reinterpret_cast<float2*>(acc_lds + row * RF + D); };
   unsigned* mask_lds = reinterpret_cast<unsigned*>(lds + L::mask);
   uint16_t* k_lds = reinterpret_cast<uint16_t*>(lds + L::keys);
   uint16_t* v_lds = k_lds + STAGE * RS;
@@ -390,7 +399,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
   if (!place_chunk(p, p.groups, bh, grp)) return;
   const int b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
   const int q_len = min(max(p.q_lens[b], 0), p.Sq), k_len = min(max(p.k_lens[b], 0), p.Sk);
-  const int chunk = grp * WAVES + wave;
+  const int chunk = grp * RUNS + run;
   const int q0 = min(chunk * p.queries, p.Sq);
   const int queries = min(p.queries, p.Sq - q0);        // written
   const int asking = min(queries, max(q_len - q0, 0));  // with a choice
@@ -405,7 +414,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
   const int32_t* sel = p.sel + (bh * p.Sq + q0) * p.topk;
   const int64_t out0 = ((int64_t)b * p.H + hk * p.group) * p.Sq + q0;  // of row 0
 
-  for (int i = lane; i < R * RF; i += 64) acc_lds[i] = 0.f;
+  for (int i = lane; i < R * D; i += 64) acc_lds[i / D * RF + i % D] = 0.f;
   if constexpr (BACK) {
     for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
       const int r = r0 + lane / LPR, c = lane % LPR;
@@ -424,12 +433,12 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
         if (gp.g_lse) delta -= gp.g_lse[o];
         const float lse = p.lse[o];
         const float2 st = {lse == -INFINITY ? INFINITY : lse * LOG2E, delta};
-        stat_lds[r] = st;
-        gp.stat[o] = st;
+        stat_of(r) = st;
+        if (team == 0) gp.stat[o] = st;
       }
     }
   } else {
-    if (lane < R) stat_lds[lane] = float2{-INFINITY, 0.f};  // maximum, sum
+    if (lane < R) stat_of(lane) = float2{-INFINITY, 0.f};  // maximum, sum
   }
 
   // Stage of keys from key0: requested into registers, put into LDS by `store`. Requests go
@@ -473,20 +482,22 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
   __syncthreads();
   const int shared = MULTI ? p.shared : 0, per_stage = 1 << shared;  // blocks of a stage
   const int tile_shift = 2 - shared;                                   // of its 16-key tiles per block
-  static_assert(KT == 4, "a stage of four tiles");
+  const int per_team = max(per_stage / TEAMS, 1);
+  const int block0 = per_stage > 1 ? team * per_team : 0;  // the team's first block of a stage
+  static_assert(KT * TEAMS == 4, "a stage of four tiles");
   for (int w0 = 0; w0 < live; w0 += WINDOW) {
-    fill_masks(p, sel, asking, w0, mask_lds + wave * 2 * WINDOW, lane);
+    if (team == 0) fill_masks(p, sel, asking, w0, mask_lds + run * 2 * WINDOW, lane);
     __syncthreads();
     const bool here = w0 + lane < live;
     uint64_t any = 0, mine = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
+    for (int w = 0; w < RUNS; ++w) {
       const uint64_t m = here ? reinterpret_cast<const uint64_t*>(mask_lds)[w * WINDOW + lane] : 0;
       any |= m;
-      if (w == wave) mine = m;
+      if (w == run) mine = m;
     }
     if constexpr (BACK)
-      if (here && chunk < p.chunks) gp.masks[(bh * gp.nb + w0 + lane) * p.chunks + chunk] = mine;
+      if (here && team == 0 && chunk < p.chunks) gp.masks[(bh * gp.nb + w0 + lane) * p.chunks + chunk] = mine;
     uint64_t todo = __ballot(any != 0);
     const uint64_t stage_bits = (1u << per_stage) - 1;
     int at = 0, key0 = 0;  // first block (of the window) and first key of a stage with chosen blocks
@@ -510,17 +521,18 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
       first_of();
       return true;
     };
-    // the wave's rows that chose a block of a stage, and which of its blocks; their list:
-    // lane j has the j-th row (the others behind them)
-    constexpr int M = MULTI ? 4 : 1;
-    auto choice = [&](int first_block, uint64_t (&mask)[M]) {
+    // the wave's rows that chose one of its blocks of the stage, and which of them; their
+    // list: lane j has the j-th row (the others behind them)
+    constexpr int M = MULTI ? 4 / TEAMS : 1;
+    auto choice = [&](uint64_t (&mask)[M]) {
       uint64_t rows = 0;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        mask[i] = i < 2 || shared == 2 ? lane_u64(mine, min(first_block + i, WINDOW - 1)) : 0;
+        mask[i] = i < per_team ? lane_u64(mine, min(at + block0 + i, WINDOW - 1)) : 0;
         rows |= mask[i];
       }
-      return rows;
+      const int from = team * KT * 16;  // its first key of the stage
+      return from < p.stage && key0 + from < k_len ? rows : 0;
     };
     auto list = [&](uint64_t of, int& count) {
       count = __popcll(of);
@@ -550,7 +562,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
     uint64_t mask[M];
     int count;
     Tile tile;
-    uint64_t rows = choice(at, mask);
+    uint64_t rows = choice(mask);
     int row_at = list(rows, count);
     gather(row_at, count, 0, tile);
     store(key0);
@@ -561,7 +573,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
       uint64_t next_mask[M];
       int next_count;
       Tile next;
-      const uint64_t next_rows = choice(at, next_mask);
+      const uint64_t next_rows = choice(next_mask);
       const int next_at = list(next_rows, next_count);
       arrived(tile.q);
       if constexpr (BACK) arrived(tile.g);
@@ -576,11 +588,12 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
 #pragma unroll
           for (int w = 0; w < WAVES; ++w) large |= large_lds[w];
         }
-        const int passes = MULTI && __builtin_amdgcn_readfirstlane((int)large) ? per_stage : 1;
+        const int passes = MULTI && __builtin_amdgcn_readfirstlane((int)large) ? per_team : 1;
         for (int pass = 0; pass < passes; ++pass) {
           if (MULTI && passes > 1) {
-            const uint64_t only =
-                pass == 0 ? mask[0] : pass == 1 ? mask[M / 4] : pass == 2 ? mask[M / 4 * 2] : mask[M / 4 * 3];
+            uint64_t only = mask[0];
+#pragma unroll
+            for (int i = 1; i < M; ++i) only = pass == i ? mask[i] : only;
             if (only == 0) continue;
             row_at = list(only, count);
             gather(row_at, count, 0, tile);
@@ -593,14 +606,14 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
           for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-              kf[kt][ks] = *reinterpret_cast<const u32x4*>(k_lds + (kt * 16 + lr) * RS + ks * 32 + lg * 8);
-              if constexpr (BACK)
-                vf[kt][ks] = *reinterpret_cast<const u32x4*>(v_lds + (kt * 16 + lr) * RS + ks * 32 + lg * 8);
+              const int from = ((team * KT + kt) * 16 + lr) * RS + ks * 32 + lg * 8;
+              kf[kt][ks] = *reinterpret_cast<const u32x4*>(k_lds + from);
+              if constexpr (BACK) vf[kt][ks] = *reinterpret_cast<const u32x4*>(v_lds + from);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               turned.raw[kt][j] = *reinterpret_cast<const Words<W>*>((BACK ? k_lds : v_lds) +
-                                                                    (kt * 16 + lg * 4 + j) * RS + lr * EPL);
+                                                                    ((team * KT + kt) * 16 + lg * 4 + j) * RS + lr * EPL);
           }
           if (MULTI && passes > 1) {
 #pragma unroll
@@ -616,14 +629,14 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
               }
           }
           for (int t = 0;;) {
-            float2 st = stat_lds[tile.row];
+            float2 st = stat_of(tile.row);
             float* to = acc_lds + tile.row * RF + lg * EPL * 4;
             f32x4 acc[EPL];
 #pragma unroll
             for (int e = 0; e < EPL; ++e) acc[e] = *reinterpret_cast<const f32x4*>(to + e * 4);
             f32x4 s[KT];
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) s[kt] = *reinterpret_cast<const f32x4*>(start_lds + kt * 16 + lg * 4);
+            for (int kt = 0; kt < KT; ++kt) s[kt] = *reinterpret_cast<const f32x4*>(start_lds + (team * KT + kt) * 16 + lg * 4);
             if constexpr (MULTI) {
               // bit i: the row chose block i of the stage (and the pass is for it)
               unsigned chose = 0;
@@ -663,7 +676,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
             if (tile.on) {
 #pragma unroll
               for (int e = 0; e < EPL; ++e) *reinterpret_cast<f32x4*>(to + e * 4) = acc[e];
-              if (!BACK && lg == 0) stat_lds[tile.row] = st;
+              if (!BACK && lg == 0) stat_of(tile.row) = st;
             }
             // (the rows' state is read again by other lanes of the wave)
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -692,20 +705,36 @@ __global__ __launch_bounds__(WAVES * 64, 1) void attn_blocks_kernel(const Blocks
     }
   }
 
-  for (int r0 = 0; r0 < queries * p.group; r0 += 64 / LPR) {
+  // The teams' rows joined, around the larger maximum, in team order; each team writes its
+  // part of them. (Behind the last window's barrier; without a window all is as it began.)
+  const float* acc0 = reinterpret_cast<const float*>(lds + L::acc) + run * R * RF;
+  const float* acc1 = acc0 + (TEAMS - 1) * RUNS * R * RF;
+  for (int r0 = team * (64 / LPR); r0 < queries * p.group; r0 += TEAMS * (64 / LPR)) {
     const int r = r0 + lane / LPR, c = lane % LPR;
     if (r >= queries * p.group) continue;
     const int query = row_query(p, r), head = r - query * p.group;
     const int64_t o = out0 + (int64_t)head * p.Sq + query;
-    const float2 st = stat_lds[r];
-    const float inv = BACK ? 1.f : st.y == 0.f ? 0.f : 1.f / st.y;
+    float2 st = *reinterpret_cast<const float2*>(acc0 + r * RF + D);
+    float mul0 = 1.f, mul1 = 1.f;
+    if constexpr (!BACK) {
+      if constexpr (TEAMS > 1) {
+        const float2 so = *reinterpret_cast<const float2*>(acc1 + r * RF + D);
+        const float top = fmaxf(st.x, so.x), off = top == -INFINITY ? 0.f : top;
+        mul0 = __builtin_amdgcn_exp2f(st.x - off);
+        mul1 = __builtin_amdgcn_exp2f(so.x - off);
+        st = float2{top, fmaf(st.y, mul0, so.y * mul1)};
+      }
+      const float inv = st.y == 0.f ? 0.f : 1.f / st.y;
+      mul0 *= inv, mul1 *= inv;
+    }
     if (c * 4 < p.d) {
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         // dimension 4 c + e is element dim % EPL of the product's row dim / EPL = 4 lg + i
         const int dim = c * 4 + e, rr = dim / EPL, ee = dim % EPL;
-        x[e] = acc_lds[r * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3)] * inv;
+        const int from = r * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3);
+        x[e] = TEAMS > 1 ? fmaf(acc0[from], mul0, acc1[from] * mul1) : acc0[from] * mul0;
       }
       *reinterpret_cast<u32x2*>((BACK ? gp.dq : p.out) + o * p.d + c * 4) =
           u32x2{Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3])};
@@ -1045,28 +1074,25 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
   p.d = a->d, p.block = a->block, p.topk = a->topk;
   p.group = a->H / a->Hk;
   p.recip = p.group > 0 ? (65536u + p.group - 1) / p.group : 0;
-  // Four waves of up to 64 rows, or at D = 64 eight of 56 (two per SIMD, which serves 1.4
-  // times the rows in a time, but takes 1.25 times as long for a workgroup): whichever
-  // ends first on 256 compute units. 8 heads of 8100 queries, 16 blocks of 64: 4 x 64
-  // 211 us, 8 x 56 264; the same with 64 heads 1690 and 1320.
   const int64_t pairs = (int64_t)a->B * a->Hk;
-  auto groups = [&](int waves, int rows) {
-    const int64_t queries = p.group > 0 ? rows / p.group : rows;
-    return (a->Sq + waves * queries - 1) / (waves * queries);
+  // At D = 64 the wide shape serves 1.75 times the rows at a time, but takes 1.37 times as
+  // long for a workgroup: whichever ends first on 256 compute units. 8 heads of 8100 queries,
+  // 16 blocks of 64: narrow 188 us, wide 261; the same with 64 heads 1516 and 1306.
+  auto groups = [&](int runs, int rows) {
+    const int64_t most = (int64_t)runs * (p.group > 0 ? rows / p.group : rows);
+    return (a->Sq + most - 1) / most;
   };
-  p.waves = 4;
-  int rows = a->d > 64 ? wave_rows<128, 4>() : wave_rows<64, 4>();
+  int runs = 4, rows = a->d > 64 ? NarrowShape<128>::R : NarrowShape<64>::R;
   if (a->d > 32 && a->d <= 64) {
-    const int eight = wave_rows<64, 8>();
-    const int64_t rounds8 = (pairs * groups(8, eight) + 255) / 256, rounds4 = (pairs * groups(4, rows) + 255) / 256;
-    if (5 * rounds8 < 4 * rounds4) {
-      p.waves = 8;
-      rows = eight;
-    }
+    const int64_t narrow = (pairs * groups(runs, rows) + 255) / 256;
+    const int64_t wide = (pairs * groups(WideShape::RUNS, WideShape::R) + 255) / 256;
+    p.wide = 11 * wide < 8 * narrow;
+    if (p.wide) runs = WideShape::RUNS, rows = WideShape::R;
   }
-  p.groups = (int)groups(p.waves, rows);
-  // the queries dealt evenly to the waves of all groups
-  p.queries = p.groups > 0 ? (a->Sq + p.groups * p.waves - 1) / (p.groups * p.waves) : 1;
+  p.groups = (int)groups(runs, rows);
+  // the queries dealt evenly to the runs of all workgroups
+  const int64_t all = (int64_t)p.groups * runs;
+  p.queries = all > 0 ? (int)((a->Sq + all - 1) / all) : 1;
   p.chunks = (a->Sq + p.queries - 1) / p.queries;
   // whole blocks of up to 64 keys together, or the largest equal part of a longer block
   p.stage = 16;
@@ -1084,24 +1110,24 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
   return p;
 }
 
-template <typename T, int D, int WAVES, bool BACK>
-int launch_chunk_waves(const BlocksParams& p, const GradParams& gp, unsigned blocks, hipStream_t st) {
-  constexpr int bytes = ChunkLds<D, WAVES>::bytes;
+template <typename T, int D, class S, bool BACK>
+int launch_shape(const BlocksParams& p, const GradParams& gp, unsigned blocks, hipStream_t st) {
+  constexpr int bytes = ChunkLds<D, S>::bytes;
   SHRIMP_REQUIRE(bytes <= max_lds_per_block(), "attn_blocks: %d bytes of LDS, %d available", bytes,
                  max_lds_per_block());
-  const dim3 grid(blocks), threads(WAVES * 64);
+  const dim3 grid(blocks), threads(S::WAVES * 64);
   if (p.shared)
-    hipLaunchKernelGGL((attn_blocks_kernel<T, D, WAVES, BACK, true>), grid, threads, bytes, st, p, gp);
+    hipLaunchKernelGGL((attn_blocks_kernel<T, D, S, BACK, true>), grid, threads, bytes, st, p, gp);
   else
-    hipLaunchKernelGGL((attn_blocks_kernel<T, D, WAVES, BACK, false>), grid, threads, bytes, st, p, gp);
+    hipLaunchKernelGGL((attn_blocks_kernel<T, D, S, BACK, false>), grid, threads, bytes, st, p, gp);
   return SHRIMP_OK;
 }
 
 template <typename T, int D, bool BACK>
 int launch_chunk(const BlocksParams& p, const GradParams& gp, unsigned blocks, hipStream_t st) {
   if constexpr (D == 64)
-    if (p.waves == 8) return launch_chunk_waves<T, D, 8, BACK>(p, gp, blocks, st);
-  return launch_chunk_waves<T, D, 4, BACK>(p, gp, blocks, st);
+    if (p.wide) return launch_shape<T, D, WideShape, BACK>(p, gp, blocks, st);
+  return launch_shape<T, D, NarrowShape<D>, BACK>(p, gp, blocks, st);
 }
 
 template <typename T, int D, int KT>

@@ -711,3 +711,27 @@ def test_sizes_that_would_wrap_are_refused():
                       [1])
     with pytest.raises(ValueError, match="means"):
         ops.block_select(k[:, :0], means, ql, kl, 16, 2)
+
+
+@pytest.mark.parametrize("block,d,dt", [(16, 64, torch.bfloat16), (32, 40, torch.float16), (48, 64, torch.bfloat16),
+                                        (64, 64, torch.float16)], ids=str)
+def test_many_workgroups(block, d, dt):
+    """Enough rows for the workgroups that take more of them at a time."""
+
+    b, h, sq, sk, topk = 50, 4, 257, 70, 2
+    gen = _gen(46)
+    q, k, v, g = (_heads(gen, b, h, n, d, dt) for n in (sq, sk, sk, sq))
+    ql, kl = [sq - i % 3 for i in range(b)], [sk - i for i in range(b)]
+    means = ops.block_means(k, _lens(*kl), block)
+    sel = ops.block_select(q, means, _lens(*ql), _lens(*kl), block, topk)
+    out, lse = _check_attend(q, k, v, sel, ql, kl, block)
+    _check_grads(q, k, v, sel, ql, kl, block, g, None)
+    # non-finite keys of one block stay with the rows that chose it; the others are within
+    # the bound of the same exact result (their blocks may be taken one by one: other sums)
+    want, ob, _, _ = _attend_want(*(t[:1, :1].cpu().double() for t in (q, k, v)), sel[:1, :1].cpu(), ql, kl, block, dt)
+    k[0, 0, 17] = float("inf")
+    again, _ = ops.attn_blocks(q, k, v, sel, _lens(*ql), _lens(*kl), block)
+    chose = (sel[0, 0] == 17 // block).any(-1).cpu()
+    assert torch.equal(again[1:], out[1:]) and torch.equal(again[0, 1:], out[0, 1:])
+    tol = ob + (want.abs() + ob) * torch.finfo(dt).eps / 2 + torch.finfo(dt).smallest_normal
+    assert ((again[0, 0].cpu().double() - want[0, 0]).abs() <= tol[0, 0])[~chose].all()
