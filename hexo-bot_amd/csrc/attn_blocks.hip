@@ -1166,10 +1166,14 @@ int64_t grad_mask_bytes(const shrimp_attn_blocks_args* a) {
   return mul_sat({a->B, a->Hk, ((int64_t)a->Sk + a->block - 1) / a->block, p.chunks, 8});
 }
 
-// Keys a workgroup of the dk / dv kernel takes: their two accumulators fill 128 registers.
+// Tiles of 16 keys that a workgroup of the dk / dv kernel takes: every row is gathered once
+// for all of them, but their two accumulators are registers. At D = 64 32 keys leave two
+// waves per SIMD (2 x 8 heads x 4096 in pairs, 8 blocks of 64: 84 us, 64 keys 92); at
+// D = 128 there is one either way (16 heads x 8192, 16 blocks of 64, the whole backward:
+// 1717 us, with 16 keys 2049).
 template <int D, int KT>
 constexpr int key_tiles() {
-  return D == 128 && KT == 4 ? 2 : KT;
+  return D >= 64 && KT == 4 ? 2 : KT;
 }
 
 template <typename T, int D, int KT>
