@@ -1084,9 +1084,8 @@ BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
   };
   int runs = 4, rows = a->d > 64 ? NarrowShape<128>::R : NarrowShape<64>::R;
   if (a->d > 32 && a->d <= 64) {
-    const int64_t narrow = (pairs * groups(runs, rows) + 255) / 256;
-    const int64_t wide = (pairs * groups(WideShape::RUNS, WideShape::R) + 255) / 256;
-    p.wide = 11 * wide < 8 * narrow;
+    auto rounds = [&](int64_t n) { return (mul_sat({pairs, n}) - 1) / 256 + 1; };
+    p.wide = rounds(groups(WideShape::RUNS, WideShape::R)) / 8.0 < rounds(groups(runs, rows)) / 11.0;
     if (p.wide) runs = WideShape::RUNS, rows = WideShape::R;
   }
   p.groups = (int)groups(runs, rows);
@@ -1133,13 +1132,13 @@ int launch_chunk(const BlocksParams& p, const GradParams& gp, unsigned blocks, h
 template <typename T, int D, int KT>
 int launch_forward(const BlocksParams& p, hipStream_t st) {
   if (p.Sq <= FEW_QUERIES) {
-    const int64_t n = (int64_t)p.B * p.Hk * p.Sq;
+    const int64_t n = mul_sat({p.B, p.Hk, p.Sq});
     SHRIMP_REQUIRE(n <= INT32_MAX, "attn_blocks: %lld queries", (long long)n);
     hipLaunchKernelGGL((attn_blocks_query_kernel<T, D, KT>), dim3((unsigned)n), dim3(QW * 64), 0, st, p);
     return SHRIMP_OK;
   }
   const int64_t pairs = (int64_t)p.B * p.Hk;
-  const int64_t n = (p.by_xcd ? (pairs + 7) / 8 * 8 : pairs) * p.groups;
+  const int64_t n = mul_sat({p.by_xcd ? (pairs + 7) / 8 * 8 : pairs, p.groups});
   SHRIMP_REQUIRE(n <= INT32_MAX, "attn_blocks: %lld groups of queries", (long long)n);
   return launch_chunk<T, D, false>(p, GradParams{}, (unsigned)n, st);
 }
@@ -1180,9 +1179,9 @@ template <typename T, int D, int KT>
 int launch_backward(const BlocksParams& p, GradParams gp, hipStream_t st) {
   constexpr int KG = key_tiles<D, KT>();
   const int64_t pairs = (int64_t)p.B * p.Hk, sets = p.by_xcd ? (pairs + 7) / 8 * 8 : pairs;
-  const int64_t n = sets * p.groups;
+  const int64_t n = mul_sat({sets, p.groups});
   gp.segments = (p.Sk + KG * 16 - 1) / (KG * 16);
-  const int64_t m = sets * gp.segments;
+  const int64_t m = mul_sat({sets, gp.segments});
   SHRIMP_REQUIRE(n <= INT32_MAX && m <= INT32_MAX, "attn_blocks_backward: %lld chunks of queries, %lld of keys",
                  (long long)n, (long long)m);
   if (n > 0) {

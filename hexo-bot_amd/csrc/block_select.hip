@@ -669,7 +669,7 @@ int means_launch(const void* k, int64_t sb, int64_t sh, int64_t sn, int dt, cons
   SHRIMP_REQUIRE(nb <= MAX_BLOCKS, "%s: %lld blocks, at most %d", what, (long long)nb, MAX_BLOCKS);
   if (B == 0 || Hk == 0 || nb == 0) return SHRIMP_OK;
   SHRIMP_REQUIRE(k && lens && means, "%s: null pointer", what);
-  const int64_t items = (int64_t)B * Hk * (last_only ? 1 : nb);
+  const int64_t items = mul_sat({B, Hk, last_only ? 1 : nb});
   SHRIMP_REQUIRE(items <= INT32_MAX, "%s: %lld blocks of keys", what, (long long)items);
   const int wide = 16 / dt_size(dt);
   // 16-byte accesses for long blocks; for short ones 8, which leave fewer lanes to add up
@@ -759,12 +759,12 @@ extern "C" int shrimp_block_select(const shrimp_block_select_args* a, void* stre
                  "block_select: null pointer");
   SHRIMP_REQUIRE(reinterpret_cast<uintptr_t>(a->means) % 16 == 0,
                  "block_select: means must start on a 16-byte boundary");
+  const int64_t rows = mul_sat({a->B, a->Hk, a->Sq});
+  SHRIMP_REQUIRE(rows <= INT32_MAX && a->Sq <= MAX_KEYS, "block_select: %lld queries", (long long)rows);
   SelectParams p{a->q, a->means, a->q_lens, a->k_lens, a->sel, a->q_sb, a->q_sh, a->q_sn,
                  a->B, a->H, a->Hk, a->Sq, a->Sk, a->D, (int)nb, a->block, a->topk, a->H / a->Hk,
                  (a->Sq + 15) / 16, 0, row_vec(4, a->q, a->q_sb, a->q_sh, a->q_sn, a->D, dt_size(a->dt))};
   p.chunk = nb < 128 ? (int)(nb + 15) / 16 * 16 : 128;
-  const int64_t rows = (int64_t)a->B * a->Hk * a->Sq;
-  SHRIMP_REQUIRE(rows <= INT32_MAX, "block_select: %lld queries", (long long)rows);
   // A tile of 16 queries takes a product's time however few of them there are.
   const bool by_row = a->Sq <= 2;
   const size_t row_lds = (MAX_D + nb) * 8;

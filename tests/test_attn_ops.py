@@ -105,7 +105,8 @@ def test_block_refusals(lib):
                       (dict(Hk=0), b"query heads"), (dict(H=3, Hk=2), b"query heads"), (dict(block=0), b"block of"),
                       (dict(Sk=5000, block=1), b"blocks"), (dict(sel=None), b"null"), (dict(means=None), b"null"),
                       (dict(H=0), b"query heads"), (dict(means=72), b"16-byte"), (dict(block=2**31 - 1), b"block of"),
-                      (dict(Sk=2**31 - 1, block=2**20), b"block of"), (dict(dt=5), b"element type"), (dict(Sq=-1), b"negative")):
+                      (dict(Sk=2**31 - 1, block=2**20), b"block of"), (dict(Sq=2**31 - 1), b"queries"),
+                      (dict(B=2**31 - 1, H=2**31 - 1, Hk=2**31 - 1, Sq=2**30), b"queries"), (dict(dt=5), b"element type"), (dict(Sq=-1), b"negative")):
         _refused(lib, select(**bad), text)
     assert select(Sq=0, q=None) == 0
 
@@ -146,6 +147,14 @@ def test_attn_blocks_refusals(lib):
     # no queries: the keys' gradients are still written, so their pointers are needed
     none = _attn(Sq=0, k=None)
     _refused(lib, lib.shrimp_attn_blocks_backward(ctypes.byref(none), ctypes.byref(grads()), None), b"null k")
+    for sq, text in ((3, b"queries"), (2**30, b"groups of queries")):
+        huge = _attn(B=2**31 - 1, H=2**31 - 1, Hk=2**31 - 1, Sq=sq)
+        _refused(lib, lib.shrimp_attn_blocks(ctypes.byref(huge), None), text)
+    many = _attn(B=2**16, H=2**16, Hk=2**16, Sq=64)
+    room = grads(workspace_bytes=2**62)
+    _refused(lib, lib.shrimp_attn_blocks_backward(ctypes.byref(many), ctypes.byref(room), None), b"chunks of queries")
+    _refused(lib, lib.shrimp_block_means(64, 64, 64, 64, _lib.DT_BF16, 64, 64, 2**31 - 1, 2**31 - 1, 100, 64, 1, 0, None),
+             b"blocks of keys")
     big = _attn(B=2**31 - 1, H=2**20, Hk=2**20, Sq=2**30)
     assert lib.shrimp_attn_blocks_workspace(ctypes.byref(big)) > 2**62  # saturated, not wrapped
 
