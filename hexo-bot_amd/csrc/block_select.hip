@@ -269,11 +269,17 @@ SHRIMP_DEV uint64_t lane_u64(uint64_t v, int lane) {  // (lane: wave-uniform)
          (unsigned)__builtin_amdgcn_readlane((int)v, lane);
 }
 
-SHRIMP_DEV unsigned row_max(unsigned v) {  // over the 16 lanes of a row, for all of them
-  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));
-  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
-  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));
-  return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));
+// The maxima over the 16 lanes of a row, for all of them: four side by side, a step of each
+// between the steps of another (a DPP read waits for the write before it).
+SHRIMP_DEV void row_max(unsigned (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = max(v[i], (unsigned)__builtin_amdgcn_mov_dpp((int)v[i], 0xB1, 0xF, 0xF, true));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = max(v[i], (unsigned)__builtin_amdgcn_mov_dpp((int)v[i], 0x4E, 0xF, 0xF, true));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = max(v[i], (unsigned)__builtin_amdgcn_mov_dpp((int)v[i], 0x141, 0xF, 0xF, true));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = max(v[i], (unsigned)__builtin_amdgcn_mov_dpp((int)v[i], 0x140, 0xF, 0xF, true));
 }
 
 template <int N>
@@ -410,8 +416,10 @@ __global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const 
   }
   for (int it = 0; it < p.topk; ++it) {
 #pragma unroll
+    for (int i = 0; i < 4; ++i) last[i] = key[i][0];
+    row_max(last);
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
-      last[i] = row_max(key[i][0]);
       const bool win = key[i][0] == last[i];
       chosen[i] |= win ? 1u << (NT - 1 - (last[i] >> 4 & (NT - 1))) : 0;
 #pragma unroll
@@ -421,10 +429,13 @@ __global__ __launch_bounds__(REG_WAVES * 64) void block_select_reg_kernel(const 
   }
   // Queries whose last and next key differ in their places only are decided by float64
   // scores, one query at a time (bit r of `open`: query r).
-  unsigned open = 0;
+  unsigned open = 0, then[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) then[i] = key[i][0];
+  row_max(then);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint64_t same = __ballot((row_max(key[i][0]) ^ last[i]) >> DROP == 0);
+    const uint64_t same = __ballot((then[i] ^ last[i]) >> DROP == 0);
 #pragma unroll
     for (int g = 0; g < 4; ++g) open |= (unsigned)(same >> (16 * g) & 1) << (4 * i + g);
   }
