@@ -13,6 +13,7 @@ where every line of Python costs three times as much.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB = torch.library.Library("shrimp", "FRAGMENT")
 
@@ -31,6 +32,10 @@ def define(schema: str, kernel, fake, function=None):
     if function is not None:
 
         def autograd(*args):
+            if forward_ad._current_level >= 0 and any(
+                isinstance(a, torch.Tensor) and forward_ad.unpack_dual(a).tangent is not None for a in args
+            ):
+                raise RuntimeError(f"shrimp::{name} has no forward-mode derivative")
             if torch.is_grad_enabled() and any(
                 isinstance(a, torch.Tensor) and a.requires_grad for a in args
             ):
@@ -43,9 +48,11 @@ def define(schema: str, kernel, fake, function=None):
 
 
 def direct(*tensors) -> bool:
-    """Plain tensors, no tracing and no dispatch mode: a kernel may be called as it is."""
+    """Plain tensors, no tracing, dispatch mode or forward-mode level: a kernel may be called
+    as it is."""
 
-    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack():
+    if (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack()
+            or forward_ad._current_level >= 0):
         return False
     for t in tensors:
         if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
