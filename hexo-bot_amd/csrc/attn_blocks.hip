@@ -295,6 +295,17 @@ struct GradParams {
   int nb, segments; // blocks; runs of keys per (sequence, key head)
 };
 
+// What p and ds are multiplied by before they are split in fp16 numbers, whose smallest step is
+// 2^-24: over thousands of keys both come near that order (4096 keys, incoming gradients of
+// 2^-6: dq and dk were 2.6e-3 off in the 2-norm, now 2.1e-4, their rounding). p <= 1 stays
+// below fp16's largest number; ds does up to 2000, past which the gradients of q and k
+// stop being finite.
+template <typename T>
+struct Up {
+  static constexpr bool HALF = std::is_same<T, _Float16>::value;
+  static constexpr float P_LOG2 = HALF ? 15.f : 0.f, P = HALF ? 0x1p15f : 1.f, DS = HALF ? 0x1p6f : 1.f;
+};
+
 template <typename T>
 SHRIMP_DEV float elem(unsigned word, int hi);
 template <>
@@ -664,7 +675,7 @@ __global__ __launch_bounds__(S::WAVES * 64, 1) void attn_blocks_kernel(const Blo
                 float w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                  w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], p.scale2, -st.x)) * gp.scale * (dp[i] - st.y);
+                  w[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], p.scale2, -st.x)) * (gp.scale * Up<T>::DS) * (dp[i] - st.y);
                 Mma<T>::split(w, hi[kt], lo[kt]);
               }
             } else {
@@ -715,7 +726,7 @@ __global__ __launch_bounds__(S::WAVES * 64, 1) void attn_blocks_kernel(const Blo
     const int query = row_query(p, r), head = r - query * p.group;
     const int64_t o = out0 + (int64_t)head * p.Sq + query;
     float2 st = *reinterpret_cast<const float2*>(acc0 + r * RF + D);
-    float mul0 = 1.f, mul1 = 1.f;
+    float mul0 = BACK ? 1.f / Up<T>::DS : 1.f, mul1 = mul0;
     if constexpr (!BACK) {
       if constexpr (TEAMS > 1) {
         const float2 so = *reinterpret_cast<const float2*>(acc1 + r * RF + D);
@@ -940,7 +951,7 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
             int query, head;
             locate(i, query, head);
             st[rt][j] = stat[(int64_t)head * p.Sq + query];
-            st[rt][j].x = i < count ? st[rt][j].x : INFINITY;
+            st[rt][j].x = i < count ? st[rt][j].x - Up<T>::P_LOG2 : INFINITY;
             qt[rt][j] = *reinterpret_cast<const Words<W>*>(q + (int64_t)head * p.q_sh + (int64_t)query * p.q_sn + c);
             gt[rt][j] = *reinterpret_cast<const Words<W>*>(g + (int64_t)head * gp.g_sh + (int64_t)query * gp.g_sn + c);
           }
@@ -965,7 +976,7 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.scale2, -st[rt][i].x));
-              x[i] = w[i] * gp.scale * (dp[i] - st[rt][i].y);
+              x[i] = w[i] * (gp.scale * (Up<T>::DS / Up<T>::P)) * (dp[i] - st[rt][i].y);
             }
             Mma<T>::split(w, ph[rt], pl[rt]);
             Mma<T>::split(x, dh[rt], dl[rt]);
@@ -1010,7 +1021,7 @@ __global__ __launch_bounds__(GW * 64) void attn_blocks_dkv_kernel(const BlocksPa
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int dim = c * 4 + e, rr = dim / EPL, ee = dim % EPL;
-      x[e] = sum[row * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3)];
+      x[e] = sum[row * RF + ((rr >> 2) * EPL + ee) * 4 + (rr & 3)] * (row < KT * 16 ? 1.f / Up<T>::DS : 1.f / Up<T>::P);
     }
     uint16_t* out = (row < KT * 16 ? gp.dk : gp.dv) + (bh * p.Sk + key) * p.d + c * 4;
     *reinterpret_cast<u32x2*>(out) = u32x2{Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3])};

@@ -379,6 +379,7 @@ def attn_blocks_backward(g: torch.Tensor, g_lse: Optional[torch.Tensor], q: torc
                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients of q, k and v from those of attn_blocks' results (that of lse may be None),
     its arguments and its results. Every sum has a fixed order: the same call gives the same
-    bits."""
+    bits. In float16 a score's gradient past 2000 makes those of q and k
+    not finite."""
 
     return _attn_blocks_backward(g, g_lse, q, k, v, sel, q_lens, k_lens, out, lse, block)

@@ -889,7 +889,8 @@ int shrimp_attn_blocks(const shrimp_attn_blocks_args* a, void* stream);
  * g (B, H, Sq, d) of type dt, the gradient of out (strides multiples of 8, 16-byte
  * aligned), and g_lse (B, H, Sq) fp32 contiguous, that of lse, or NULL. dq (B, H,
  * Sq, d), dk and dv (B, Hk, Sk, d) of type dt, contiguous, written whole (zeros
- * where nothing flows); every sum in a fixed order. workspace: at least
+ * where nothing flows); every sum in a fixed order; with SHRIMP_DT_F16 a score's gradient past
+ * 2000 leaves dq and dk not finite. workspace: at least
  * shrimp_attn_blocks_workspace(a) bytes (-1 for arguments it refuses), 8-byte
  * aligned, used only during the call's launches. */
 typedef struct {

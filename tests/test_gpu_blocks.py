@@ -735,3 +735,29 @@ def test_many_workgroups(block, d, dt):
     assert torch.equal(again[1:], out[1:]) and torch.equal(again[0, 1:], out[0, 1:])
     tol = ob + (want.abs() + ob) * torch.finfo(dt).eps / 2 + torch.finfo(dt).smallest_normal
     assert ((again[0, 0].cpu().double() - want[0, 0]).abs() <= tol[0, 0])[~chose].all()
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=str)
+def test_gradients_over_many_keys(dt):
+    """Weights and score gradients far below the type's smallest normal number. The results'
+    rounding alone is within H of each element, so of the norm; its mean square is a third of
+    that (eps / 2 over sqrt 3), and what the sums of two numbers add is far below the rest.
+    Results below the smallest normal number are off by half of its step."""
+
+    b, h, hk, sq, sk, d, block, topk = 1, 2, 1, 40, 4096, 64, 64, 64
+    gen = _gen(47)
+    q, k, v, g = (_heads(gen, b, n, s, d, dt) for n, s in ((h, sq), (hk, sk), (hk, sk), (h, sq)))
+    g = g * 2.0**-6
+    sel = torch.arange(64, dtype=torch.int32, device=DEV).expand(b, hk, sq, topk).contiguous()
+    x = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    out, _ = ops.attn_blocks(*x, sel, _lens(sq), _lens(sk), block)
+    got = torch.autograd.grad(out, x, g)
+    y = [t.detach().cpu().double().requires_grad_() for t in (q, k, v)]
+    p = torch.softmax(y[0] @ y[1].transpose(2, 3) / math.sqrt(d), -1)
+    # delta = g . out with out as it was rounded
+    want_v = p.transpose(2, 3) @ g.cpu().double()
+    ds = p * (g.cpu().double() @ y[2].transpose(2, 3) - (g.double() * out.detach().double()).sum(-1, keepdim=True).cpu()) / math.sqrt(d)
+    want = ds @ y[1], (ds.transpose(2, 3) @ y[0]).sum(1, keepdim=True), want_v.sum(1, keepdim=True)
+    for name, a, e in zip("qkv", got, want):
+        tiny = torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2 * math.sqrt(e.numel())
+        assert (a.cpu().double() - e).norm() <= torch.finfo(dt).eps / 2 * e.norm() + tiny, name
