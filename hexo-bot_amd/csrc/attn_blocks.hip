@@ -1068,7 +1068,7 @@ int check_blocks(const shrimp_attn_blocks_args* a, bool back, const char* what) 
 // 16 that divide a block.
 int key_step(int block) { return block % 64 == 0 ? 64 : block % 32 == 0 ? 32 : 16; }
 
-BlocksParams blocks_params(const shrimp_attn_blocks_args* a, bool back) {
+BlocksParams blocks_params(const shrimp_attn_blocks_args* a) {
   BlocksParams p{};
   p.q = static_cast<const uint16_t*>(a->q);
   p.k = static_cast<const uint16_t*>(a->k);
@@ -1172,7 +1172,7 @@ int64_t grad_stat_bytes(const shrimp_attn_blocks_args* a) {
   return mul_sat({a->B, a->H, a->Sq, 8});
 }
 int64_t grad_mask_bytes(const shrimp_attn_blocks_args* a) {
-  const BlocksParams p = blocks_params(a, true);
+  const BlocksParams p = blocks_params(a);
   return mul_sat({a->B, a->Hk, ((int64_t)a->Sk + a->block - 1) / a->block, p.chunks, 8});
 }
 
@@ -1232,7 +1232,7 @@ extern "C" int shrimp_attn_blocks(const shrimp_attn_blocks_args* a, void* stream
   const int rc = check_blocks(a, false, "attn_blocks");
   if (rc != SHRIMP_OK) return rc;
   if (a->B == 0 || a->H == 0 || a->Sq == 0) return SHRIMP_OK;
-  const BlocksParams p = blocks_params(a, false);
+  const BlocksParams p = blocks_params(a);
   const int e = a->dt == SHRIMP_DT_F16 ? launch_forward_d<_Float16>(p, as_stream(stream))
                                        : launch_forward_d<__bf16>(p, as_stream(stream));
   if (e != SHRIMP_OK) return e;
@@ -1265,7 +1265,7 @@ extern "C" int shrimp_attn_blocks_backward(const shrimp_attn_blocks_args* a,
                      (g->workspace || stat + mask == 0) && reinterpret_cast<uintptr_t>(g->workspace) % 8 == 0,
                  "attn_blocks_backward: workspace of %lld bytes, %lld + %lld needed",
                  (long long)g->workspace_bytes, (long long)stat, (long long)mask);
-  BlocksParams p = blocks_params(a, true);
+  BlocksParams p = blocks_params(a);
   if (!rows) p.groups = p.chunks = 0;  // (no heads: the keys' gradients are zero)
   GradParams gp{};
   gp.g = static_cast<const uint16_t*>(g->g);

@@ -52,7 +52,7 @@ def direct(*tensors) -> bool:
     as it is."""
 
     if (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack()
-            or forward_ad._current_level >= 0):
+            or forward_ad._current_level >= 0 or torch._C._is_tracing()):
         return False
     for t in tensors:
         if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:

@@ -70,6 +70,22 @@ def test_compiled(data):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_traced(data):
+    """A traced program holds the operators, not the results of the traced call."""
+
+    q, k, v, w, fr, pos, ql, kl = data
+
+    def run(q, k, v):
+        qn, kn = ops.qk_norm_rope(q, k, w, w, pos, fr, [D // 2])
+        sel = ops.block_select(qn, ops.block_means(kn, kl, BLOCK), ql, kl, BLOCK, TOPK)
+        return ops.attn_blocks(ops.rope_axes(qn, pos, fr, [D // 2]), kn, v, sel, ql, kl, BLOCK)
+
+    with torch.no_grad():
+        traced = torch.jit.trace(run, (q, k, v))
+        for a, b in zip(traced(q.flip(2), k * 0.5, v.flip(2)), run(q.flip(2), k * 0.5, v.flip(2))):
+            assert torch.equal(a, b)
+
+
 def test_streams_and_threads_at_once(data):
     layer = _layer(data)
     want = _grads(layer, data)
